@@ -66,6 +66,13 @@ typedef enum {
 #define SSA_DEVICE_INDEX_FULL 0x8  /* decode index: a bucket had no free slot; the
                                       entry was dropped (rebuild before appending
                                       more keys than min_free allows)               */
+#define SSA_DEVICE_BAD_PAGE 0x10   /* paged cache: a page table entry of a used slot is
+                                      outside [0, num_pages); the slot is not written,
+                                      and what is computed from it is undefined       */
+#define SSA_DEVICE_BAD_LENGTH 0x20 /* paged cache: q_starts does not ascend within
+                                      [0, rows], a length is outside its table, or more
+                                      rows are appended than the sequence holds; the
+                                      sequence is skipped                             */
 #define SSA_DEVICE_TIMEOUT 0x100   /* route: a pipeline wait gave up (~1 s); the
                                       affected codes are undefined                  */
 
@@ -314,6 +321,82 @@ ssa_status ssa_sparse_attn_segments(const SsaAttnArgs* args, const SsaQuerySegme
  * order of the adds).  Indices receive no gradient. */
 ssa_status ssa_sparse_attn_backward(const SsaAttnArgs* args, const void* d_out, void* d_q, float* d_k,
                                     float* d_v, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Paged key/value cache                                                      */
+/* ------------------------------------------------------------------------ */
+/* Keys and values of `batch` sequences in pages of page_size slots: slot j of
+ * sequence s lies in page page_table[s * table_stride + j / page_size] at row
+ * j % page_size.  kv_lens[s] slots of it are filled.  The reference keeps no
+ * cache; these entry points serve the dense layers, prompts and comparisons
+ * that run next to its sparse attention. */
+typedef struct {
+  int32_t batch;
+  int32_t max_pages;          /* columns of page_table                          */
+  int32_t page_size;          /* 1..1024 slots                                   */
+  int32_t h_kv, d;            /* d: a multiple of 8 in [8, 256]                  */
+  ssa_dtype dtype;            /* k_pages and v_pages                             */
+  int64_t num_pages;
+  void* k_pages; int64_t k_stride_p, k_stride_n, k_stride_h;  /* [num_pages, page_size, h_kv, d] */
+  void* v_pages; int64_t v_stride_p, v_stride_n, v_stride_h;
+  float* weights; int64_t w_stride_p, w_stride_n, w_stride_h; /* [num_pages, page_size, h_kv], NULL: none */
+  const int32_t* page_table; int64_t table_stride;            /* [batch, max_pages]   */
+  const int32_t* kv_lens;                                     /* [batch]              */
+  int32_t* status;            /* optional word that device code can write (device
+                                 memory or mapped host memory), SSA_DEVICE_* bits     */
+} SsaPagedCache;
+
+/* A chunk of new rows of the sequences: rows q_starts[s] .. q_starts[s+1]-1
+ * are sequence s's, and stand at its last slots (kv_lens counts them). */
+typedef struct {
+  int64_t rows;
+  const int32_t* q_starts;    /* [batch + 1], ascending from 0 to rows          */
+  const void* k_new; int64_t k_new_stride_n, k_new_stride_h;  /* [rows, h_kv, d] */
+  const void* v_new; int64_t v_new_stride_n, v_new_stride_h;
+} SsaPagedAppendArgs;
+
+/* Writes the new rows to their slots and zeroes the slots' weights. */
+ssa_status ssa_paged_append(const SsaPagedCache* cache, const SsaPagedAppendArgs* args, void* stream);
+
+typedef struct {
+  int64_t rows;
+  const int32_t* q_starts;    /* [batch + 1], ascending from 0 to rows          */
+  int32_t h_q;                /* h_q % h_kv == 0, h_q / h_kv <= 16              */
+  int32_t causal;             /* 1: row i of n sees the slots j <= kv_len - n + i */
+  float scale;                /* logits = (q . k) / scale                       */
+  const void* q; int64_t q_stride_n, q_stride_h;              /* [rows, h_q, d]  */
+  void* out; int64_t out_stride_n, out_stride_h;              /* [rows, h_q, d]  */
+  float* lse;                 /* optional [rows, h_q]: log of the row's sum of exponentials */
+} SsaPagedAttnArgs;
+
+size_t ssa_paged_attn_workspace_size(const SsaPagedCache* cache, const SsaPagedAttnArgs* args);
+
+/* Softmax attention of the new rows over what their sequences have cached.
+ * With cache->weights, every slot's weight grows by the attention it
+ * received: the sum over the sequence's new rows and the heads of the group.
+ * A row that sees no slot gets a zero output row and lse = -inf.  A page that
+ * several sequences of the call share collects the weight of all of them, in
+ * an unspecified order of additions; every other result is the same from
+ * call to call. */
+ssa_status ssa_paged_attn(const SsaPagedCache* cache, const SsaPagedAttnArgs* args, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+typedef struct {
+  int32_t budget;             /* slots a (sequence, KV head) keeps at most: >= 1  */
+  int32_t recent;             /* its last slots, kept in any case: 0..budget     */
+  int32_t new_max_pages;
+  const int32_t* new_table; int64_t new_table_stride;  /* [batch, new_max_pages]  */
+  int32_t* kept;              /* [batch, h_kv, budget] slots kept, ascending, then -1 */
+  int32_t* new_lens;          /* [batch]: min(kv_len, budget)                    */
+} SsaPagedEvictArgs;
+
+/* Every (sequence, KV head) keeps min(kv_len, budget) slots: the last `recent`
+ * and the heaviest of the others by cache->weights (the lower slot first
+ * among equal weights; NaN ranks below every number).  Keys, values and
+ * weights of the kept slots are copied in order to the first slots of the
+ * pages of new_table, which must not be pages the call reads from: pages that
+ * sequences share stay whole. */
+ssa_status ssa_paged_evict(const SsaPagedCache* cache, const SsaPagedEvictArgs* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Test hooks (bit-exact parity on caller-provided inputs)                   */

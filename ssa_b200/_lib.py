@@ -20,6 +20,8 @@ SSA_DEVICE_INDEX_OOB = 0x1
 SSA_DEVICE_BAD_CODE = 0x2
 SSA_DEVICE_BAD_INDEX = 0x4
 SSA_DEVICE_INDEX_FULL = 0x8
+SSA_DEVICE_BAD_PAGE = 0x10
+SSA_DEVICE_BAD_LENGTH = 0x20
 SSA_DEVICE_TIMEOUT = 0x100
 STATUS_NAMES = {0: "SSA_OK", 1: "SSA_ERR_INVALID_ARG", 2: "SSA_ERR_UNSUPPORTED", 3: "SSA_ERR_WORKSPACE",
                 4: "SSA_ERR_ALIGNMENT", 5: "SSA_ERR_CUDA", 6: "SSA_ERR_DEVICE"}
@@ -81,6 +83,40 @@ class SsaDecodeIndex(ctypes.Structure):
     ]
 
 
+class SsaPagedCache(ctypes.Structure):
+    _fields_ = [
+        ("batch", _c_i32), ("max_pages", _c_i32), ("page_size", _c_i32), ("h_kv", _c_i32), ("d", _c_i32),
+        ("dtype", _c_i32), ("num_pages", _c_i64),
+        ("k_pages", _vp), ("k_stride_p", _c_i64), ("k_stride_n", _c_i64), ("k_stride_h", _c_i64),
+        ("v_pages", _vp), ("v_stride_p", _c_i64), ("v_stride_n", _c_i64), ("v_stride_h", _c_i64),
+        ("weights", _vp), ("w_stride_p", _c_i64), ("w_stride_n", _c_i64), ("w_stride_h", _c_i64),
+        ("page_table", _vp), ("table_stride", _c_i64), ("kv_lens", _vp), ("status", _vp),
+    ]
+
+
+class SsaPagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _c_i64), ("q_starts", _vp),
+        ("k_new", _vp), ("k_new_stride_n", _c_i64), ("k_new_stride_h", _c_i64),
+        ("v_new", _vp), ("v_new_stride_n", _c_i64), ("v_new_stride_h", _c_i64),
+    ]
+
+
+class SsaPagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _c_i64), ("q_starts", _vp), ("h_q", _c_i32), ("causal", _c_i32), ("scale", ctypes.c_float),
+        ("q", _vp), ("q_stride_n", _c_i64), ("q_stride_h", _c_i64),
+        ("out", _vp), ("out_stride_n", _c_i64), ("out_stride_h", _c_i64), ("lse", _vp),
+    ]
+
+
+class SsaPagedEvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("budget", _c_i32), ("recent", _c_i32), ("new_max_pages", _c_i32),
+        ("new_table", _vp), ("new_table_stride", _c_i64), ("kept", _vp), ("new_lens", _vp),
+    ]
+
+
 # exported symbol -> (restype, argtypes)
 SIGNATURES = {
     "ssa_decode_index_capacity": (_c_i64, [_c_i32, _c_i32, _c_i32, _c_i32]),
@@ -112,6 +148,12 @@ SIGNATURES = {
     "ssa_select_candidates_segments": (ctypes.c_int, [ctypes.POINTER(SsaRouteArgs),
                                                       ctypes.POINTER(SsaQuerySegments), _vp, _vp, _vp,
                                                       ctypes.c_size_t, _vp]),
+    "ssa_paged_append": (ctypes.c_int, [ctypes.POINTER(SsaPagedCache), ctypes.POINTER(SsaPagedAppendArgs), _vp]),
+    "ssa_paged_attn_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(SsaPagedCache),
+                                                        ctypes.POINTER(SsaPagedAttnArgs)]),
+    "ssa_paged_attn": (ctypes.c_int, [ctypes.POINTER(SsaPagedCache), ctypes.POINTER(SsaPagedAttnArgs), _vp,
+                                      ctypes.c_size_t, _vp]),
+    "ssa_paged_evict": (ctypes.c_int, [ctypes.POINTER(SsaPagedCache), ctypes.POINTER(SsaPagedEvictArgs), _vp]),
     "ssa_status_str": (ctypes.c_char_p, [ctypes.c_int]),
     "ssa_last_error": (ctypes.c_char_p, []),
 }

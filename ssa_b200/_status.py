@@ -19,11 +19,17 @@ never waits for the GPU on the fast path.  ``SSA_CHECKED=sync`` reads the
 word right after each op (one host synchronisation per op, the error raised
 by the failing call itself); ``SSA_CHECKED=0`` passes no status word at all.
 Inside a CUDA graph capture no word is used.
+
+The paged-cache ops, called once per layer and token, are too short for a
+copy, a reset and an event each.  Their kernels write an error straight into a
+word of mapped pinned host memory, one per op and device, which later op calls
+read as plain memory (:func:`poll`); it is valid inside a graph capture too.
 """
 
 from __future__ import annotations
 
 import collections
+import ctypes
 import os
 import threading
 from typing import Callable, Optional
@@ -73,6 +79,8 @@ def _ring(dev: torch.device) -> _Ring:
 def poll(dev: torch.device) -> None:
     """Raise for the first finished op whose status word came back non-zero
     (does not wait for the GPU)."""
+    if _words:
+        _poll_words(dev)
     if not _rings:
         return
     with _lock:
@@ -81,6 +89,59 @@ def poll(dev: torch.device) -> None:
             err = r._resolve(r.pending.popleft())
             if err is not None:
                 raise err
+
+
+class _HostWords:
+    """One word of mapped pinned memory per paged-cache op of one device."""
+
+    OPS = ("paged_append", "paged_attention", "paged_evict")
+
+    def __init__(self):
+        self.host = torch.zeros(len(self.OPS), dtype=torch.int32).pin_memory()
+        self.base = self.host.data_ptr()
+        self.view = (ctypes.c_int32 * len(self.OPS)).from_address(self.base)
+        self.used = False
+
+
+_words = {}
+
+
+def _device_index(dev: torch.device) -> int:
+    return dev.index if dev.index is not None else torch.cuda.current_device()
+
+
+def host_word(dev: torch.device, op: int) -> Optional[int]:
+    """Address of the error word of op number ``op`` (in ``_HostWords.OPS``), or
+    None with ``SSA_CHECKED=0``; raises for an error already found."""
+    if mode() == "off":
+        return None
+    key = _device_index(dev)
+    w = _words.get(key)
+    if w is None:
+        with _lock:
+            w = _words.setdefault(key, _HostWords())
+    elif any(w.view):
+        _poll_words(dev)
+    w.used = True
+    return w.base + 4 * op
+
+
+def host_word_done(dev: torch.device) -> None:
+    """After the launch: with ``SSA_CHECKED=sync`` wait for it and raise now."""
+    if mode() == "sync" and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(dev).synchronize()
+        _poll_words(dev)
+
+
+def _poll_words(dev: torch.device) -> None:
+    w = _words.get(_device_index(dev))
+    if w is None:
+        return
+    for i, op in enumerate(w.OPS):
+        bits = w.view[i]
+        if bits:
+            w.view[i] = 0
+            raise paged_error(op, bits)
 
 
 class Slot:
@@ -138,6 +199,11 @@ def release(slot: Optional[Slot], op: str, decode: Callable[[str, int], Optional
 def check_errors(device=None) -> None:
     """Wait for every op launched so far on ``device`` (default: all devices
     with pending words) and raise for the first error a kernel reported."""
+    for key, w in list(_words.items()):
+        if w.used and (device is None or key == _device_index(torch.device(device))):
+            torch.cuda.synchronize(key)
+            w.used = False
+            _poll_words(torch.device("cuda", key))
     with _lock:
         rings = list(_rings.values()) if device is None else [_ring(torch.device(device))]
         first = None
@@ -170,4 +236,14 @@ def route_error(op: str, bits: int) -> Optional[Exception]:
 def attn_error(op: str, bits: int) -> Optional[Exception]:
     if bits & L.SSA_DEVICE_INDEX_OOB:
         return IndexError(f"{op}: an index is outside [0, seq_len)")
+    return RuntimeError(f"{op}: device status 0x{bits:x}")
+
+
+def paged_error(op: str, bits: int) -> Exception:
+    if bits & L.SSA_DEVICE_BAD_PAGE:
+        return IndexError(f"{op}: a page table entry is outside [0, num_pages)")
+    if bits & L.SSA_DEVICE_BAD_LENGTH:
+        return ValueError(f"{op}: q_starts or a length does not fit the rows and the page table")
+    if bits & L.SSA_DEVICE_TIMEOUT:
+        return RuntimeError(f"{op}: a device pipeline wait timed out; results are undefined")
     return RuntimeError(f"{op}: device status 0x{bits:x}")

@@ -4,43 +4,18 @@
 // launches the stage kernels on the caller's stream.  It never allocates.
 #include <algorithm>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <string>
 
+#include "abi_util.cuh"
 #include "common.cuh"
 #include "kernels.cuh"
 
 namespace {
 
-thread_local std::string g_last_error;
-
-ssa_status fail(ssa_status s, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-ssa_status fail(ssa_status s, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return s;
-}
-
-ssa_status cuda_status(cudaError_t e, const char* what) {
-  if (e == cudaSuccess) return SSA_OK;
-  return fail(SSA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-size_t elem_size(ssa_dtype t) { return t == SSA_F32 ? 4 : 2; }
-bool valid_dtype(ssa_dtype t) { return t == SSA_F32 || t == SSA_BF16 || t == SSA_F16; }
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool stride16(int64_t s, ssa_dtype t) { return (s * static_cast<int64_t>(elem_size(t))) % 16 == 0; }
-
-constexpr size_t kAlign = 256;
-size_t round_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+using namespace ssa::abi;
 
 constexpr int kMaxCap = 16384;   // shared-memory candidate capacity limit
 

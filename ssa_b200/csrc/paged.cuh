@@ -1,0 +1,302 @@
+// The paged key/value cache: parameter blocks, launchers, and the division of
+// attention work over CTAs that its kernels share.  Internal.
+//
+// Attention work is a line of units.  An item is (sequence, KV head, tile of
+// query rows): the g heads of a KV group at `tokens` consecutive new tokens
+// are the rows of one tile.  Its units are the key tiles of KT slots its last
+// row sees (one unit where it sees none, so that its zero rows are written).
+// Items follow one another by sequence, head, tile.  CTA c of G takes units
+// [c W / G, (c + 1) W / G) of the W there are, whatever the lengths of the
+// batch: ragged batches and long contexts of few rows spread evenly, with no
+// plan made on the host.  An item cut by a CTA boundary leaves partial results
+// (running maximum, sum, unnormalised rows) that combine_kernel joins in CTA
+// order, so results do not depend on timing.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace ssa {
+
+struct PagedCacheParams {
+  const void* k; int64_t k_sp, k_sn, k_sh;
+  const void* v; int64_t v_sp, v_sn, v_sh;
+  float* w; int64_t w_sp, w_sn, w_sh;
+  const int32_t* table; int64_t table_stride;
+  const int32_t* kv_lens;
+  int32_t* status;
+  int64_t num_pages;
+  int batch, max_pages, page_size, page_shift, h_kv, d;   // page_shift: log2(page_size), -1 if no power of two
+};
+
+struct PagedAppendParams {
+  PagedCacheParams c;
+  const int32_t* q_starts;
+  const void* k_new; int64_t kn_sn, kn_sh;
+  const void* v_new; int64_t vn_sn, vn_sh;
+  int64_t rows;
+};
+
+// What a CTA leaves about the item its first unit belongs to.
+struct PagedSplit {
+  int64_t item_first;              // the item's first unit
+  int32_t seq, head, tile;
+  int32_t cta_first, cta_last;     // the CTAs that hold its first and its last unit
+  int32_t valid;                   // 0: the CTA had no unit
+};
+
+struct PagedAttnParams {
+  PagedCacheParams c;
+  const int32_t* q_starts;
+  const void* q; int64_t q_sn, q_sh;
+  void* out; int64_t o_sn, o_sh;
+  float* lse;                      // [rows, h_q] or NULL
+  float* lse2;                     // [rows, h_q] row log2-sum-exp2 for the weights pass, or NULL
+  float* part;                     // [grid][2][tile rows][d + 2]: unnormalised row, maximum (log2), sum
+  PagedSplit* split;               // [grid]
+  int64_t rows;
+  int group, causal;
+  float inv_scale;
+};
+
+struct PagedEvictParams {
+  PagedCacheParams c;
+  const int32_t* new_table; int64_t new_table_stride;
+  int32_t* kept;
+  int32_t* new_lens;
+  int new_max_pages, budget, recent;
+};
+
+// A run-time error word: plain stores, so that it may be mapped host memory.
+__device__ __forceinline__ void paged_error(const PagedCacheParams& c, int32_t bits) {
+  if (c.status) *reinterpret_cast<volatile int32_t*>(c.status) = bits;
+}
+
+__device__ __forceinline__ void page_of(const PagedCacheParams& c, int slot, int& page, int& row) {
+  if (c.page_shift >= 0) {
+    page = slot >> c.page_shift;
+    row = slot & (c.page_size - 1);
+  } else {
+    page = slot / c.page_size;
+    row = slot - page * c.page_size;
+  }
+}
+
+// Page of a slot below the sequence's length; -1 where the table is wrong.
+__device__ __forceinline__ int64_t physical_page(const PagedCacheParams& c, const int32_t* table, int64_t stride,
+                                                 int seq, int page) {
+  const int32_t pg = table[static_cast<int64_t>(seq) * stride + page];
+  if (pg < 0 || pg >= c.num_pages) {
+    paged_error(c, SSA_DEVICE_BAD_PAGE);
+    return -1;
+  }
+  return pg;
+}
+
+// New rows [q0, q0 + n) and length of a sequence; n = 0 where they are wrong.
+struct PagedSeq {
+  int64_t q0;
+  int n, len;
+};
+__device__ __forceinline__ int paged_len(const PagedCacheParams& c, int s) {
+  const int len = c.kv_lens[s];
+  if (len < 0 || len > static_cast<int64_t>(c.max_pages) * c.page_size) {
+    paged_error(c, SSA_DEVICE_BAD_LENGTH);
+    return -1;
+  }
+  return len;
+}
+__device__ __forceinline__ PagedSeq paged_seq(const PagedCacheParams& c, const int32_t* q_starts, int64_t rows,
+                                              int s) {
+  const int q0 = q_starts[s], q1 = q_starts[s + 1];
+  PagedSeq r;
+  r.len = paged_len(c, s);
+  if (q0 < 0 || q1 < q0 || q1 > rows) {
+    paged_error(c, SSA_DEVICE_BAD_LENGTH);
+    r.len = -1;
+  }
+  r.q0 = q0;
+  r.n = r.len < 0 ? 0 : q1 - q0;
+  return r;
+}
+
+// sum_{i < n} floor((a i + b) / m) for non-negative a, b, n and m > 0, by the
+// Euclidean reduction of lattice points under a line.
+__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t ans = 0;
+  while (n > 0) {
+    if (a >= m) {
+      ans += n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      ans += n * (b / m);
+      b %= m;
+    }
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return ans;
+}
+
+// The tiles of one sequence: `tiles` of them, `tt` tokens each, and their units.
+struct TileCosts {
+  int n, len, tt, kt, causal, tiles;
+  __host__ __device__ TileCosts(int n_, int len_, int tt_, int kt_, int causal_)
+      : n(n_), len(len_), tt(tt_), kt(kt_), causal(causal_), tiles(n_ > 0 ? (n_ + tt_ - 1) / tt_ : 0) {}
+  // slots the tile's last row sees
+  __host__ __device__ int seen(int r) const {
+    if (!causal) return len;
+    const int64_t last = static_cast<int64_t>(r + 1) * tt < n ? static_cast<int64_t>(r + 1) * tt : n;
+    const int64_t e = static_cast<int64_t>(len) - n + last;
+    return e > 0 ? static_cast<int>(e) : 0;
+  }
+  __host__ __device__ int units(int r) const {
+    const int u = (seen(r) + kt - 1) / kt;
+    return u > 0 ? u : 1;
+  }
+  // units of tiles 0 .. r-1
+  __host__ __device__ int64_t before(int r) const {
+    if (!causal) return static_cast<int64_t>(r) * units(0);
+    int64_t extra = 0;
+    if (r == tiles && r > 0) {                 // the last tile may be short
+      extra = units(r - 1);
+      --r;
+    }
+    // tile i < tiles - 1 sees base + (i + 1) tt slots; one unit while that is at most kt
+    const int64_t base = static_cast<int64_t>(len) - n;
+    int64_t one = base >= kt ? 0 : (kt - base) / tt;
+    if (one > r) one = r;
+    return extra + one + floor_sum(r - one, kt, tt, base + (one + 1) * tt + kt - 1);
+  }
+  // the tile unit u (of the sequence's units of one head) lies in
+  __host__ __device__ int find(int64_t u) const {
+    int lo = 0, hi = tiles - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before(mid) <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
+
+// A CTA's walk over its units: the current item, and the unit in it.
+struct PagedWalk {
+  int64_t total, ctas;             // all units, and the CTAs that share them
+  int64_t u, end;                  // next unit and the CTA's last + 1
+  int64_t item_first;              // first unit of the current item
+  int64_t q0;
+  int seq, head, tile, n, len, units;   // units: of the current item
+};
+
+// Total units, and the walk of CTA `cta` of `grid` (CTAs of less than
+// `min_units` each are not made: the rest stay idle).  Called by one full
+// warp; every lane gets the result.  False: no work.
+__device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int min_units, int64_t cta,
+                                      int64_t grid, PagedWalk& w) {
+  const int lane = threadIdx.x & 31;
+  const int hk = p.c.h_kv;
+  int64_t mine = 0;
+  for (int s = lane; s < p.c.batch; s += 32) {
+    const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, s);
+    const TileCosts t(q.n, q.len, tt, kt, p.causal);
+    mine += t.before(t.tiles) * hk;
+  }
+  int64_t total = mine;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  int64_t ctas = (total + min_units - 1) / min_units;
+  if (ctas > grid) ctas = grid;
+  w.total = total;
+  w.ctas = ctas;
+  if (cta >= ctas) return false;
+  w.u = cta * total / ctas;
+  w.end = (cta + 1) * total / ctas;
+  // the sequence holding unit w.u: running totals over groups of 32 sequences
+  int64_t base = 0;
+  for (int s0 = 0;; s0 += 32) {
+    const int s = s0 + lane;
+    int64_t cost = 0;
+    PagedSeq q{0, 0, 0};
+    if (s < p.c.batch) {
+      q = paged_seq(p.c, p.q_starts, p.rows, s);
+      const TileCosts t(q.n, q.len, tt, kt, p.causal);
+      cost = t.before(t.tiles) * hk;
+    }
+    int64_t incl = cost;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + incl > w.u);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      int64_t first = base + incl - cost;
+      first = __shfl_sync(0xffffffffu, first, src);
+      w.seq = s0 + src;
+      w.n = __shfl_sync(0xffffffffu, q.n, src);
+      w.len = __shfl_sync(0xffffffffu, q.len, src);
+      w.q0 = __shfl_sync(0xffffffffu, q.q0, src);
+      const TileCosts t(w.n, w.len, tt, kt, p.causal);
+      const int64_t per = t.before(t.tiles), off = w.u - first;
+      w.head = static_cast<int>(off / per);
+      const int64_t in_head = off - w.head * per;
+      w.tile = t.find(in_head);
+      w.item_first = first + w.head * per + t.before(w.tile);
+      w.units = t.units(w.tile);
+      return true;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+    if (s0 + 32 >= p.c.batch) return false;   // not reached: w.u < total
+  }
+}
+
+// The item after the current one (w.u is its first unit).  Every lane of a
+// warp, or a single thread, may call it: no exchange between lanes.
+__device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt, PagedWalk& w) {
+  w.item_first += w.units;
+  TileCosts t(w.n, w.len, tt, kt, p.causal);
+  if (++w.tile >= t.tiles) {
+    w.tile = 0;
+    if (++w.head >= p.c.h_kv) {
+      w.head = 0;
+      do {
+        if (++w.seq >= p.c.batch) return;
+        const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, w.seq);
+        w.n = q.n;
+        w.len = q.len;
+        w.q0 = q.q0;
+      } while (w.n == 0);
+      t = TileCosts(w.n, w.len, tt, kt, p.causal);
+    }
+  }
+  w.units = t.units(w.tile);
+}
+
+// The CTA that holds unit u: the last c with floor(c W / G) <= u.
+__device__ __forceinline__ int unit_cta(const PagedWalk& w, int64_t u) {
+  return static_cast<int>(((u + 1) * w.ctas - 1) / w.total);
+}
+__device__ __forceinline__ PagedSplit paged_split(const PagedWalk& w) {
+  return PagedSplit{w.item_first, w.seq, w.head, w.tile, unit_cta(w, w.item_first),
+                    unit_cta(w, w.item_first + w.units - 1), 1};
+}
+
+__host__ __device__ inline int tile_tokens(int tile_rows, int group) { return tile_rows / group; }
+
+cudaError_t launch_paged_append(const PagedAppendParams& p, ssa_dtype dt, cudaStream_t st);
+cudaError_t launch_paged_evict(const PagedEvictParams& p, ssa_dtype dt, cudaStream_t st);
+// Attention on the CUDA cores: every type, head size and page size.
+size_t paged_attn_simt_workspace(const PagedAttnParams& p);
+cudaError_t launch_paged_attn_simt(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st);
+
+}  // namespace ssa

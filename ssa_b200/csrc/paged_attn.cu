@@ -1,0 +1,451 @@
+// Attention over the paged cache on the CUDA cores: every type, head size up
+// to 256 and page size, in fp32 throughout; the join of split items; and the
+// slot weights.
+//
+//   s_ij = (q_i . k_j) / scale,  p_ij = exp(s_ij - m_i),  out_i = sum_j p_ij v_j / sum_j p_ij
+//
+// with the running maximum m_i and sum of the online softmax, in base 2
+// (s * log2 e is folded into q when it is loaded).  One CTA holds a tile of R
+// query rows (the g heads of a KV group at R / g consecutive tokens) and walks
+// key tiles of 64 slots: 256 threads form a 16 x 16 grid, a thread owns R / 16
+// rows and every 16th key (scores) or column quad (output).
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "paged.cuh"
+
+namespace ssa {
+namespace {
+
+constexpr int kKT = 64;            // slots per key tile
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Rows of the item's tile: row r is token tile * tt + r / g, head h * g + r % g.
+struct TileRows {
+  int tok0, rows;
+};
+__device__ __forceinline__ TileRows tile_rows(const PagedWalk& w, int tt, int group) {
+  TileRows t;
+  t.tok0 = w.tile * tt;
+  t.rows = min(tt, w.n - t.tok0) * group;
+  return t;
+}
+// Slots the row of token `tok` sees.
+__device__ __forceinline__ int seen_slots(const PagedAttnParams& p, int n, int len, int tok) {
+  return p.causal ? max(len - n + tok + 1, 0) : len;
+}
+
+// lse of a row from its maximum (base 2) and sum; -inf for a row that saw nothing.
+__device__ __forceinline__ void store_lse(const PagedAttnParams& p, int64_t tok, int head, float m, float l) {
+  const int64_t at = tok * (static_cast<int64_t>(p.c.h_kv) * p.group) + head;
+  const float z = l == 0.f ? -INFINITY : m + log2f(l);
+  if (p.lse) p.lse[at] = z * kLn2;
+  if (p.lse2) p.lse2[at] = z;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_rows(const PagedAttnParams& p, int64_t q0, int head, const TileRows& t, int R,
+                                          int stride, float* qs) {
+  const int d = p.c.d, vecs = d / 8;
+  const float c = p.inv_scale * kLog2e;
+  for (int e = threadIdx.x; e < R * vecs; e += kThreads) {
+    const int r = e / vecs, x = (e - r * vecs) * 8;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < t.rows) {
+      const T* src = static_cast<const T*>(p.q) + (q0 + t.tok0 + r / p.group) * p.q_sn +
+                     static_cast<int64_t>(head * p.group + r % p.group) * p.q_sh + x;
+      load8<T>(src, f);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) qs[r * stride + x + i] = f[i] * c;
+  }
+}
+
+// 64 slots' element offsets in the pages (-1: past `lim`, or a bad page).
+__device__ __forceinline__ void tile_offsets(const PagedCacheParams& c, int seq, int head, int k0, int lim,
+                                             int64_t* koff, int64_t* voff) {
+  if (threadIdx.x < kKT) {
+    const int j = k0 + threadIdx.x;
+    int64_t ko = -1, vo = -1;
+    if (j < lim) {
+      int page, row;
+      page_of(c, j, page, row);
+      const int64_t pg = physical_page(c, c.table, c.table_stride, seq, page);
+      if (pg >= 0) {
+        ko = pg * c.k_sp + row * c.k_sn + static_cast<int64_t>(head) * c.k_sh;
+        vo = pg * c.v_sp + row * c.v_sn + static_cast<int64_t>(head) * c.v_sh;
+      }
+    }
+    koff[threadIdx.x] = ko;
+    voff[threadIdx.x] = vo;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_tile(const void* base, const int64_t* off, int d, int dpad, int stride,
+                                          float* dst) {
+  const int vecs = dpad / 8;
+  for (int e = threadIdx.x; e < kKT * vecs; e += kThreads) {
+    const int r = e / vecs, x = (e - r * vecs) * 8;
+    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (off[r] >= 0 && x < d) load8<T>(static_cast<const T*>(base) + off[r] + x, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dst[r * stride + x + i] = f[i];
+  }
+}
+
+// s[i][j] = q_{ty + 16 i} . k_{tx + 16 j}
+template <int RI>
+__device__ __forceinline__ void scores(const float* qs, const float* ks, int d, int stride, int tx, int ty,
+                                       float (&s)[RI][4]) {
+#pragma unroll
+  for (int i = 0; i < RI; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+  for (int x = 0; x < d; x += 4) {
+    float4 a[RI], b[4];
+#pragma unroll
+    for (int i = 0; i < RI; ++i) a[i] = *reinterpret_cast<const float4*>(qs + (ty + 16 * i) * stride + x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(ks + (tx + 16 * j) * stride + x);
+#pragma unroll
+    for (int i = 0; i < RI; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
+        s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
+        s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
+        s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+      }
+  }
+}
+
+template <int R, int DP>
+struct SimtGeo {
+  static constexpr int QS = DP + 4, PS = kKT + 4;          // row strides: 16-byte rows on shifted banks
+  static constexpr size_t kSmem = sizeof(float) * (R * QS + kKT * QS + R * PS) + 2 * sizeof(int64_t) * kKT;
+};
+
+template <typename T, int R, int DP>
+__global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) {
+  using G = SimtGeo<R, DP>;
+  constexpr int RI = R / 16, CI = DP / 64;
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;
+  float* ks = qs + R * G::QS;
+  float* ps = ks + kKT * G::QS;
+  int64_t* koff = reinterpret_cast<int64_t*>(ps + R * G::PS);
+  int64_t* voff = koff + kKT;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int tt = tile_tokens(R, p.group), d = p.c.d;
+  PagedWalk w;
+  const bool any = paged_schedule(p, tt, kKT, 1, blockIdx.x, gridDim.x, w);
+  if (!any) {
+    if (tid == 0) p.split[blockIdx.x].valid = 0;
+    return;
+  }
+  if (tid == 0) p.split[blockIdx.x] = paged_split(w);
+  for (int slot = 0; w.u < w.end; slot = 1) {
+    const TileRows t = tile_rows(w, tt, p.group);
+    __syncthreads();
+    load_rows<T>(p, w.q0, w.head, t, R, G::QS, qs);
+    float m[RI], l[RI], o[RI][CI][4];
+    int lim[RI];
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+      lim[i] = seen_slots(p, w.n, w.len, t.tok0 + min((ty + 16 * i) / p.group, tt - 1));
+#pragma unroll
+      for (int c = 0; c < CI; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][c][e] = 0.f;
+    }
+    const int tile_min = seen_slots(p, w.n, w.len, t.tok0);                              // every row sees these
+    const int tile_max = seen_slots(p, w.n, w.len, t.tok0 + t.rows / p.group - 1);       // some row sees these
+    const int64_t from = w.u, stop = min(w.end, w.item_first + w.units);
+    for (; w.u < stop; ++w.u) {
+      const int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+      tile_offsets(p.c, w.seq, w.head, k0, tile_max, koff, voff);
+      __syncthreads();
+      load_tile<T>(p.c.k, koff, d, d, G::QS, ks);
+      __syncthreads();
+      float s[RI][4];
+      scores<RI>(qs, ks, d, G::QS, tx, ty, s);
+#pragma unroll
+      for (int i = 0; i < RI; ++i) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (k0 + tx + 16 * j >= lim[i]) s[i][j] = -INFINITY;
+          mx = fmaxf(mx, s[i][j]);
+        }
+#pragma unroll
+        for (int off = 8; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float mn = fmaxf(m[i], mx);
+        const float base = mn == -INFINITY ? 0.f : mn;       // a row that has seen nothing: p = 0, no NaN
+        const float r = exp2f(m[i] - base);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e = exp2f(s[i][j] - base);
+          sum += e;
+          ps[(ty + 16 * i) * G::PS + tx + 16 * j] = e;
+        }
+        l[i] = l[i] * r + sum;                               // this thread's keys only; joined at the end
+        m[i] = mn;
+#pragma unroll
+        for (int c = 0; c < CI; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][c][e] *= r;
+      }
+      __syncthreads();
+      load_tile<T>(p.c.v, voff, d, DP, G::QS, ks);
+      __syncthreads();
+      if (k0 + kKT <= tile_min) {
+#pragma unroll 2
+        for (int j = 0; j < kKT; j += 4) {
+          float4 pr[RI];
+#pragma unroll
+          for (int i = 0; i < RI; ++i) pr[i] = *reinterpret_cast<const float4*>(ps + (ty + 16 * i) * G::PS + j);
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+            for (int c = 0; c < CI; ++c) {
+              const float4 v = *reinterpret_cast<const float4*>(ks + (j + jj) * G::QS + 64 * c + 4 * tx);
+#pragma unroll
+              for (int i = 0; i < RI; ++i) {
+                const float e = jj == 0 ? pr[i].x : jj == 1 ? pr[i].y : jj == 2 ? pr[i].z : pr[i].w;
+                o[i][c][0] = fmaf(e, v.x, o[i][c][0]);
+                o[i][c][1] = fmaf(e, v.y, o[i][c][1]);
+                o[i][c][2] = fmaf(e, v.z, o[i][c][2]);
+                o[i][c][3] = fmaf(e, v.w, o[i][c][3]);
+              }
+            }
+        }
+      } else {
+        // some row does not see the whole tile: a hidden slot's value is not
+        // multiplied at all (0 * inf would be NaN)
+        for (int j = 0; j < kKT; ++j)
+#pragma unroll
+          for (int c = 0; c < CI; ++c) {
+            const float4 v = *reinterpret_cast<const float4*>(ks + j * G::QS + 64 * c + 4 * tx);
+#pragma unroll
+            for (int i = 0; i < RI; ++i) {
+              const float e = ps[(ty + 16 * i) * G::PS + j];
+              if (k0 + j < lim[i]) {
+                o[i][c][0] = fmaf(e, v.x, o[i][c][0]);
+                o[i][c][1] = fmaf(e, v.y, o[i][c][1]);
+                o[i][c][2] = fmaf(e, v.z, o[i][c][2]);
+                o[i][c][3] = fmaf(e, v.w, o[i][c][3]);
+              }
+            }
+          }
+      }
+      __syncthreads();
+    }
+    const bool whole = from == w.item_first && stop == w.item_first + w.units;
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+#pragma unroll
+      for (int off = 8; off; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+      const int r = ty + 16 * i;
+      if (r >= t.rows) continue;
+      if (whole) {
+        const int64_t tok = w.q0 + t.tok0 + r / p.group;
+        const int head = w.head * p.group + r % p.group;
+        const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+        T* dst = static_cast<T*>(p.out) + tok * p.o_sn + head * p.o_sh;
+#pragma unroll
+        for (int c = 0; c < CI; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = 64 * c + 4 * tx + e;
+            if (x < d) dst[x] = Elem<T>::from_f(o[i][c][e] * inv);
+          }
+        if (tx == 0) store_lse(p, tok, head, m[i], l[i]);
+      } else {
+        float* dst = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * R + r) * (d + 2);
+#pragma unroll
+        for (int c = 0; c < CI; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = 64 * c + 4 * tx + e;
+            if (x < d) dst[x] = o[i][c][e];
+          }
+        if (tx == 0) {
+          dst[d] = m[i];
+          dst[d + 1] = l[i];
+        }
+      }
+    }
+    if (w.u < w.end) paged_next_item(p, tt, kKT, w);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// join of the items cut by CTA boundaries.  Block (b, y) looks at the boundary
+// before CTA b: if it is the first one inside its item, the block joins its
+// share of the item's rows over the CTAs that hold parts of it, in CTA order.
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(128) combine_kernel(PagedAttnParams p, int R) {
+  const int b = blockIdx.x + 1;
+  const PagedSplit it = p.split[b], before = p.split[b - 1];
+  if (!it.valid) return;
+  // the item starts before this CTA, and in the CTA before it
+  if (it.cta_first != b - 1) return;
+  const int tt = tile_tokens(R, p.group), d = p.c.d;
+  const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, it.seq);
+  const int tok0 = it.tile * tt, rows = min(tt, q.n - tok0) * p.group;
+  const int slot0 = before.item_first == it.item_first ? 0 : 1;    // CTA b - 1: is it also that CTA's first item
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+  for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
+    float m = -INFINITY;
+    for (int c = b - 1; c <= it.cta_last; ++c)
+      m = fmaxf(m, p.part[(static_cast<int64_t>(c * 2 + (c == b - 1 ? slot0 : 0)) * R + r) * (d + 2) + d]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] = 0.f;
+    for (int c = b - 1; c <= it.cta_last; ++c) {
+      const float* src = p.part + (static_cast<int64_t>(c * 2 + (c == b - 1 ? slot0 : 0)) * R + r) * (d + 2);
+      const float f = exp2f(src[d] - base);
+      l = fmaf(f, src[d + 1], l);
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (lane + 32 * x < d) o[x] = fmaf(f, src[lane + 32 * x], o[x]);
+    }
+    const int64_t tok = q.q0 + tok0 + r / p.group;
+    const int head = it.head * p.group + r % p.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* dst = static_cast<T*>(p.out) + tok * p.o_sn + head * p.o_sh;
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (lane + 32 * x < d) dst[lane + 32 * x] = Elem<T>::from_f(o[x] * inv);
+    if (lane == 0) store_lse(p, tok, head, m, l);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// slot weights: w_j += sum over the rows i of the group that see j of
+// exp2(s_ij - lse2_i).  One CTA per (64 slots, KV head, sequence) walks the row
+// tiles that see its slots; every slot is added to once per call, so without
+// shared pages the sums do not depend on timing.
+// ---------------------------------------------------------------------------
+template <typename T, int R, int DP>
+__global__ void __launch_bounds__(kThreads) weights_simt_kernel(PagedAttnParams p) {
+  using G = SimtGeo<R, DP>;
+  constexpr int RI = R / 16;
+  extern __shared__ __align__(16) float smem[];
+  float* qs = smem;
+  float* ks = qs + R * G::QS;
+  float* ps = ks + kKT * G::QS;
+  int64_t* koff = reinterpret_cast<int64_t*>(ps + R * G::PS);
+  int64_t* voff = koff + kKT;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int seq = blockIdx.z, head = blockIdx.y, k0 = blockIdx.x * kKT;
+  const int tt = tile_tokens(R, p.group), d = p.c.d;
+  const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, seq);
+  if (q.n == 0 || k0 >= q.len) return;
+  tile_offsets(p.c, seq, head, k0, q.len, koff, voff);
+  __syncthreads();
+  load_tile<T>(p.c.k, koff, d, d, G::QS, ks);
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int t0 = 0; t0 < q.n; t0 += tt) {
+    const TileRows t{t0, min(tt, q.n - t0) * p.group};
+    if (seen_slots(p, q.n, q.len, t0 + t.rows / p.group - 1) <= k0) continue;
+    __syncthreads();
+    load_rows<T>(p, q.q0, head, t, R, G::QS, qs);
+    __syncthreads();
+    float s[RI][4];
+    scores<RI>(qs, ks, d, G::QS, tx, ty, s);
+#pragma unroll
+    for (int i = 0; i < RI; ++i) {
+      const int r = ty + 16 * i;
+      if (r >= t.rows) continue;
+      const int lim = seen_slots(p, q.n, q.len, t0 + r / p.group);
+      const float z = p.lse2[(q.q0 + t0 + r / p.group) * (static_cast<int64_t>(p.c.h_kv) * p.group) +
+                             head * p.group + r % p.group];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k0 + tx + 16 * j < lim) sum[j] += exp2f(s[i][j] - z);
+    }
+  }
+  // over the 16 row groups of the CTA, in a fixed order
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ps[ty * G::PS + tx + 16 * j] = sum[j];
+  __syncthreads();
+  if (tid < kKT && k0 + tid < q.len) {
+    float a = 0.f;
+    for (int y = 0; y < 16; ++y) a += ps[y * G::PS + tid];
+    int page, row;
+    page_of(p.c, k0 + tid, page, row);
+    const int64_t pg = physical_page(p.c, p.c.table, p.c.table_stride, seq, page);
+    if (pg >= 0) atomicAdd(&p.c.w[pg * p.c.w_sp + row * p.c.w_sn + head * p.c.w_sh], a);
+  }
+}
+
+template <typename T, int R, int DP>
+cudaError_t launch_simt(const PagedAttnParams& p, int grid, cudaStream_t st) {
+  const int smem = static_cast<int>(SimtGeo<R, DP>::kSmem);
+  auto kern = attn_simt_kernel<T, R, DP>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, kThreads, smem, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  if (grid > 1) {
+    combine_kernel<T><<<dim3(grid - 1, R / 16), 128, 0, st>>>(p, R);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  if (!p.c.w) return cudaSuccess;
+  auto wk = weights_simt_kernel<T, R, DP>;
+  e = cudaFuncSetAttribute(wk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
+  wk<<<dim3(static_cast<unsigned>(cdiv(slots, kKT)), p.c.h_kv, p.c.batch), kThreads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int R>
+cudaError_t launch_simt_d(const PagedAttnParams& p, int grid, cudaStream_t st) {
+  if (p.c.d <= 64) return launch_simt<T, R, 64>(p, grid, st);
+  if (p.c.d <= 128) return launch_simt<T, R, 128>(p, grid, st);
+  return launch_simt<T, R, 256>(p, grid, st);
+}
+
+// Tile rows: 64 where the mean chunk fills more than one 16-row tile.
+int simt_rows(const PagedAttnParams& p) { return p.rows * p.group > 16ll * p.c.batch ? 64 : 16; }
+constexpr int kGrid = 2 * 148;
+
+}  // namespace
+
+size_t paged_attn_simt_workspace(const PagedAttnParams& p) {
+  return (static_cast<size_t>(kGrid) * 2 * simt_rows(p) * (p.c.d + 2) * 4 + 255) / 256 * 256 +
+         (kGrid * sizeof(PagedSplit) + 255) / 256 * 256 +
+         (p.c.w ? static_cast<size_t>(p.rows) * p.c.h_kv * p.group * 4 : 0);
+}
+
+cudaError_t launch_paged_attn_simt(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st) {
+  const int R = simt_rows(p);
+  char* at = static_cast<char*>(ws);
+  p.part = reinterpret_cast<float*>(at);
+  at += (static_cast<size_t>(kGrid) * 2 * R * (p.c.d + 2) * 4 + 255) / 256 * 256;
+  p.split = reinterpret_cast<PagedSplit*>(at);
+  at += (kGrid * sizeof(PagedSplit) + 255) / 256 * 256;
+  p.lse2 = p.c.w ? reinterpret_cast<float*>(at) : nullptr;
+  switch (dt) {
+    case SSA_F32: return R == 64 ? launch_simt_d<float, 64>(p, kGrid, st) : launch_simt_d<float, 16>(p, kGrid, st);
+    case SSA_BF16:
+      return R == 64 ? launch_simt_d<__nv_bfloat16, 64>(p, kGrid, st) : launch_simt_d<__nv_bfloat16, 16>(p, kGrid, st);
+    default: return R == 64 ? launch_simt_d<__half, 64>(p, kGrid, st) : launch_simt_d<__half, 16>(p, kGrid, st);
+  }
+}
+
+}  // namespace ssa

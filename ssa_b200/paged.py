@@ -1,0 +1,353 @@
+"""A paged key/value cache, exact attention over it, and eviction.
+
+Keys and values of many sequences live in pages of a fixed number of slots:
+``k_pages``, ``v_pages`` ``[num_pages, page_size, h_kv, d]`` (any strides with a
+contiguous last dimension; :class:`PagedCache` keeps a head's rows of a page
+side by side).  Slot ``j`` of sequence ``s`` is row ``j % page_size`` of page
+``page_table[s, j // page_size]``, and ``kv_lens[s]`` slots are filled.
+
+A call takes a ragged batch: ``q_starts [B + 1]`` splits the new rows among the
+sequences, and the rows of a sequence are its last cached positions
+(``kv_lens`` counts them).  The lengths stay on the device -- no op copies them
+back or waits -- so a call can be captured in a CUDA graph and replayed with
+other lengths.
+
+The reference keeps no cache.  These ops are exact attention for what runs
+next to its sparse attention: dense layers, prompts too short to route, and
+caches that must not grow (:func:`paged_evict`).  They serve; they have no
+gradient.
+
+Errors in the data (a page number outside the cache, lengths that do not fit)
+are found on the device and raised by a later op call or by
+:func:`ssa_b200.check_errors`.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib as L
+from . import _status as S
+from .ops import _dtype_code, _last_contig, _require_cuda
+
+_APPEND, _ATTEND, _EVICT = range(3)
+
+
+def _index(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
+    if t.device != dev:
+        raise RuntimeError(f"tensors on different devices: {dev} and {t.device} ({name})")
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("*" if n is None else str(n) for n in shape)
+        raise ValueError(f"{name} must have shape [{want}], got {list(t.shape)}")
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _cache_args(k_pages, v_pages, page_table, kv_lens, weights, op):
+    """The filled :class:`SsaPagedCache` (with the op's error word) and the index
+    tensors it points into."""
+    dev = _require_cuda(k_pages, v_pages)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("k_pages and v_pages must both be [num_pages, page_size, h_kv, d], got "
+                         f"{list(k_pages.shape)} and {list(v_pages.shape)}")
+    if k_pages.dtype != v_pages.dtype:
+        raise TypeError(f"k_pages, v_pages dtypes differ: {k_pages.dtype}, {v_pages.dtype}")
+    # the pages are written in place, so a copy would be of no use
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise ValueError("the last dimension of k_pages and v_pages must be contiguous")
+    kv_lens = _index(kv_lens, "kv_lens", (None,), dev)
+    page_table = _index(page_table, "page_table", (kv_lens.shape[0], None), dev)
+    c = L.SsaPagedCache()
+    c.num_pages, c.page_size, c.h_kv, c.d = k_pages.shape
+    c.batch, c.max_pages = page_table.shape
+    c.dtype = _dtype_code(k_pages)
+    c.k_pages = k_pages.data_ptr()
+    c.k_stride_p, c.k_stride_n, c.k_stride_h, _ = k_pages.stride()
+    c.v_pages = v_pages.data_ptr()
+    c.v_stride_p, c.v_stride_n, c.v_stride_h, _ = v_pages.stride()
+    if weights is not None:
+        if weights.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} and {weights.device} (weights)")
+        if weights.dtype != torch.float32:
+            raise TypeError(f"weights must be float32, got {weights.dtype}")
+        if weights.shape != k_pages.shape[:3]:
+            raise ValueError(f"weights must be [num_pages, page_size, h_kv] = {list(k_pages.shape[:3])}, got "
+                             f"{list(weights.shape)}")
+        c.weights = weights.data_ptr()
+        c.w_stride_p, c.w_stride_n, c.w_stride_h = weights.stride()
+    c.page_table = page_table.data_ptr()
+    c.table_stride = page_table.stride(0)
+    c.kv_lens = kv_lens.data_ptr()
+    c.status = S.host_word(dev, op)
+    return dev, c, (page_table, kv_lens)
+
+
+def _call(dev, fn, *args):
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        code = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, stream)
+    L.check(fn.__name__, code)
+    S.host_word_done(dev)
+
+
+def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                 page_table: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor,
+                 weights: Optional[torch.Tensor] = None) -> None:
+    """Writes new keys and values into the cache, in place.
+
+    Args:
+        k_new, v_new: ``[T, h_kv, d]``, the rows of all sequences one after another.
+        k_pages, v_pages: ``[num_pages, page_size, h_kv, d]``, written.
+        page_table: ``[B, max_pages]`` int32.
+        q_starts: ``[B + 1]`` int32: rows ``q_starts[s] .. q_starts[s + 1] - 1`` are
+            sequence ``s``'s and go to its slots ``kv_lens[s] - n .. kv_lens[s] - 1``.
+        kv_lens: ``[B]`` int32, the lengths with the new rows counted.
+        weights: optional ``[num_pages, page_size, h_kv]`` float32 slot weights;
+            those of the written slots become 0.
+    """
+    dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _APPEND)
+    _require_cuda(k_pages, k_new, v_new)
+    if k_new.shape != v_new.shape or k_new.dim() != 3 or k_new.shape[1:] != k_pages.shape[2:]:
+        raise ValueError(f"k_new and v_new must be [rows, {k_pages.shape[2]}, {k_pages.shape[3]}], got "
+                         f"{list(k_new.shape)} and {list(v_new.shape)}")
+    if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
+        raise TypeError(f"k_new, v_new ({k_new.dtype}, {v_new.dtype}) must have the cache's dtype {k_pages.dtype}")
+    q_starts = _index(q_starts, "q_starts", (c.batch + 1,), dev)
+    k_new, v_new = _last_contig(k_new), _last_contig(v_new)
+    a = L.SsaPagedAppendArgs()
+    a.rows, a.q_starts = k_new.shape[0], q_starts.data_ptr()
+    a.k_new = k_new.data_ptr()
+    a.k_new_stride_n, a.k_new_stride_h, _ = k_new.stride()
+    a.v_new = v_new.data_ptr()
+    a.v_new_stride_n, a.v_new_stride_h, _ = v_new.stride()
+    _call(dev, L.lib().ssa_paged_append, ctypes.byref(c), ctypes.byref(a))
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    q_starts: torch.Tensor, kv_lens: torch.Tensor, scale: Optional[float] = None,
+                    is_causal: bool = True, weights: Optional[torch.Tensor] = None, return_lse: bool = False
+                    ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Softmax attention of a ragged batch of new rows over the paged cache.
+
+    Args:
+        q: ``[T, h_q, d]``, the rows of all sequences one after another, split by
+            ``q_starts`` as in :func:`paged_append`; query head ``e`` reads KV head
+            ``e // (h_q // h_kv)``.
+        scale: logits are ``(q . k) / scale``; default ``sqrt(d)`` (a divisor, as in
+            :func:`ssa_b200.sparse_exact_attention`).
+        is_causal: row ``i`` of a sequence's ``n`` sees the slots
+            ``j <= kv_lens[s] - n + i``; otherwise every filled slot.
+        weights: optional ``[num_pages, page_size, h_kv]`` float32; every slot's
+            weight grows, in place, by the attention it receives in this call,
+            summed over the sequence's rows and the heads of its group.  A page
+            shared by several sequences of the call collects from all of them
+            (in no fixed order of additions).
+        return_lse: also return the rows' log-sum-exp of the logits.
+
+    Returns ``[T, h_q, d]`` in ``q``'s dtype (and ``[T, h_q]`` float32).  A row that
+    sees no slot gets zeros (and ``-inf``).  Rows outside ``q_starts`` are not
+    written.
+    """
+    dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
+    _require_cuda(k_pages, q)
+    if q.dim() != 3 or q.shape[2] != c.d:
+        raise ValueError(f"q must be [rows, h_q, {c.d}], got {list(q.shape)}")
+    if q.shape[1] % c.h_kv:
+        raise ValueError("num_q_heads must be divisible by num_kv_heads")
+    if q.dtype != k_pages.dtype:
+        raise TypeError(f"q ({q.dtype}) must have the cache's dtype {k_pages.dtype}")
+    q_starts = _index(q_starts, "q_starts", (c.batch + 1,), dev)
+    q = _last_contig(q)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+    a = L.SsaPagedAttnArgs()
+    a.rows, a.q_starts, a.h_q, a.causal = q.shape[0], q_starts.data_ptr(), q.shape[1], 1 if is_causal else 0
+    a.scale = math.sqrt(c.d) if scale is None else float(scale)
+    a.q = q.data_ptr()
+    a.q_stride_n, a.q_stride_h, _ = q.stride()
+    a.out = out.data_ptr()
+    a.out_stride_n, a.out_stride_h, _ = out.stride()
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    lib, rc, ra = L.lib(), ctypes.byref(c), ctypes.byref(a)
+    ws = torch.empty(max(int(lib.ssa_paged_attn_workspace_size(rc, ra)), 16), dtype=torch.uint8, device=dev)
+    _call(dev, lib.ssa_paged_attn, rc, ra, ws.data_ptr(), ws.numel())
+    return (out, lse) if return_lse else out
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Tensor, page_table: torch.Tensor,
+                kv_lens: torch.Tensor, new_table: torch.Tensor, budget: int, recent: int = 0
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cuts every sequence's cache back to ``budget`` slots per KV head.
+
+    Each (sequence, KV head) keeps ``min(kv_len, budget)`` slots: its last ``recent``
+    and the heaviest of the others by ``weights`` (the lower slot first among equal
+    weights).  Keys, values and weights of the kept slots are copied, in order, to
+    the first slots of the pages ``new_table [B, *]`` names; these must not be pages
+    that ``page_table`` uses, which stay as they are (other sequences may share them).
+
+    Returns ``kept [B, h_kv, budget]`` int32, the kept slots in ascending order
+    followed by -1, and the new lengths ``[B]`` int32.
+    """
+    if weights is None:
+        raise ValueError("weights is needed: eviction ranks slots by them")
+    dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
+    budget, recent = int(budget), int(recent)
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"budget {budget}, recent {recent}: need budget >= 1 and 0 <= recent <= budget")
+    new_table = _index(new_table, "new_table", (c.batch, None), dev)
+    kept = torch.empty((c.batch, c.h_kv, budget), dtype=torch.int32, device=dev)
+    new_lens = torch.empty((c.batch,), dtype=torch.int32, device=dev)
+    a = L.SsaPagedEvictArgs()
+    a.budget, a.recent, a.new_max_pages = budget, recent, new_table.shape[1]
+    a.new_table, a.new_table_stride = new_table.data_ptr(), new_table.stride(0)
+    a.kept, a.new_lens = kept.data_ptr(), new_lens.data_ptr()
+    _call(dev, L.lib().ssa_paged_evict, ctypes.byref(c), ctypes.byref(a))
+    return kept, new_lens
+
+
+class PagedBatch:
+    """The sequences of one step: index tensors of the three ops, made once and
+    used by every layer."""
+
+    __slots__ = ("ids", "q_lens", "kv_lens_host", "page_table", "q_starts", "kv_lens")
+
+    def __init__(self, ids, q_lens, kv_lens, page_table, q_starts, kv_lens_dev):
+        self.ids, self.q_lens, self.kv_lens_host = ids, q_lens, kv_lens
+        self.page_table, self.q_starts, self.kv_lens = page_table, q_starts, kv_lens_dev
+
+
+class PagedCache:
+    """Pages, and which of them hold which sequence, for ``num_layers`` layers on one GPU.
+
+    A step: :meth:`extend` makes room for the new rows of some sequences and
+    returns their :class:`PagedBatch`; then each layer calls :meth:`append` and
+    :meth:`attend` with it.  :meth:`evict` cuts sequences back to a budget (with
+    ``track_weights=True``, where :meth:`attend` counts the attention every slot
+    receives).  Page numbers are handed out on the host; pages given back are
+    reused at once, which is safe for work on one stream."""
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, num_layers: int = 1,
+                 dtype=torch.bfloat16, device="cuda", track_weights: bool = False):
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.page_size, self.num_pages, self.num_layers = page_size, num_pages, num_layers
+        # zeros, not garbage: slots past a length are loaded (and masked) with their tile
+        shape = (num_layers, num_pages, num_kv_heads, page_size)
+        self.k_pages = torch.zeros(shape + (head_dim,), dtype=dtype, device=self.device).transpose(2, 3)
+        self.v_pages = torch.zeros(shape + (head_dim,), dtype=dtype, device=self.device).transpose(2, 3)
+        self.weights = (torch.zeros(shape, dtype=torch.float32, device=self.device).transpose(2, 3)
+                        if track_weights else None)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages = {}
+        self._len = {}
+        self._next = 0
+
+    # -- sequences ---------------------------------------------------------
+    def add(self) -> int:
+        """A new, empty sequence's id."""
+        sid, self._next = self._next, self._next + 1
+        self._pages[sid], self._len[sid] = [], 0
+        return sid
+
+    def remove(self, sid: int) -> None:
+        """Gives the sequence's pages back."""
+        self._free.extend(reversed(self._pages.pop(sid)))
+        del self._len[sid]
+
+    def length(self, sid: int) -> int:
+        return self._len[sid]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _pages_for(self, n: int) -> int:
+        return -(-n // self.page_size)
+
+    def _upload(self, pages: Sequence[List[int]], *vectors: Sequence[int]):
+        """Page lists as a padded table, and integer vectors, in one copy."""
+        width = max([len(p) for p in pages] + [1])
+        flat = [x for p in pages for x in p + [0] * (width - len(p))]
+        for v in vectors:
+            flat.extend(v)
+        dev = torch.tensor(flat, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        at = len(pages) * width
+        parts = [dev[:at].view(len(pages), width)]
+        for v in vectors:
+            parts.append(dev[at:at + len(v)])
+            at += len(v)
+        return parts
+
+    def extend(self, ids: Sequence[int], new_rows: Sequence[int]) -> PagedBatch:
+        """Room for ``new_rows[i]`` more rows of sequence ``ids[i]``; nothing changes
+        when the free pages do not suffice (``RuntimeError``)."""
+        ids, q_lens = list(ids), [int(n) for n in new_rows]
+        if len(ids) != len(q_lens) or len(set(ids)) != len(ids):
+            raise ValueError("ids must be distinct and match new_rows")
+        if any(n < 0 for n in q_lens):
+            raise ValueError("new_rows must not be negative")
+        kv = [self._len[s] + n for s, n in zip(ids, q_lens)]
+        need = [self._pages_for(n) - len(self._pages[s]) for s, n in zip(ids, kv)]
+        if sum(need) > len(self._free):
+            raise RuntimeError(f"paged cache full: {sum(need)} pages needed, {len(self._free)} free")
+        for s, n, more in zip(ids, kv, need):
+            self._pages[s].extend(self._free.pop() for _ in range(more))
+            self._len[s] = n
+        starts = [0]
+        for n in q_lens:
+            starts.append(starts[-1] + n)
+        table, q_starts, kv_dev = self._upload([self._pages[s] for s in ids], starts, kv)
+        return PagedBatch(ids, q_lens, kv, table, q_starts, kv_dev)
+
+    # -- one layer of a step -------------------------------------------------
+    def append(self, batch: PagedBatch, k_new: torch.Tensor, v_new: torch.Tensor, layer: int = 0) -> None:
+        """:func:`paged_append` of the batch's rows to one layer."""
+        paged_append(k_new, v_new, self.k_pages[layer], self.v_pages[layer], batch.page_table, batch.q_starts,
+                     batch.kv_lens, None if self.weights is None else self.weights[layer])
+
+    def attend(self, batch: PagedBatch, q: torch.Tensor, layer: int = 0, scale: Optional[float] = None,
+               is_causal: bool = True) -> torch.Tensor:
+        """:func:`paged_attention` of the batch's rows over one layer (weights
+        counted where the cache tracks them)."""
+        return paged_attention(q, self.k_pages[layer], self.v_pages[layer], batch.page_table, batch.q_starts,
+                               batch.kv_lens, scale, is_causal, None if self.weights is None else self.weights[layer])
+
+    # -- between steps ---------------------------------------------------------
+    def evict(self, ids: Sequence[int], budget: int, recent: int = 0) -> List[int]:
+        """Cuts the sequences longer than ``budget`` back to it in every layer
+        (:func:`paged_evict`); returns their ids.  The copies go to free pages,
+        so at least one sequence's budget of them must be free; as many
+        sequences as fit are cut at a time."""
+        if self.weights is None:
+            raise ValueError("the cache keeps no weights: make it with track_weights=True")
+        ids = list(ids)
+        if len(set(ids)) != len(ids):
+            raise ValueError("ids must be distinct")
+        todo = [s for s in ids if self._len[s] > budget]
+        done, need = list(todo), self._pages_for(budget)
+        if todo and len(self._free) < need:
+            raise RuntimeError(f"paged cache full: eviction copies to {need} free pages, {len(self._free)} are")
+        while todo:
+            now = todo[:len(self._free) // need]
+            todo = todo[len(now):]
+            old = [self._pages[s] for s in now]
+            new = [[self._free.pop() for _ in range(need)] for _ in now]
+            table, lens = self._upload(old, [self._len[s] for s in now])
+            new_table, = self._upload(new)
+            for layer in range(self.num_layers):
+                paged_evict(self.k_pages[layer], self.v_pages[layer], self.weights[layer], table, lens, new_table,
+                            budget, recent)
+            for s, o, p in zip(now, old, new):
+                self._free.extend(reversed(o))
+                self._pages[s], self._len[s] = p, budget
+        return done
