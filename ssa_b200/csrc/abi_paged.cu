@@ -116,7 +116,7 @@ ssa_status ssa_paged_append(const SsaPagedCache* cache, const SsaPagedAppendArgs
 size_t ssa_paged_attn_workspace_size(const SsaPagedCache* cache, const SsaPagedAttnArgs* args) {
   ssa::PagedAttnParams p{};
   if (attn_params(cache, args, p) != SSA_OK) return 0;
-  return ssa::paged_attn_simt_workspace(p);
+  return ssa::paged_attn_workspace(p, cache->dtype);
 }
 
 ssa_status ssa_paged_attn(const SsaPagedCache* cache, const SsaPagedAttnArgs* args, void* workspace,
@@ -125,11 +125,11 @@ ssa_status ssa_paged_attn(const SsaPagedCache* cache, const SsaPagedAttnArgs* ar
   const ssa_status s = attn_params(cache, args, p);
   if (s != SSA_OK) return s;
   if (args->rows == 0 || cache->batch == 0) return SSA_OK;
-  const size_t need = ssa::paged_attn_simt_workspace(p);
+  const size_t need = ssa::paged_attn_workspace(p, cache->dtype);
   if (!workspace || workspace_bytes < need)
     return fail(SSA_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, workspace_bytes);
   if (!aligned16(workspace)) return fail(SSA_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-  return cuda_status(ssa::launch_paged_attn_simt(p, cache->dtype, workspace, static_cast<cudaStream_t>(stream)),
+  return cuda_status(ssa::launch_paged_attn(p, cache->dtype, workspace, static_cast<cudaStream_t>(stream)),
                      "paged_attn");
 }
 

@@ -295,8 +295,11 @@ __host__ __device__ inline int tile_tokens(int tile_rows, int group) { return ti
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, ssa_dtype dt, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictParams& p, ssa_dtype dt, cudaStream_t st);
-// Attention on the CUDA cores: every type, head size and page size.
-size_t paged_attn_simt_workspace(const PagedAttnParams& p);
-cudaError_t launch_paged_attn_simt(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st);
+// Attention (paged_attn.cu): picks the kernel, joins split items, adds slot weights.
+size_t paged_attn_workspace(const PagedAttnParams& p, ssa_dtype dt);
+cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st);
+// Chunks on the tensor cores (paged_attn_tc.cu), 256 rows an item, one CTA per SM.
+bool paged_attn_tc_supported(const PagedAttnParams& p, ssa_dtype dt);
+cudaError_t launch_paged_attn_tc(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st);
 
 }  // namespace ssa

@@ -391,61 +391,85 @@ __global__ void __launch_bounds__(kThreads) weights_simt_kernel(PagedAttnParams 
 }
 
 template <typename T, int R, int DP>
-cudaError_t launch_simt(const PagedAttnParams& p, int grid, cudaStream_t st) {
+cudaError_t launch_simt(const PagedAttnParams& p, int grid, bool weights, cudaStream_t st) {
   const int smem = static_cast<int>(SimtGeo<R, DP>::kSmem);
-  auto kern = attn_simt_kernel<T, R, DP>;
+  if (!weights) {
+    auto kern = attn_simt_kernel<T, R, DP>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    kern<<<grid, kThreads, smem, st>>>(p);
+    return cudaGetLastError();
+  }
+  auto kern = weights_simt_kernel<T, R, DP>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kern<<<grid, kThreads, smem, st>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  if (grid > 1) {
-    combine_kernel<T><<<dim3(grid - 1, R / 16), 128, 0, st>>>(p, R);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
-  if (!p.c.w) return cudaSuccess;
-  auto wk = weights_simt_kernel<T, R, DP>;
-  e = cudaFuncSetAttribute(wk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
   const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
-  wk<<<dim3(static_cast<unsigned>(cdiv(slots, kKT)), p.c.h_kv, p.c.batch), kThreads, smem, st>>>(p);
+  if (slots == 0) return cudaSuccess;
+  kern<<<dim3(static_cast<unsigned>(cdiv(slots, kKT)), p.c.h_kv, p.c.batch), kThreads, smem, st>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T, int R>
-cudaError_t launch_simt_d(const PagedAttnParams& p, int grid, cudaStream_t st) {
-  if (p.c.d <= 64) return launch_simt<T, R, 64>(p, grid, st);
-  if (p.c.d <= 128) return launch_simt<T, R, 128>(p, grid, st);
-  return launch_simt<T, R, 256>(p, grid, st);
+cudaError_t launch_simt_d(const PagedAttnParams& p, int grid, bool weights, cudaStream_t st) {
+  if (p.c.d <= 64) return launch_simt<T, R, 64>(p, grid, weights, st);
+  if (p.c.d <= 128) return launch_simt<T, R, 128>(p, grid, weights, st);
+  return launch_simt<T, R, 256>(p, grid, weights, st);
 }
 
-// Tile rows: 64 where the mean chunk fills more than one 16-row tile.
-int simt_rows(const PagedAttnParams& p) { return p.rows * p.group > 16ll * p.c.batch ? 64 : 16; }
-constexpr int kGrid = 2 * 148;
+template <int R>
+cudaError_t launch_simt_t(const PagedAttnParams& p, ssa_dtype dt, int grid, bool weights, cudaStream_t st) {
+  switch (dt) {
+    case SSA_F32: return launch_simt_d<float, R>(p, grid, weights, st);
+    case SSA_BF16: return launch_simt_d<__nv_bfloat16, R>(p, grid, weights, st);
+    default: return launch_simt_d<__half, R>(p, grid, weights, st);
+  }
+}
+
+// The kernel that serves a call, its tile rows and grid, and the workspace.
+struct AttnPlan {
+  bool tc;
+  int rows, grid;
+  size_t split, lse2, total;
+};
+
+// More than 16 rows (new tokens x heads of a group) per sequence on average:
+// tiles of many rows, on the tensor cores where they apply.
+AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
+  AttnPlan a{};
+  const bool chunks = p.rows * p.group > 16ll * p.c.batch;
+  a.tc = chunks && paged_attn_tc_supported(p, dt);
+  a.rows = a.tc ? 256 : chunks ? 64 : 16;
+  a.grid = a.tc ? 148 : 2 * 148;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  a.split = up(static_cast<size_t>(a.grid) * 2 * a.rows * (p.c.d + 2) * 4);
+  a.lse2 = a.split + up(a.grid * sizeof(PagedSplit));
+  a.total = a.lse2 + (p.c.w ? up(static_cast<size_t>(p.rows) * p.c.h_kv * p.group * 4) : 0);
+  return a;
+}
 
 }  // namespace
 
-size_t paged_attn_simt_workspace(const PagedAttnParams& p) {
-  return (static_cast<size_t>(kGrid) * 2 * simt_rows(p) * (p.c.d + 2) * 4 + 255) / 256 * 256 +
-         (kGrid * sizeof(PagedSplit) + 255) / 256 * 256 +
-         (p.c.w ? static_cast<size_t>(p.rows) * p.c.h_kv * p.group * 4 : 0);
-}
+size_t paged_attn_workspace(const PagedAttnParams& p, ssa_dtype dt) { return attn_plan(p, dt).total; }
 
-cudaError_t launch_paged_attn_simt(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st) {
-  const int R = simt_rows(p);
+cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st) {
+  const AttnPlan a = attn_plan(p, dt);
   char* at = static_cast<char*>(ws);
   p.part = reinterpret_cast<float*>(at);
-  at += (static_cast<size_t>(kGrid) * 2 * R * (p.c.d + 2) * 4 + 255) / 256 * 256;
-  p.split = reinterpret_cast<PagedSplit*>(at);
-  at += (kGrid * sizeof(PagedSplit) + 255) / 256 * 256;
-  p.lse2 = p.c.w ? reinterpret_cast<float*>(at) : nullptr;
+  p.split = reinterpret_cast<PagedSplit*>(at + a.split);
+  p.lse2 = p.c.w ? reinterpret_cast<float*>(at + a.lse2) : nullptr;
+  cudaError_t e = a.tc           ? launch_paged_attn_tc(p, dt, a.grid, st)
+                  : a.rows == 64 ? launch_simt_t<64>(p, dt, a.grid, false, st)
+                                 : launch_simt_t<16>(p, dt, a.grid, false, st);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(a.grid - 1, a.rows / 16);
   switch (dt) {
-    case SSA_F32: return R == 64 ? launch_simt_d<float, 64>(p, kGrid, st) : launch_simt_d<float, 16>(p, kGrid, st);
-    case SSA_BF16:
-      return R == 64 ? launch_simt_d<__nv_bfloat16, 64>(p, kGrid, st) : launch_simt_d<__nv_bfloat16, 16>(p, kGrid, st);
-    default: return R == 64 ? launch_simt_d<__half, 64>(p, kGrid, st) : launch_simt_d<__half, 16>(p, kGrid, st);
+    case SSA_F32: combine_kernel<float><<<grid, 128, 0, st>>>(p, a.rows); break;
+    case SSA_BF16: combine_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p, a.rows); break;
+    default: combine_kernel<__half><<<grid, 128, 0, st>>>(p, a.rows); break;
   }
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !p.c.w) return e;
+  return a.rows >= 64 ? launch_simt_t<64>(p, dt, 0, true, st) : launch_simt_t<16>(p, dt, 0, true, st);
 }
 
 }  // namespace ssa

@@ -1,0 +1,609 @@
+// Attention of chunks over the paged cache on the 5th-generation tensor cores:
+// bf16 / fp16, head size 64 or 128, pages of a power of two of at least 8 slots.
+//
+// A CTA (one per SM) holds 256 query rows of one item (the g heads of a KV
+// group at floor(256 / g) tokens) as two streams of 128 rows, and walks key
+// tiles of 128 slots.  Per tile and stream: S = Q K^T (tcgen05, fp32 in TMEM),
+// the online softmax of a row by the thread that owns its TMEM lane, P written
+// back to TMEM over S in the input type, O += P V (tcgen05, A from TMEM).
+// While one stream is in its softmax the tensor cores work for the other: a
+// tile costs them 4 * 128 * 128 * d flops and the MUFU 128 * 128 exponentials,
+// about 1000 clocks each at d = 128.
+//
+//   warps 0-3   stream A: loads its Q rows, softmax, epilogue (a row per thread)
+//   warps 4-7   stream B
+//   warp 8      TMEM allocation, single-thread MMA issue
+//   warp 9      TMA producer: a lane per page box, K and V tiles in a ring
+//   warps 10-11 nothing: they complete the warpgroup that gives registers up
+//
+// Registers: 384 threads x 168 at launch = 64512; warps 8-11 keep 88 each
+// (128 x 88 = 11264), the streams take 208 (256 x 208 = 53248): 64512 again.
+//
+// TMEM (512 columns): S_A, S_B (128 each; P in the first 64), O_A, O_B (d each).
+//
+// The running maximum that scales a row's exponentials is raised only when a
+// tile exceeds it by more than 2^8 (O, in TMEM, is then multiplied by the
+// quotient): exponentials stay below 2^8, sums in fp32.  P is rounded to the
+// input type, as the tensor cores take it (relative error 2^-9 / 2^-12 of each
+// weight); the row sum adds the unrounded values.  For fp16 every exponential
+// carries a factor 2^7, so that weights down to 2^-21 of the largest stay
+// normal numbers.
+//
+// Hidden slots (past a row's position, or past the sequence in the last page)
+// have P = 0, but 0 times an infinite or NaN value is NaN.  So on a tile that
+// some row does not see whole, the streams look through V: if it holds a
+// non-finite value, that tile's product is made on the CUDA cores over the
+// visible slots alone.
+//
+// Every wait is bounded (about one second); on expiry the CTA records
+// SSA_DEVICE_TIMEOUT, waits (bounded) for its copies and MMAs in flight, frees
+// TMEM and exits.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "common.cuh"
+#include "mma_utils.cuh"
+#include "paged.cuh"
+#include "tc_utils.cuh"
+
+namespace ssa {
+namespace ptc {
+
+using namespace tc;
+
+constexpr int kRows = 256;         // rows of an item
+constexpr int kKT = 128;           // slots per key tile
+constexpr int kThreads = 384;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.f;      // how far (log2) a tile may exceed the running maximum
+
+template <int D>
+struct Geo {
+  static constexpr int kTileBytes = kKT * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr size_t kSmem = 1024 + 2 * kTileBytes + static_cast<size_t>(kStages) * kTileBytes + 512;
+};
+
+// Coordinates of a page box in its 4-D tensor map (d, two of {slot, head}, page).
+struct MapOrder {
+  int head_first;                  // 1: the head dimension has the smaller stride
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+// A from TMEM, B from shared memory.
+__device__ __forceinline__ void mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bd), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Boxes of one K or V tile: lane i < boxes copies 64 columns of one page piece.
+template <int D>
+__device__ __forceinline__ void load_kv(const PagedAttnParams& p, const MapOrder& mo, const void* map, int seq, int head,
+                                        int k0, int lim, uint32_t dst, uint32_t bar) {
+  const int lane = threadIdx.x & 31;
+  const int rows = min(p.c.page_size, kKT), pieces = kKT / rows, boxes = pieces * (D / 64);
+  if (lane == 0) mbar_expect_tx(bar, Geo<D>::kTileBytes);
+  __syncwarp();
+  if (lane < boxes) {
+    const int piece = lane & (pieces - 1), half = lane / pieces;
+    const int j = k0 + piece * rows;
+    int pg = -1, row = 0;
+    // a page outside the table's use reads as zeros (a coordinate out of range)
+    if (j < lim) {
+      int lp;
+      page_of(p.c, j, lp, row);
+      pg = static_cast<int>(physical_page(p.c, p.c.table, p.c.table_stride, seq, lp));
+    }
+    tma_load_4d(dst + half * (kKT * 128) + piece * rows * 128, map, half * 64, mo.head_first ? head : row,
+                mo.head_first ? row : head, pg, bar);
+  }
+}
+
+template <typename T>
+struct Half16;
+template <> struct Half16<__nv_bfloat16> { static constexpr uint32_t kExp = 0x7f807f80u, kOne = 0x00800080u; };
+template <> struct Half16<__half> { static constexpr uint32_t kExp = 0x7c007c00u, kOne = 0x04000400u; };
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// The tile's O += P V for this thread's row over its first `see` slots, on the
+// CUDA cores (P in TMEM columns of S, V swizzled in shared memory).  `fresh`: O
+// holds nothing yet.  The whole stream calls it.
+template <typename T, int D>
+__device__ __forceinline__ void visible_product(uint32_t s_addr, uint32_t o_addr, const unsigned char* v, int see,
+                                             bool fresh) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < D; c0 += 16) {
+    uint32_t o[16];
+    if (!fresh) {
+      tmem_ld16_async(o_addr + c0, o);
+      tmem_wait();
+    }
+    float acc[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) acc[x] = fresh ? 0.f : __uint_as_float(o[x]);
+#pragma unroll 1
+    for (int j0 = 0; j0 < kKT; j0 += 32) {
+      uint32_t pk[16];
+      tmem_ld16_async(s_addr + j0 / 2, pk);
+      tmem_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float2 two = unpack2<T>(pk[j / 2]);
+        const float pj = (j & 1) ? two.y : two.x;
+        if (j0 + j < see) {
+          const unsigned char* row = v + (c0 / 64) * (kKT * 128) + (j0 + j) * 128;
+#pragma unroll
+          for (int x = 0; x < 16; x += 8) {
+            const int piece = ((c0 % 64) + x) / 8;
+            const uint4 w = *reinterpret_cast<const uint4*>(row + ((piece ^ ((j0 + j) & 7)) << 4));
+            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack2<T>(ww[e]);
+              acc[x + 2 * e] = fmaf(pj, f.x, acc[x + 2 * e]);
+              acc[x + 2 * e + 1] = fmaf(pj, f.y, acc[x + 2 * e + 1]);
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(acc[x]);
+    tmem_st16(o_addr + c0, o);
+    tmem_wait_st();
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                              const __grid_constant__ CUtensorMap vmap,
+                                                              PagedAttnParams p, MapOrder mo) {
+  using G = Geo<D>;
+  constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
+  constexpr float kShift = kBf ? 0.f : 7.f;              // factor 2^kShift on every exponential
+  constexpr uint32_t kIdS = idesc_f16(128, kKT, kBf);
+  constexpr uint32_t kIdO = idesc_f16(128, D, kBf) | (1u << 16);   // B (= V) is MN-major
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* q_tile = base;                          // [2][D / 64][128][128 B], SWIZZLE_128B
+  unsigned char* ring = base + 2 * G::kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + G::kStages * G::kTileBytes);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * G::kStages;
+  const uint32_t q_full = empty + 8 * G::kStages, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16;
+  const uint32_t v_seen = o_full + 16, drain = v_seen + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * G::kStages + 11);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* odd_tile = abort_flag + 1;               // [2] the last tile whose product the stream made itself
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+  const int tt = tile_tokens(kRows, p.group);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < G::kStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(q_full + 8 * x, 128);
+      mbar_init(s_full + 8 * x, 1);
+      mbar_init(p_full + 8 * x, 128);
+      mbar_init(o_full + 8 * x, 1);
+      mbar_init(v_seen + 8 * x, 128);
+      odd_tile[x] = 0;
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&vmap);
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  PagedWalk w;
+  const bool any = paged_schedule(p, tt, kKT, 1, blockIdx.x, gridDim.x, w);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(w) : PagedSplit{};
+  auto fail = [&]() {
+    *abort_flag = 1;
+    paged_error(p.c, SSA_DEVICE_TIMEOUT);
+  };
+
+  // a tile is named by its place in the ring, counted from 1
+  auto tile_name = [](int64_t g) { return static_cast<int>(g & 0x3fffffff) + 1; };
+
+  if (warp >= 8) {
+  regs_down<88>();
+  if (any && warp == 9) {
+    // ---------------- TMA producer ----------------
+    int64_t g = 0;
+    bool stop = false;
+    while (w.u < w.end && !stop) {
+      const int tok0 = w.tile * tt, rows = min(tt, w.n - tok0) * p.group;
+      const int last_tok = tok0 + rows / p.group - 1;
+      const int lim = p.causal ? max(w.len - w.n + last_tok + 1, 0) : w.len;
+      const int64_t end = min(w.end, w.item_first + w.units);
+      for (; w.u < end && !stop; ++w.u) {
+        const int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++g) {
+          const int s = static_cast<int>(g % G::kStages);
+          if (*abort_flag || !mbar_wait(empty + 8 * s, static_cast<uint32_t>((g / G::kStages) & 1) ^ 1u)) stop = true;
+          stop = __any_sync(0xffffffffu, stop);
+          if (stop) {
+            fail();
+            break;
+          }
+          load_kv<D>(p, mo, kv ? &vmap : &kmap, w.seq, w.head, k0, lim, smem_u32(ring + s * G::kTileBytes),
+                     full + 8 * s);
+        }
+      }
+      if (w.u < w.end) paged_next_item(p, tt, kKT, w);
+    }
+    // every issued copy lands before the CTA exits
+    if (lane == 0)
+      for (int64_t r = g - 1; r >= 0 && r >= g - G::kStages; --r)
+        mbar_wait(full + 8 * static_cast<int>(r % G::kStages), static_cast<uint32_t>((r / G::kStages) & 1));
+  } else if (any && warp == 8) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      int64_t g = 0;                                     // K tile of the current unit: ring entry g, V: g + 1
+      uint32_t p_ph[2] = {0, 0}, q_ph[2] = {0, 0};
+      bool stop = false, issued = false;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (stop || *abort_flag || !mbar_wait(bar, parity)) {
+          if (!stop) fail();
+          stop = true;
+        }
+        fence_after();
+        return !stop;
+      };
+      auto ring_at = [&](int64_t i) { return smem_u32(ring + static_cast<int>(i % G::kStages) * G::kTileBytes); };
+      auto wait_full = [&](int64_t i) {
+        return wait(full + 8 * static_cast<int>(i % G::kStages), static_cast<uint32_t>((i / G::kStages) & 1));
+      };
+      auto scores = [&](int x, int64_t i) {              // S_x = Q_x K^T, K in ring entry i
+        const uint32_t kb = ring_at(i), qb = smem_u32(q_tile) + x * G::kTileBytes;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = (ks / 4) * (kKT * 128) + (ks % 4) * 32;
+          mma_f16(tmem + x * 128, sdesc(qb + off, 0, 1024, 2), sdesc(kb + off, 0, 1024, 2), kIdS, ks > 0);
+        }
+        mma_commit(s_full + 8 * x);
+        issued = true;
+      };
+      while (w.u < w.end && !stop) {
+        const int rows = min(tt, w.n - w.tile * tt) * p.group, streams = rows > 128 ? 2 : 1;
+        const int64_t end = min(w.end, w.item_first + w.units);
+        bool fresh[2] = {true, true};
+        if (!wait_full(g)) break;
+        for (int x = 0; x < streams; ++x) {
+          if (!wait(q_full + 8 * x, q_ph[x])) break;
+          q_ph[x] ^= 1u;
+          scores(x, g);
+        }
+        if (stop) break;
+        mma_commit(empty + 8 * static_cast<int>(g % G::kStages));
+        for (; w.u < end && !stop; ++w.u, g += 2) {
+          const bool more = w.u + 1 < end;
+          for (int x = 0; x < streams; ++x) {
+            if (!wait_full(g + 1) || !wait(p_full + 8 * x, p_ph[x])) break;
+            p_ph[x] ^= 1u;
+            if (odd_tile[x] != tile_name(g)) {
+              const uint32_t vb = ring_at(g + 1);
+#pragma unroll
+              for (int ks = 0; ks < kKT / 16; ++ks)      // 16 slots a step; N chunks of 64 columns 16 KB apart
+                mma_f16_ta(tmem + 256 + x * D, tmem + x * 128 + ks * 8, sdesc(vb + ks * 2048, kKT * 128, 1024, 2), kIdO,
+                           (!fresh[x] || ks > 0) ? 1u : 0u);
+            }
+            fresh[x] = false;
+            if (x == streams - 1) mma_commit(empty + 8 * static_cast<int>((g + 1) % G::kStages));
+            if (more) {
+              if (!wait_full(g + 2)) break;
+              scores(x, g + 2);
+              if (x == streams - 1) mma_commit(empty + 8 * static_cast<int>((g + 2) % G::kStages));
+            } else {
+              mma_commit(o_full + 8 * x);
+            }
+          }
+        }
+        if (!stop && w.u < w.end) paged_next_item(p, tt, kKT, w);
+      }
+      // after a failed wait: the commit arrives once every MMA issued before it is done
+      if (issued && stop) {
+        mma_commit(drain);
+        mbar_wait(drain, 0);
+      }
+    }
+  }
+  } else {
+    regs_up<208>();
+    // ---------------- softmax and epilogue of stream x ----------------
+    const int x = warp >> 2, r = (warp & 3) * 32 + lane;  // row of the stream, its TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + x * 128, o_addr = tmem + lane_base + 256 + x * D;
+    const float c = p.inv_scale * kLog2e;
+    uint32_t s_ph = 0, o_ph = 0, v_ph = 0;
+    int64_t g = 0;                                        // ring entry of the current unit's K
+    bool stop = false;
+    // the same answer in every lane: what follows is done by whole warps
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      const bool ok = !*abort_flag && mbar_wait(bar, parity);
+      if (!__all_sync(0xffffffffu, ok)) {
+        fail();
+        stop = true;
+      }
+      fence_after();
+      return !stop;
+    };
+    for (int slot = 0; any && w.u < w.end && !stop; slot = 1) {
+      const int tok0 = w.tile * tt, rows = min(tt, w.n - tok0) * p.group;
+      const int64_t from = w.u, end = min(w.end, w.item_first + w.units);
+      if (x == 1 && rows <= 128) {                        // nothing for this stream here
+        g += 2 * (end - from);
+        w.u = end;
+        if (w.u < w.end) paged_next_item(p, tt, kKT, w);
+        continue;
+      }
+      const int row = x * 128 + r;
+      const bool live = row < rows;
+      const int tok = tok0 + min(row, rows - 1) / p.group, head = w.head * p.group + row % p.group;
+      const int lim = p.causal ? max(w.len - w.n + tok + 1, 0) : w.len;     // slots this row sees
+      const int lim0 = p.causal ? max(w.len - w.n + tok0 + (x * 128) / p.group + 1, 0) : w.len;   // the stream's first row
+      // ---- Q ----
+      {
+        unsigned char* dst = q_tile + x * G::kTileBytes + r * 128;
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (w.q0 + tok) * p.q_sn +
+                                                          static_cast<int64_t>(head) * p.q_sh);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 f = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(dst + (i / 8) * (kKT * 128) + (((i % 8) ^ (r & 7)) << 4)) = f;
+        }
+        fence_proxy_async();
+        fence_before();
+        mbar_arrive(q_full + 8 * x);
+      }
+      float m = -INFINITY, l = 0.f;
+      for (; w.u < end; ++w.u, g += 2) {
+        const int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+        if (!wait(s_full + 8 * x, s_ph)) break;
+        s_ph ^= 1u;
+        float s[kKT];
+        {
+          uint32_t v[4][32];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld32_async(s_addr + 32 * i, v[i]);
+          tmem_wait();
+#pragma unroll
+          for (int j = 0; j < kKT; ++j) s[j] = __uint_as_float(v[j / 32][j % 32]);
+        }
+        const bool masked = k0 + kKT > lim0;              // the same for the whole stream
+        if (masked) {
+          const int see = lim - k0;
+#pragma unroll
+          for (int j = 0; j < kKT; ++j) s[j] = j < see ? s[j] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int j = 4; j < kKT; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        const bool raise = top > m + kSlack;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float mn = raise ? top : m;
+          const float f = m == -INFINITY ? 0.f : ex2_approx(m - mn);       // 1 where the row keeps its maximum
+          m = mn;
+          l *= f;
+          if (w.u > from) {                               // the PV of the tile before is done: S of this one came after it
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              uint32_t o[16];
+              tmem_ld16_async(o_addr + c0, o);
+              tmem_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(o_addr + c0, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        const float off = (m == -INFINITY ? 0.f : m) - kShift;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float a = ex2_approx(fmaf(s[32 * i + 2 * j], c, -off));
+            const float b = ex2_approx(fmaf(s[32 * i + 2 * j + 1], c, -off));
+            sum[j & 3] += a + b;
+            pk[j] = pack2<T>(a, b);
+          }
+          tmem_st16(s_addr + 16 * i, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        if (masked) {
+          // a non-finite value in V, perhaps hidden from this row or another?
+          const int64_t e = g + 1;
+          const int st = static_cast<int>(e % G::kStages);
+          if (!wait(full + 8 * st, static_cast<uint32_t>((e / G::kStages) & 1))) break;
+          const unsigned char* v = ring + st * G::kTileBytes;
+          uint32_t odd = 0;
+          for (int i = r; i < G::kTileBytes / 16; i += 128) {
+            const uint4 a = *reinterpret_cast<const uint4*>(v + i * 16);
+            odd |= ((a.x & Half16<T>::kExp) + Half16<T>::kOne) | ((a.y & Half16<T>::kExp) + Half16<T>::kOne) |
+                   ((a.z & Half16<T>::kExp) + Half16<T>::kOne) | ((a.w & Half16<T>::kExp) + Half16<T>::kOne);
+          }
+          if (odd & 0x80008000u) odd_tile[x] = tile_name(g);
+          mbar_arrive(v_seen + 8 * x);
+          if (!wait(v_seen + 8 * x, v_ph)) break;
+          v_ph ^= 1u;
+          if (odd_tile[x] == tile_name(g)) visible_product<T, D>(s_addr, o_addr, v, lim - k0, w.u == from);
+        }
+        fence_before();
+        mbar_arrive(p_full + 8 * x);
+      }
+      if (stop) break;
+      // ---- epilogue ----
+      if (!wait(o_full + 8 * x, o_ph)) break;
+      o_ph ^= 1u;
+      const bool whole = from == w.item_first && end == w.item_first + w.units;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* out = static_cast<T*>(p.out) + (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh;
+      float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + row) * (D + 2);
+#pragma unroll
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32_async(o_addr + c0, o);
+        tmem_wait();
+        if (!live) continue;
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 f;
+            f.x = pack2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+            f.y = pack2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+            f.z = pack2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+            f.w = pack2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + c0 + i) = f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            *reinterpret_cast<float2*>(part + c0 + i) = make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+        }
+      }
+      if (live) {
+        if (whole) {
+          const int64_t at = (w.q0 + tok) * (static_cast<int64_t>(p.c.h_kv) * p.group) + head;
+          const float z = l == 0.f ? -INFINITY : m - kShift + log2f(l);
+          if (p.lse) p.lse[at] = z * kLn2;
+          if (p.lse2) p.lse2[at] = z;
+        } else {
+          part[D] = m - kShift;
+          part[D + 1] = l;
+        }
+      }
+      if (w.u < w.end) paged_next_item(p, tt, kKT, w);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// The pages as a 4-D tensor of (d, slot and head by ascending stride, page),
+// boxes of 64 columns x one page (at most 128 slots).
+bool page_map(const PagedCacheParams& c, const void* base, int64_t sp, int64_t sn, int64_t sh, ssa_dtype dt,
+              CUtensorMap* map, MapOrder* mo) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  // strides of dimensions with one entry do not matter
+  if (c.h_kv == 1) sh = sn * c.page_size;
+  const bool head_first = sh < sn;
+  mo->head_first = head_first;
+  const int64_t s1 = head_first ? sh : sn, s2 = head_first ? sn : sh;
+  const cuuint64_t n1 = head_first ? c.h_kv : c.page_size, n2 = head_first ? c.page_size : c.h_kv;
+  if (s1 < c.d || s2 < s1 * static_cast<int64_t>(n1)) return false;
+  if (c.num_pages == 1) sp = s2 * static_cast<int64_t>(n2);
+  if (sp < s2 || sp * 2 >= (1ll << 40)) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.d), n1, n2, static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s1) * 2, static_cast<cuuint64_t>(s2) * 2,
+                                 static_cast<cuuint64_t>(sp) * 2};
+  const cuuint32_t rows = c.page_size < kKT ? c.page_size : kKT;
+  const cuuint32_t box[4] = {64, head_first ? 1 : rows, head_first ? rows : 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = dt == SSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, t, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st) {
+  CUtensorMap km, vm;
+  MapOrder mo, vo;
+  if (!page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, &km, &mo) ||
+      !page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, &vm, &vo) || mo.head_first != vo.head_first)
+    return cudaErrorInvalidValue;
+  auto kern = attn_tc_kernel<T, D>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(Geo<D>::kSmem));
+  if (e != cudaSuccess) return e;
+  kern<<<grid, kThreads, Geo<D>::kSmem, st>>>(km, vm, p, mo);
+  return cudaGetLastError();
+}
+
+}  // namespace ptc
+
+bool paged_attn_tc_supported(const PagedAttnParams& p, ssa_dtype dt) {
+  if (dt != SSA_BF16 && dt != SSA_F16) return false;
+  if (p.c.d != 64 && p.c.d != 128) return false;
+  if (p.c.page_shift < 3 || p.c.num_pages < 1 || !(p.inv_scale > 0.f)) return false;
+  CUtensorMap m;
+  ptc::MapOrder a, b;
+  return ptc::page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, &m, &a) &&
+         ptc::page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, &m, &b) && a.head_first == b.head_first;
+}
+
+cudaError_t launch_paged_attn_tc(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st) {
+  if (dt == SSA_BF16)
+    return p.c.d == 128 ? ptc::launch_t<__nv_bfloat16, 128>(p, dt, grid, st) : ptc::launch_t<__nv_bfloat16, 64>(p, dt, grid, st);
+  return p.c.d == 128 ? ptc::launch_t<__half, 128>(p, dt, grid, st) : ptc::launch_t<__half, 64>(p, dt, grid, st);
+}
+
+}  // namespace ssa
