@@ -56,6 +56,7 @@ struct PagedAttnParams {
   float* lse2;                     // [rows, h_q] row log2-sum-exp2 for the weights pass, or NULL
   float* part;                     // [grid][2][tile rows][d + 2]: unnormalised row, maximum (log2), sum
   PagedSplit* split;               // [grid]
+  float* scores;                   // [rows, h_q, slots of a table row] scaled logits (base 2), or NULL
   int64_t rows;
   int group, causal;
   float inv_scale;
@@ -299,7 +300,9 @@ cudaError_t launch_paged_evict(const PagedEvictParams& p, ssa_dtype dt, cudaStre
 size_t paged_attn_workspace(const PagedAttnParams& p, ssa_dtype dt);
 cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st);
 // Chunks on the tensor cores (paged_attn_tc.cu), 256 rows an item, one CTA per SM.
-bool paged_attn_tc_supported(const PagedAttnParams& p, ssa_dtype dt);
 cudaError_t launch_paged_attn_tc(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st);
+// Few rows (paged_attn_dec.cu), 16 an item; the slot weights from the scores it leaves.
+cudaError_t launch_paged_attn_dec(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st);
+cudaError_t launch_paged_weights_dec(const PagedAttnParams& p, cudaStream_t st);
 
 }  // namespace ssa

@@ -14,6 +14,7 @@
 
 #include "common.cuh"
 #include "paged.cuh"
+#include "paged_tma.cuh"
 
 namespace ssa {
 namespace {
@@ -303,29 +304,43 @@ __global__ void __launch_bounds__(128) combine_kernel(PagedAttnParams p, int R) 
   const int tok0 = it.tile * tt, rows = min(tt, q.n - tok0) * p.group;
   const int slot0 = before.item_first == it.item_first ? 0 : 1;    // CTA b - 1: is it also that CTA's first item
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+  const int parts = it.cta_last - b + 2;                            // CTAs b - 1 .. cta_last
+  auto row_of = [&](int i, int r) {                                 // part i of row r
+    return p.part + (static_cast<int64_t>((b - 1 + i) * 2 + (i == 0 ? slot0 : 0)) * R + r) * (d + 2);
+  };
   for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
     float m = -INFINITY;
-    for (int c = b - 1; c <= it.cta_last; ++c)
-      m = fmaxf(m, p.part[(static_cast<int64_t>(c * 2 + (c == b - 1 ? slot0 : 0)) * R + r) * (d + 2) + d]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[8];
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, row_of(i, r)[d]);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) o[x] = 0.f;
-    for (int c = b - 1; c <= it.cta_last; ++c) {
-      const float* src = p.part + (static_cast<int64_t>(c * 2 + (c == b - 1 ? slot0 : 0)) * R + r) * (d + 2);
+    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float2 o[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[x] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+      const float* src = row_of(i, r);
       const float f = exp2f(src[d] - base);
       l = fmaf(f, src[d + 1], l);
 #pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (lane + 32 * x < d) o[x] = fmaf(f, src[lane + 32 * x], o[x]);
+      for (int x = 0; x < 4; ++x)
+        if (2 * lane + 64 * x < d) {
+          const float2 a = *reinterpret_cast<const float2*>(src + 2 * lane + 64 * x);
+          o[x].x = fmaf(f, a.x, o[x].x);
+          o[x].y = fmaf(f, a.y, o[x].y);
+        }
     }
     const int64_t tok = q.q0 + tok0 + r / p.group;
     const int head = it.head * p.group + r % p.group;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* dst = static_cast<T*>(p.out) + tok * p.o_sn + head * p.o_sh;
 #pragma unroll
-    for (int x = 0; x < 8; ++x)
-      if (lane + 32 * x < d) dst[lane + 32 * x] = Elem<T>::from_f(o[x] * inv);
+    for (int x = 0; x < 4; ++x)
+      if (2 * lane + 64 * x < d) {
+        dst[2 * lane + 64 * x] = Elem<T>::from_f(o[x].x * inv);
+        dst[2 * lane + 64 * x + 1] = Elem<T>::from_f(o[x].y * inv);
+      }
     if (lane == 0) store_lse(p, tok, head, m, l);
   }
 }
@@ -426,24 +441,28 @@ cudaError_t launch_simt_t(const PagedAttnParams& p, ssa_dtype dt, int grid, bool
 }
 
 // The kernel that serves a call, its tile rows and grid, and the workspace.
+enum class AttnKernel { kSimt, kTokens, kChunks };
 struct AttnPlan {
-  bool tc;
+  AttnKernel kernel;
   int rows, grid;
-  size_t split, lse2, total;
+  size_t split, lse2, scores, total;
 };
 
-// More than 16 rows (new tokens x heads of a group) per sequence on average:
-// tiles of many rows, on the tensor cores where they apply.
+// More than 16 rows (new tokens x heads of a group) per sequence on average
+// take tiles of many rows; 16-bit caches that page tiles fit, the tensor cores.
 AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   AttnPlan a{};
   const bool chunks = p.rows * p.group > 16ll * p.c.batch;
-  a.tc = chunks && paged_attn_tc_supported(p, dt);
-  a.rows = a.tc ? 256 : chunks ? 64 : 16;
-  a.grid = a.tc ? 148 : 2 * 148;
+  a.kernel = !page_tiles_supported(p, dt) ? AttnKernel::kSimt : chunks ? AttnKernel::kChunks : AttnKernel::kTokens;
+  a.rows = !chunks ? 16 : a.kernel == AttnKernel::kChunks ? 256 : 64;
+  a.grid = a.kernel == AttnKernel::kSimt ? 2 * 148 : 148;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t lines = static_cast<size_t>(p.rows) * p.c.h_kv * p.group;
   a.split = up(static_cast<size_t>(a.grid) * 2 * a.rows * (p.c.d + 2) * 4);
   a.lse2 = a.split + up(a.grid * sizeof(PagedSplit));
-  a.total = a.lse2 + (p.c.w ? up(static_cast<size_t>(p.rows) * p.c.h_kv * p.group * 4) : 0);
+  a.scores = a.lse2 + (p.c.w ? up(lines * 4) : 0);
+  a.total = a.scores;
+  if (p.c.w && a.kernel == AttnKernel::kTokens) a.total += up(lines * p.c.max_pages * p.c.page_size * 4);
   return a;
 }
 
@@ -457,11 +476,16 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
   p.part = reinterpret_cast<float*>(at);
   p.split = reinterpret_cast<PagedSplit*>(at + a.split);
   p.lse2 = p.c.w ? reinterpret_cast<float*>(at + a.lse2) : nullptr;
-  cudaError_t e = a.tc           ? launch_paged_attn_tc(p, dt, a.grid, st)
-                  : a.rows == 64 ? launch_simt_t<64>(p, dt, a.grid, false, st)
-                                 : launch_simt_t<16>(p, dt, a.grid, false, st);
+  p.scores = a.total > a.scores ? reinterpret_cast<float*>(at + a.scores) : nullptr;
+  cudaError_t e;
+  switch (a.kernel) {
+    case AttnKernel::kChunks: e = launch_paged_attn_tc(p, dt, a.grid, st); break;
+    case AttnKernel::kTokens: e = launch_paged_attn_dec(p, dt, a.grid, st); break;
+    default:
+      e = a.rows == 64 ? launch_simt_t<64>(p, dt, a.grid, false, st) : launch_simt_t<16>(p, dt, a.grid, false, st);
+  }
   if (e != cudaSuccess) return e;
-  const dim3 grid(a.grid - 1, a.rows / 16);
+  const dim3 grid(a.grid - 1, a.rows == 16 ? 4 : a.rows / 16);
   switch (dt) {
     case SSA_F32: combine_kernel<float><<<grid, 128, 0, st>>>(p, a.rows); break;
     case SSA_BF16: combine_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p, a.rows); break;
@@ -469,6 +493,7 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
   }
   e = cudaGetLastError();
   if (e != cudaSuccess || !p.c.w) return e;
+  if (p.scores) return launch_paged_weights_dec(p, st);
   return a.rows >= 64 ? launch_simt_t<64>(p, dt, 0, true, st) : launch_simt_t<16>(p, dt, 0, true, st);
 }
 

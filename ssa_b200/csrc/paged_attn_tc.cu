@@ -38,15 +38,12 @@
 // Every wait is bounded (about one second); on expiry the CTA records
 // SSA_DEVICE_TIMEOUT, waits (bounded) for its copies and MMAs in flight, frees
 // TMEM and exits.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
 #include "mma_utils.cuh"
 #include "paged.cuh"
+#include "paged_tma.cuh"
 #include "tc_utils.cuh"
 
 namespace ssa {
@@ -68,18 +65,6 @@ struct Geo {
   static constexpr size_t kSmem = 1024 + 2 * kTileBytes + static_cast<size_t>(kStages) * kTileBytes + 512;
 };
 
-// Coordinates of a page box in its 4-D tensor map (d, two of {slot, head}, page).
-struct MapOrder {
-  int head_first;                  // 1: the head dimension has the smaller stride
-};
-
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x, int y, int z, int w, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-      : "memory");
-}
 // A from TMEM, B from shared memory.
 __device__ __forceinline__ void mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bd, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -107,35 +92,11 @@ template <int D>
 __device__ __forceinline__ void load_kv(const PagedAttnParams& p, const MapOrder& mo, const void* map, int seq, int head,
                                         int k0, int lim, uint32_t dst, uint32_t bar) {
   const int lane = threadIdx.x & 31;
-  const int rows = min(p.c.page_size, kKT), pieces = kKT / rows, boxes = pieces * (D / 64);
+  const int pieces = kKT / min(p.c.page_size, kKT), boxes = pieces * (D / 64);
   if (lane == 0) mbar_expect_tx(bar, Geo<D>::kTileBytes);
   __syncwarp();
-  if (lane < boxes) {
-    const int piece = lane & (pieces - 1), half = lane / pieces;
-    const int j = k0 + piece * rows;
-    int pg = -1, row = 0;
-    // a page outside the table's use reads as zeros (a coordinate out of range)
-    if (j < lim) {
-      int lp;
-      page_of(p.c, j, lp, row);
-      pg = static_cast<int>(physical_page(p.c, p.c.table, p.c.table_stride, seq, lp));
-    }
-    tma_load_4d(dst + half * (kKT * 128) + piece * rows * 128, map, half * 64, mo.head_first ? head : row,
-                mo.head_first ? row : head, pg, bar);
-  }
-}
-
-template <typename T>
-struct Half16;
-template <> struct Half16<__nv_bfloat16> { static constexpr uint32_t kExp = 0x7f807f80u, kOne = 0x00800080u; };
-template <> struct Half16<__half> { static constexpr uint32_t kExp = 0x7c007c00u, kOne = 0x04000400u; };
-
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  else
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  if (lane < boxes)
+    load_box<kKT>(p, mo, map, seq, head, k0, lim, lane & (pieces - 1), lane / pieces, dst, bar);
 }
 
 // The tile's O += P V for this thread's row over its first `see` slots, on the
@@ -469,10 +430,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           uint32_t odd = 0;
           for (int i = r; i < G::kTileBytes / 16; i += 128) {
             const uint4 a = *reinterpret_cast<const uint4*>(v + i * 16);
-            odd |= ((a.x & Half16<T>::kExp) + Half16<T>::kOne) | ((a.y & Half16<T>::kExp) + Half16<T>::kOne) |
-                   ((a.z & Half16<T>::kExp) + Half16<T>::kOne) | ((a.w & Half16<T>::kExp) + Half16<T>::kOne);
+            odd |= odd_bits<T>(a.x) | odd_bits<T>(a.y) | odd_bits<T>(a.z) | odd_bits<T>(a.w);
           }
-          if (odd & 0x80008000u) odd_tile[x] = tile_name(g);
+          if (odd) odd_tile[x] = tile_name(g);
           mbar_arrive(v_seen + 8 * x);
           if (!wait(v_seen + 8 * x, v_ph)) break;
           v_ph ^= 1u;
@@ -533,52 +493,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  });
-  return fn;
-}
-
-// The pages as a 4-D tensor of (d, slot and head by ascending stride, page),
-// boxes of 64 columns x one page (at most 128 slots).
-bool page_map(const PagedCacheParams& c, const void* base, int64_t sp, int64_t sn, int64_t sh, ssa_dtype dt,
-              CUtensorMap* map, MapOrder* mo) {
-  auto enc = encode_fn();
-  if (!enc) return false;
-  // strides of dimensions with one entry do not matter
-  if (c.h_kv == 1) sh = sn * c.page_size;
-  const bool head_first = sh < sn;
-  mo->head_first = head_first;
-  const int64_t s1 = head_first ? sh : sn, s2 = head_first ? sn : sh;
-  const cuuint64_t n1 = head_first ? c.h_kv : c.page_size, n2 = head_first ? c.page_size : c.h_kv;
-  if (s1 < c.d || s2 < s1 * static_cast<int64_t>(n1)) return false;
-  if (c.num_pages == 1) sp = s2 * static_cast<int64_t>(n2);
-  if (sp < s2 || sp * 2 >= (1ll << 40)) return false;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.d), n1, n2, static_cast<cuuint64_t>(c.num_pages)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s1) * 2, static_cast<cuuint64_t>(s2) * 2,
-                                 static_cast<cuuint64_t>(sp) * 2};
-  const cuuint32_t rows = c.page_size < kKT ? c.page_size : kKT;
-  const cuuint32_t box[4] = {64, head_first ? 1 : rows, head_first ? rows : 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType t = dt == SSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return enc(map, t, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int D>
 cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st) {
   CUtensorMap km, vm;
   MapOrder mo, vo;
-  if (!page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, &km, &mo) ||
-      !page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, &vm, &vo) || mo.head_first != vo.head_first)
+  if (!page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, kKT, &km, &mo) ||
+      !page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, kKT, &vm, &vo) || mo.head_first != vo.head_first)
     return cudaErrorInvalidValue;
   auto kern = attn_tc_kernel<T, D>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -589,16 +509,6 @@ cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStrea
 }
 
 }  // namespace ptc
-
-bool paged_attn_tc_supported(const PagedAttnParams& p, ssa_dtype dt) {
-  if (dt != SSA_BF16 && dt != SSA_F16) return false;
-  if (p.c.d != 64 && p.c.d != 128) return false;
-  if (p.c.page_shift < 3 || p.c.num_pages < 1 || !(p.inv_scale > 0.f)) return false;
-  CUtensorMap m;
-  ptc::MapOrder a, b;
-  return ptc::page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, &m, &a) &&
-         ptc::page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, &m, &b) && a.head_first == b.head_first;
-}
 
 cudaError_t launch_paged_attn_tc(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st) {
   if (dt == SSA_BF16)

@@ -1,0 +1,122 @@
+// Page tiles by TMA, shared by the paged attention kernels: the tensor map over
+// the pages, and the boxes of one key tile.
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "common.cuh"
+#include "paged.cuh"
+#include "tc_utils.cuh"
+
+namespace ssa {
+
+// Coordinates of a page box in its 4-D tensor map (d, two of {slot, head}, page).
+struct MapOrder {
+  int head_first;                  // 1: the head dimension has the smaller stride
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
+// The box of one 64-column half of one page piece of a tile of KT slots
+// (shared layout [D / 64][KT][128 bytes], SWIZZLE_128B).  Slots from `lim` on
+// that lie in no page of the sequence, and bad pages, read as zeros (a page
+// coordinate out of range).
+template <int KT>
+__device__ __forceinline__ void load_box(const PagedAttnParams& p, const MapOrder& mo, const void* map, int seq,
+                                         int head, int k0, int lim, int piece, int half, uint32_t dst, uint32_t bar) {
+  const int rows = min(p.c.page_size, KT);
+  const int j = k0 + piece * rows;
+  int pg = -1, row = 0;
+  if (j < lim) {
+    int lp;
+    page_of(p.c, j, lp, row);
+    pg = static_cast<int>(physical_page(p.c, p.c.table, p.c.table_stride, seq, lp));
+  }
+  tma_load_4d(dst + half * (KT * 128) + piece * rows * 128, map, half * 64, mo.head_first ? head : row,
+              mo.head_first ? row : head, pg, bar);
+}
+
+// Non-finite 16-bit values: all exponent bits set.  (x & kExp) + kOne carries
+// into a half's top bit exactly then.
+template <typename T>
+struct Half16;
+template <> struct Half16<__nv_bfloat16> { static constexpr uint32_t kExp = 0x7f807f80u, kOne = 0x00800080u; };
+template <> struct Half16<__half> { static constexpr uint32_t kExp = 0x7c007c00u, kOne = 0x04000400u; };
+template <typename T>
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+  return ((w & Half16<T>::kExp) + Half16<T>::kOne) & 0x80008000u;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// The pages as a 4-D tensor of (d, slot and head by ascending stride, page),
+// boxes of 64 columns x one page (at most kt slots).  False: not such a tensor.
+inline bool page_map(const PagedCacheParams& c, const void* base, int64_t sp, int64_t sn, int64_t sh, ssa_dtype dt,
+                     int kt, CUtensorMap* map, MapOrder* mo) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return false;
+  // strides of dimensions with one entry do not matter
+  if (c.h_kv == 1) sh = sn * c.page_size;
+  const bool head_first = sh < sn;
+  mo->head_first = head_first;
+  const int64_t s1 = head_first ? sh : sn, s2 = head_first ? sn : sh;
+  const cuuint64_t n1 = head_first ? c.h_kv : c.page_size, n2 = head_first ? c.page_size : c.h_kv;
+  if (s1 < c.d || s2 < s1 * static_cast<int64_t>(n1)) return false;
+  if (c.num_pages == 1) sp = s2 * static_cast<int64_t>(n2);
+  if (sp < s2 || sp * 2 >= (1ll << 40)) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.d), n1, n2, static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s1) * 2, static_cast<cuuint64_t>(s2) * 2,
+                                 static_cast<cuuint64_t>(sp) * 2};
+  const cuuint32_t rows = c.page_size < kt ? c.page_size : kt;
+  const cuuint32_t box[4] = {64, head_first ? 1 : rows, head_first ? rows : 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = dt == SSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, t, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What the kernels on page tiles need of a cache: 16-bit rows of 64 or 128,
+// pages of a power of two of at least 8 slots, strides a tensor map takes.
+inline bool page_tiles_supported(const PagedAttnParams& p, ssa_dtype dt) {
+  if (dt != SSA_BF16 && dt != SSA_F16) return false;
+  if (p.c.d != 64 && p.c.d != 128) return false;
+  if (p.c.page_shift < 3 || p.c.num_pages < 1 || !(p.inv_scale > 0.f)) return false;
+  CUtensorMap m;
+  MapOrder a, b;
+  return page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, 64, &m, &a) &&
+         page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, 64, &m, &b) && a.head_first == b.head_first;
+}
+
+}  // namespace ssa
