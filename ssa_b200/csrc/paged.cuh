@@ -301,8 +301,11 @@ size_t paged_attn_workspace(const PagedAttnParams& p, ssa_dtype dt);
 cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st);
 // Chunks on the tensor cores (paged_attn_tc.cu), 256 rows an item, one CTA per SM.
 cudaError_t launch_paged_attn_tc(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st);
-// Few rows (paged_attn_dec.cu), 16 an item; the slot weights from the scores it leaves.
+// Few rows (paged_attn_dec.cu), 16 an item; the slot weights from the scores it
+// leaves, and those of chunks from scores made again (paged_weights_tc.cu).
 cudaError_t launch_paged_attn_dec(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st);
+bool paged_weights_tc_supported(const PagedAttnParams& p, ssa_dtype dt);
+cudaError_t launch_paged_weights_tc(const PagedAttnParams& p, ssa_dtype dt, cudaStream_t st);
 cudaError_t launch_paged_weights_dec(const PagedAttnParams& p, cudaStream_t st);
 
 }  // namespace ssa

@@ -494,6 +494,7 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
   e = cudaGetLastError();
   if (e != cudaSuccess || !p.c.w) return e;
   if (p.scores) return launch_paged_weights_dec(p, st);
+  if (a.kernel == AttnKernel::kChunks && paged_weights_tc_supported(p, dt)) return launch_paged_weights_tc(p, dt, st);
   return a.rows >= 64 ? launch_simt_t<64>(p, dt, 0, true, st) : launch_simt_t<16>(p, dt, 0, true, st);
 }
 

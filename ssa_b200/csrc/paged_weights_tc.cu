@@ -1,0 +1,347 @@
+// Slot weights of chunks on the 5th-generation tensor cores: bf16 / fp16, head
+// size 64 or 128, page tiles (paged_tma.cuh).
+//
+//   w_j += sum_i exp2(s_ij log2 e - lse2_i) over the rows i that see slot j,
+//
+// with lse2_i from the attention kernel.  The scores are made again, transposed:
+// S^T = K Q^T puts a slot in every TMEM lane and the rows in its columns, so
+// the sum over rows is a thread's own, with no exchange between lanes and no
+// atomics between CTAs: one CTA has all rows of its slots, in one order.
+//
+// An item is 256 slots of one (sequence, KV head): two streams of 128 slots
+// share every tile of Q rows (the g heads of a group at floor(128 / g) tokens).
+// Per row tile and stream the tensor cores do 128 x 128 x d products, the MUFU
+// 128 x 128 exponentials, which bound it (1024 clocks against 512 at d = 128).
+//
+//   warps 0-3, 4-7  streams: a slot per thread; scores from TMEM, two buffers each
+//   warp 8          TMEM allocation, single-thread MMA issue
+//   warp 9          TMA producer: K (two items deep), Q rows and their lse2 (ring of 3)
+//
+// Every wait is bounded (about one second); on expiry the CTA records
+// SSA_DEVICE_TIMEOUT and runs to its end without further waits or copies.
+#include <type_traits>
+
+#include "common.cuh"
+#include "mma_utils.cuh"
+#include "paged.cuh"
+#include "paged_tma.cuh"
+#include "tc_utils.cuh"
+
+namespace ssa {
+namespace pwt {
+
+using namespace tc;
+
+constexpr int kSlots = 128;        // of a stream
+constexpr int kRows = 128;         // of a Q tile
+constexpr int kThreads = 320;
+constexpr int kQStages = 3;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct Geo {
+  static constexpr int kTileBytes = 128 * D * 2;
+  static constexpr size_t kSmem = 1024 + (4 + kQStages) * static_cast<size_t>(kTileBytes) + kQStages * kRows * 4 + 256;
+};
+
+struct QueryMap {
+  int tokens;                      // per Q tile
+  int head_first;                  // row r of a tile: token r / g, head r % g; else token r % tokens, head r / tokens
+};
+
+// Item i of the call: 256 slots of a (sequence, KV head).  Items of a sequence
+// run tile by tile, heads inside, later tiles (seen by fewer rows) last.
+struct Items {
+  int64_t base;                    // items of the sequences before `seq`
+  int seq;
+  PagedSeq q;
+};
+__device__ __forceinline__ int64_t items_of(const PagedAttnParams& p, const PagedSeq& q) {
+  return q.n > 0 ? static_cast<int64_t>((q.len + 2 * kSlots - 1) / (2 * kSlots)) * p.c.h_kv : 0;
+}
+__device__ __forceinline__ bool seek(const PagedAttnParams& p, Items& it, int64_t i) {
+  while (it.seq < p.c.batch) {
+    if (it.seq >= 0) {
+      const int64_t n = items_of(p, it.q);
+      if (i < it.base + n) return true;
+      it.base += n;
+    }
+    if (++it.seq < p.c.batch) it.q = paged_seq(p.c, p.q_starts, p.rows, it.seq);
+  }
+  return false;
+}
+// First token of the sequence that sees slot k0 (q.n if none does).
+__device__ __forceinline__ int first_token(const PagedAttnParams& p, const PagedSeq& q, int k0) {
+  if (!p.causal) return 0;
+  const int64_t t = static_cast<int64_t>(k0) - (static_cast<int64_t>(q.len) - q.n);
+  return t < 0 ? 0 : t > q.n ? q.n : static_cast<int>(t);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                                 const __grid_constant__ CUtensorMap qmap,
+                                                                 PagedAttnParams p, MapOrder mo, QueryMap qm) {
+  using G = Geo<D>;
+  constexpr uint32_t kId = idesc_f16(128, kRows, std::is_same<T, __nv_bfloat16>::value);
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  unsigned char* q_ring = base + 4 * G::kTileBytes;      // base: K [2 items][2 streams]
+  float* z_ring = reinterpret_cast<float*>(q_ring + kQStages * G::kTileBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(z_ring + kQStages * kRows);
+  const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, q_full = k_empty + 16, q_empty = q_full + 8 * kQStages;
+  const uint32_t s_full = q_empty + 8 * kQStages, s_empty = s_full + 32;     // [stream][buffer]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 2 * kQStages + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
+  const int g = p.group, tt = qm.tokens;
+
+  // rows of a Q slot that no box fills (tokens * g < 128) read as zero queries
+  for (int i = threadIdx.x; i < kQStages * G::kTileBytes / 16; i += kThreads)
+    reinterpret_cast<uint4*>(q_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async();
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(k_full + 8 * b, 1);
+      mbar_init(k_empty + 8 * b, 1);
+    }
+    for (int s = 0; s < kQStages; ++s) {
+      mbar_init(q_full + 8 * s, 1 + 32);                 // the copies' bytes, and the lse2 of 32 lanes
+      mbar_init(q_empty + 8 * s, 1 + 8);                 // the MMAs, and the streams' warps
+    }
+    for (int b = 0; b < 4; ++b) {
+      mbar_init(s_full + 8 * b, 1);
+      mbar_init(s_empty + 8 * b, 4);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tensormap(&kmap);
+    prefetch_tensormap(&qmap);
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!*abort_flag && !mbar_wait(bar, parity)) {
+      *abort_flag = 1;
+      paged_error(p.c, SSA_DEVICE_TIMEOUT);
+    }
+  };
+  Items it{0, -1, {0, 0, 0}};
+  int64_t t = 0, n = 0;                                  // Q tiles and items so far
+
+  if (warp == 9) {
+    // ---------------- producer ----------------
+    const int pieces = kSlots / min(p.c.page_size, kSlots), boxes = pieces * (D / 64);
+    const int64_t h_q = static_cast<int64_t>(p.c.h_kv) * g;
+    const uint32_t q_bytes = static_cast<uint32_t>(tt * g) * 128 * (D / 64);
+    bool stop = false;
+    for (int64_t i = blockIdx.x; !stop && seek(p, it, i); i += gridDim.x, ++n) {
+      const int head = static_cast<int>((i - it.base) % p.c.h_kv);
+      const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots;
+      const int b = static_cast<int>(n & 1);
+      wait(k_empty + 8 * b, static_cast<uint32_t>((n >> 1) & 1) ^ 1u);
+      stop = __any_sync(0xffffffffu, *abort_flag);
+      if (stop) break;
+      if (lane == 0) mbar_expect_tx(k_full + 8 * b, 2 * G::kTileBytes);
+      __syncwarp();
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (lane < boxes)
+          load_box<kSlots>(p, mo, &kmap, it.seq, head, k0 + x * kSlots, it.q.len, lane & (pieces - 1), lane / pieces,
+                           smem_u32(base) + (2 * b + x) * G::kTileBytes, k_full + 8 * b);
+      for (int r = first_token(p, it.q, k0) / tt; r * tt < it.q.n; ++r, ++t) {
+        const int s = static_cast<int>(t % kQStages);
+        wait(q_empty + 8 * s, static_cast<uint32_t>((t / kQStages) & 1) ^ 1u);
+        stop = __any_sync(0xffffffffu, *abort_flag);
+        if (stop) break;
+        if (lane == 0) mbar_expect_tx(q_full + 8 * s, q_bytes);
+        __syncwarp();
+        const int64_t tok = it.q.q0 + static_cast<int64_t>(r) * tt;
+        if (lane < D / 64) {
+          const int y = head * g, zc = static_cast<int>(tok);
+          tma_load_3d(smem_u32(q_ring + s * G::kTileBytes) + lane * (kRows * 128), &qmap, lane * 64,
+                      qm.head_first ? y : zc, qm.head_first ? zc : y, q_full + 8 * s);
+        }
+        const int rows = min(tt, it.q.n - r * tt) * g;
+#pragma unroll
+        for (int e = lane; e < kRows; e += 32) {
+          const int a = qm.head_first ? e / g : e % tt, j = qm.head_first ? e % g : e / tt;
+          float z = INFINITY;                            // exp2(s - inf) = 0: no row
+          if (a * g < rows && j < g) z = p.lse2[(tok + a) * h_q + head * g + j];
+          z_ring[s * kRows + e] = z;
+        }
+        mbar_arrive(q_full + 8 * s);
+      }
+    }
+    // every issued copy lands before the CTA exits
+    for (int64_t r = n - (stop ? 0 : 1); lane == 0 && r >= 0 && r >= n - 2; --r)
+      if (r < n || stop) mbar_wait(k_full + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
+    for (int64_t r = t - 1; lane == 0 && r >= 0 && r >= t - kQStages; --r)
+      mbar_wait(q_full + 8 * static_cast<int>(r % kQStages), static_cast<uint32_t>((r / kQStages) & 1));
+  } else if (warp == 8) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      for (int64_t i = blockIdx.x; !*abort_flag && seek(p, it, i); i += gridDim.x, ++n) {
+        const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots;
+        const int b = static_cast<int>(n & 1);
+        wait(k_full + 8 * b, static_cast<uint32_t>((n >> 1) & 1));
+        for (int r = first_token(p, it.q, k0) / tt; r * tt < it.q.n && !*abort_flag; ++r, ++t) {
+          const int s = static_cast<int>(t % kQStages), sb = static_cast<int>(t & 1);
+          wait(q_full + 8 * s, static_cast<uint32_t>((t / kQStages) & 1));
+          const uint32_t qb = smem_u32(q_ring + s * G::kTileBytes);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            wait(s_empty + 8 * (2 * x + sb), static_cast<uint32_t>((t >> 1) & 1) ^ 1u);
+            if (*abort_flag) break;
+            fence_after();
+            const uint32_t kb = smem_u32(base) + (2 * b + x) * G::kTileBytes;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+              const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
+              mma_f16(tmem + (2 * x + sb) * 128, sdesc(kb + off, 0, 1024, 2), sdesc(qb + off, 0, 1024, 2), kId, ks > 0);
+            }
+            mma_commit(s_full + 8 * (2 * x + sb));
+          }
+          mma_commit(q_empty + 8 * s);
+        }
+        mma_commit(k_empty + 8 * b);
+      }
+      // the last commits arrive once every MMA is done; both buffers of K are
+      // then free (an item's k_empty is its n-th phase)
+      for (int64_t r = n - 1; r >= 0 && r >= n - 2; --r)
+        mbar_wait(k_empty + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
+    }
+  } else {
+    // ---------------- stream x: a slot per thread ----------------
+    const int x = warp >> 2, r0 = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const float c = p.inv_scale * kLog2e;
+    for (int64_t i = blockIdx.x; !__any_sync(0xffffffffu, *abort_flag) && seek(p, it, i); i += gridDim.x, ++n) {
+      const int head = static_cast<int>((i - it.base) % p.c.h_kv);
+      const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots, slot = k0 + x * kSlots + r0;
+      float total = 0.f;
+      for (int r = first_token(p, it.q, k0) / tt; r * tt < it.q.n; ++r, ++t) {
+        const int s = static_cast<int>(t % kQStages), sb = static_cast<int>(t & 1);
+        wait(q_full + 8 * s, static_cast<uint32_t>((t / kQStages) & 1));   // lse2 of the rows
+        wait(s_full + 8 * (2 * x + sb), static_cast<uint32_t>((t >> 1) & 1));
+        __syncwarp();
+        fence_after();
+        const int rows = min(tt, it.q.n - r * tt) * g;
+        const int64_t lim0 = p.causal ? static_cast<int64_t>(it.q.len) - it.q.n + r * tt + 1 : it.q.len;
+        const bool masked = lim0 < k0 + (x + 1) * kSlots || rows < tt * g;
+        const float4* zs = reinterpret_cast<const float4*>(z_ring + s * kRows);
+        const uint32_t ta = tmem + lane_base + (2 * x + sb) * 128;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t v[2][32];
+        tmem_ld32_async(ta, v[0]);
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          tmem_wait();
+          if (q4 < 3) tmem_ld32_async(ta + 32 * (q4 + 1), v[(q4 + 1) & 1]);
+          if (!masked) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 z = zs[q4 * 8 + j];
+              sum[0] += ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j]), c, -z.x));
+              sum[1] += ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 1]), c, -z.y));
+              sum[2] += ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 2]), c, -z.z));
+              sum[3] += ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 3]), c, -z.w));
+            }
+          } else {
+            const float* z1 = z_ring + s * kRows + 32 * q4;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int e = 32 * q4 + j, a = qm.head_first ? e / g : e % tt, hh = qm.head_first ? e % g : e / tt;
+              const bool row = a * g < rows && hh < g;
+              const bool sees = row && (!p.causal || slot < it.q.len - it.q.n + r * tt + a + 1);
+              const float ex = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][j]), c, -z1[j]));
+              sum[j & 3] += sees ? ex : 0.f;
+            }
+          }
+        }
+        total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(s_empty + 8 * (2 * x + sb));
+          mbar_arrive(q_empty + 8 * s);
+        }
+        __syncwarp();
+      }
+      if (slot < it.q.len) {
+        int page, row;
+        page_of(p.c, slot, page, row);
+        const int64_t pg = physical_page(p.c, p.c.table, p.c.table_stride, it.seq, page);
+        if (pg >= 0) atomicAdd(&p.c.w[pg * p.c.w_sp + row * p.c.w_sn + head * p.c.w_sh], total);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// q as a 3-D tensor (d, heads and tokens by ascending stride), boxes of 64
+// columns x the g heads of a group x `tokens` tokens.
+bool query_map(const PagedAttnParams& p, ssa_dtype dt, CUtensorMap* map, QueryMap* qm) {
+  auto enc = tensor_map_encoder();
+  if (!enc || !p.q) return false;
+  const int64_t h_q = static_cast<int64_t>(p.c.h_kv) * p.group;
+  int64_t sh = p.q_sh, sn = p.q_sn;
+  if (h_q == 1) sh = p.c.d;
+  if (p.rows == 1 && sn < sh * h_q) sn = sh * h_q;
+  qm->tokens = kRows / p.group;
+  qm->head_first = sh < sn;
+  const int64_t s1 = qm->head_first ? sh : sn, s2 = qm->head_first ? sn : sh;
+  const int64_t n1 = qm->head_first ? h_q : p.rows, n2 = qm->head_first ? p.rows : h_q;
+  if (s1 < p.c.d || s2 < s1 * n1 || s2 * 2 >= (1ll << 40)) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.c.d), static_cast<cuuint64_t>(n1), static_cast<cuuint64_t>(n2)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(s1) * 2, static_cast<cuuint64_t>(s2) * 2};
+  const cuuint32_t gh = p.group, tk = qm->tokens;
+  const cuuint32_t box[3] = {64, qm->head_first ? gh : tk, qm->head_first ? tk : gh};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType t = dt == SSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, t, 3, const_cast<void*>(p.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, cudaStream_t st) {
+  CUtensorMap km, qm;
+  MapOrder mo;
+  QueryMap qo;
+  if (!page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, kSlots, &km, &mo) || !query_map(p, dt, &qm, &qo))
+    return cudaErrorInvalidValue;
+  auto kern = weights_tc_kernel<T, D>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(Geo<D>::kSmem));
+  if (e != cudaSuccess) return e;
+  kern<<<148, kThreads, Geo<D>::kSmem, st>>>(km, qm, p, mo, qo);
+  return cudaGetLastError();
+}
+
+}  // namespace pwt
+
+bool paged_weights_tc_supported(const PagedAttnParams& p, ssa_dtype dt) {
+  CUtensorMap m;
+  pwt::QueryMap q;
+  return page_tiles_supported(p, dt) && pwt::query_map(p, dt, &m, &q);
+}
+
+cudaError_t launch_paged_weights_tc(const PagedAttnParams& p, ssa_dtype dt, cudaStream_t st) {
+  if (dt == SSA_BF16)
+    return p.c.d == 128 ? pwt::launch_t<__nv_bfloat16, 128>(p, dt, st) : pwt::launch_t<__nv_bfloat16, 64>(p, dt, st);
+  return p.c.d == 128 ? pwt::launch_t<__half, 128>(p, dt, st) : pwt::launch_t<__half, 64>(p, dt, st);
+}
+
+}  // namespace ssa
