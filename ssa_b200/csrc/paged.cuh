@@ -42,7 +42,8 @@ struct PagedAppendParams {
 // What a CTA leaves about the item its first unit belongs to.
 struct PagedSplit {
   int64_t item_first;              // the item's first unit
-  int32_t seq, head, tile;
+  int64_t tok0;                    // row (of q) of the tile's first token
+  int32_t head, rows;              // KV head, rows of the tile
   int32_t cta_first, cta_last;     // the CTAs that hold its first and its last unit
   int32_t valid;                   // 0: the CTA had no unit
 };
@@ -54,7 +55,7 @@ struct PagedAttnParams {
   void* out; int64_t o_sn, o_sh;
   float* lse;                      // [rows, h_q] or NULL
   float* lse2;                     // [rows, h_q] row log2-sum-exp2 for the weights pass, or NULL
-  float* part;                     // [grid][2][tile rows][d + 2]: unnormalised row, maximum (log2), sum
+  float* part;                     // [grid][2][tile rows][d + 4]: unnormalised row, maximum (log2), sum, -
   PagedSplit* split;               // [grid]
   float* scores;                   // [rows, h_q, slots of a table row] scaled logits (base 2), or NULL
   int64_t rows;
@@ -287,9 +288,10 @@ __device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt,
 __device__ __forceinline__ int unit_cta(const PagedWalk& w, int64_t u) {
   return static_cast<int>(((u + 1) * w.ctas - 1) / w.total);
 }
-__device__ __forceinline__ PagedSplit paged_split(const PagedWalk& w) {
-  return PagedSplit{w.item_first, w.seq, w.head, w.tile, unit_cta(w, w.item_first),
-                    unit_cta(w, w.item_first + w.units - 1), 1};
+__device__ __forceinline__ PagedSplit paged_split(const PagedAttnParams& p, const PagedWalk& w, int tt) {
+  const int tok0 = w.tile * tt;
+  return PagedSplit{w.item_first, w.q0 + tok0, w.head, (w.n - tok0 < tt ? w.n - tok0 : tt) * p.group,
+                    unit_cta(w, w.item_first), unit_cta(w, w.item_first + w.units - 1), 1};
 }
 
 __host__ __device__ inline int tile_tokens(int tile_rows, int group) { return tile_rows / group; }

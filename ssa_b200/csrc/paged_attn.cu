@@ -13,6 +13,7 @@
 #include <cmath>
 
 #include "common.cuh"
+#include "mma_utils.cuh"
 #include "paged.cuh"
 #include "paged_tma.cuh"
 
@@ -45,6 +46,18 @@ __device__ __forceinline__ void store_lse(const PagedAttnParams& p, int64_t tok,
   const float z = l == 0.f ? -INFINITY : m + log2f(l);
   if (p.lse) p.lse[at] = z * kLn2;
   if (p.lse2) p.lse2[at] = z;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, const float4& v, float f) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(dst) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+  } else {
+    uint2 u;
+    u.x = pack2<T>(v.x * f, v.y * f);
+    u.y = pack2<T>(v.z * f, v.w * f);
+    *reinterpret_cast<uint2*>(dst) = u;
+  }
 }
 
 template <typename T>
@@ -148,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
     if (tid == 0) p.split[blockIdx.x].valid = 0;
     return;
   }
-  if (tid == 0) p.split[blockIdx.x] = paged_split(w);
+  if (tid == 0) p.split[blockIdx.x] = paged_split(p, w, tt);
   for (int slot = 0; w.u < w.end; slot = 1) {
     const TileRows t = tile_rows(w, tt, p.group);
     __syncthreads();
@@ -269,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
           }
         if (tx == 0) store_lse(p, tok, head, m[i], l[i]);
       } else {
-        float* dst = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * R + r) * (d + 2);
+        float* dst = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * R + r) * (d + 4);
 #pragma unroll
         for (int c = 0; c < CI; ++c)
 #pragma unroll
@@ -288,59 +301,67 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
 }
 
 // ---------------------------------------------------------------------------
-// join of the items cut by CTA boundaries.  Block (b, y) looks at the boundary
-// before CTA b: if it is the first one inside its item, the block joins its
-// share of the item's rows over the CTAs that hold parts of it, in CTA order.
+// join of the items cut by CTA boundaries.  Block b looks at the boundary
+// before CTA b + 1: if it is the first one inside its item, the block joins the
+// item's rows, a warp per row, over the CTAs that hold parts of it, in CTA
+// order, in one pass with a running maximum.  A matter of latency: everything
+// it needs to find its rows is in the two split records, and the parts of a
+// row are loaded four at a time.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(128) combine_kernel(PagedAttnParams p, int R) {
+__global__ void __launch_bounds__(1024) combine_kernel(PagedAttnParams p, int R) {
   const int b = blockIdx.x + 1;
-  const PagedSplit it = p.split[b], before = p.split[b - 1];
-  if (!it.valid) return;
+  const PagedSplit it = p.split[b];
+  const int64_t before = p.split[b - 1].item_first;
   // the item starts before this CTA, and in the CTA before it
-  if (it.cta_first != b - 1) return;
-  const int tt = tile_tokens(R, p.group), d = p.c.d;
-  const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, it.seq);
-  const int tok0 = it.tile * tt, rows = min(tt, q.n - tok0) * p.group;
-  const int slot0 = before.item_first == it.item_first ? 0 : 1;    // CTA b - 1: is it also that CTA's first item
+  if (!it.valid || it.cta_first != b - 1) return;
+  const int d = p.c.d, pd = d + 4, parts = it.cta_last - b + 2;     // CTAs b - 1 .. cta_last
+  const int slot0 = before == it.item_first ? 0 : 1;                // CTA b - 1: is it also that CTA's first item
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-  const int parts = it.cta_last - b + 2;                            // CTAs b - 1 .. cta_last
-  auto row_of = [&](int i, int r) {                                 // part i of row r
-    return p.part + (static_cast<int64_t>((b - 1 + i) * 2 + (i == 0 ? slot0 : 0)) * R + r) * (d + 2);
-  };
-  for (int r = blockIdx.y * 4 + warp; r < rows; r += gridDim.y * 4) {
-    float m = -INFINITY;
-    for (int i = lane; i < parts; i += 32) m = fmaxf(m, row_of(i, r)[d]);
+  const int64_t step = static_cast<int64_t>(2) * R * pd;
+  const int x0 = 4 * lane, x1 = x0 + 128;                           // this lane's columns
+  for (int r = warp; r < it.rows; r += blockDim.x / kWarp) {
+    const float* src = p.part + (static_cast<int64_t>(b - 1) * 2 * R + r) * pd;
+    float m = -INFINITY, l = 0.f;
+    float4 o0 = make_float4(0.f, 0.f, 0.f, 0.f), o1 = o0;
+    for (int i0 = 0; i0 < parts; i0 += 4) {
+      float2 ml[4];
+      float4 a0[4], a1[4];
 #pragma unroll
-    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    float2 o[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) o[x] = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float* src = row_of(i, r);
-      const float f = exp2f(src[d] - base);
-      l = fmaf(f, src[d + 1], l);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (2 * lane + 64 * x < d) {
-          const float2 a = *reinterpret_cast<const float2*>(src + 2 * lane + 64 * x);
-          o[x].x = fmaf(f, a.x, o[x].x);
-          o[x].y = fmaf(f, a.y, o[x].y);
+      for (int i = 0; i < 4; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        a0[i] = a1[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + i < parts) {
+          const float* s = src + (i0 + i) * step + (i0 + i == 0 && slot0 ? static_cast<int64_t>(R) * pd : 0);
+          ml[i] = *reinterpret_cast<const float2*>(s + d);
+          if (x0 < d) a0[i] = *reinterpret_cast<const float4*>(s + x0);
+          if (x1 < d) a1[i] = *reinterpret_cast<const float4*>(s + x1);
         }
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mn = fmaxf(mn, ml[i].x);
+      const float base = mn == -INFINITY ? 0.f : mn, f = exp2f(m - base);
+      m = mn;
+      l *= f;
+      o0.x *= f; o0.y *= f; o0.z *= f; o0.w *= f;
+      o1.x *= f; o1.y *= f; o1.z *= f; o1.w *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float g = exp2f(ml[i].x - base);
+        l = fmaf(g, ml[i].y, l);
+        o0.x = fmaf(g, a0[i].x, o0.x); o0.y = fmaf(g, a0[i].y, o0.y);
+        o0.z = fmaf(g, a0[i].z, o0.z); o0.w = fmaf(g, a0[i].w, o0.w);
+        o1.x = fmaf(g, a1[i].x, o1.x); o1.y = fmaf(g, a1[i].y, o1.y);
+        o1.z = fmaf(g, a1[i].z, o1.z); o1.w = fmaf(g, a1[i].w, o1.w);
+      }
     }
-    const int64_t tok = q.q0 + tok0 + r / p.group;
+    const int64_t tok = it.tok0 + r / p.group;
     const int head = it.head * p.group + r % p.group;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     T* dst = static_cast<T*>(p.out) + tok * p.o_sn + head * p.o_sh;
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (2 * lane + 64 * x < d) {
-        dst[2 * lane + 64 * x] = Elem<T>::from_f(o[x].x * inv);
-        dst[2 * lane + 64 * x + 1] = Elem<T>::from_f(o[x].y * inv);
-      }
+    if (x0 < d) store4(dst + x0, o0, inv);
+    if (x1 < d) store4(dst + x1, o1, inv);
     if (lane == 0) store_lse(p, tok, head, m, l);
   }
 }
@@ -458,7 +479,7 @@ AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   a.grid = a.kernel == AttnKernel::kSimt ? 2 * 148 : 148;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t lines = static_cast<size_t>(p.rows) * p.c.h_kv * p.group;
-  a.split = up(static_cast<size_t>(a.grid) * 2 * a.rows * (p.c.d + 2) * 4);
+  a.split = up(static_cast<size_t>(a.grid) * 2 * a.rows * (p.c.d + 4) * 4);
   a.lse2 = a.split + up(a.grid * sizeof(PagedSplit));
   a.scores = a.lse2 + (p.c.w ? up(lines * 4) : 0);
   a.total = a.scores;
@@ -485,11 +506,11 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
       e = a.rows == 64 ? launch_simt_t<64>(p, dt, a.grid, false, st) : launch_simt_t<16>(p, dt, a.grid, false, st);
   }
   if (e != cudaSuccess) return e;
-  const dim3 grid(a.grid - 1, a.rows == 16 ? 4 : a.rows / 16);
+  const int threads = a.rows == 16 ? 512 : 1024;
   switch (dt) {
-    case SSA_F32: combine_kernel<float><<<grid, 128, 0, st>>>(p, a.rows); break;
-    case SSA_BF16: combine_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p, a.rows); break;
-    default: combine_kernel<__half><<<grid, 128, 0, st>>>(p, a.rows); break;
+    case SSA_F32: combine_kernel<float><<<a.grid - 1, threads, 0, st>>>(p, a.rows); break;
+    case SSA_BF16: combine_kernel<__nv_bfloat16><<<a.grid - 1, threads, 0, st>>>(p, a.rows); break;
+    default: combine_kernel<__half><<<a.grid - 1, threads, 0, st>>>(p, a.rows); break;
   }
   e = cudaGetLastError();
   if (e != cudaSuccess || !p.c.w) return e;

@@ -74,12 +74,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
   }
   PagedWalk w;
   const bool any = paged_schedule(p, tt, kKT, 1, blockIdx.x, gridDim.x, w);
-  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(w) : PagedSplit{};
+  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt) : PagedSplit{};
   __syncthreads();
   if (!any) return;
   auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (*abort_flag) return;
-    if (!mbar_wait(bar, parity)) {
+    if (!mbar_wait_or(bar, parity, abort_flag) && !*abort_flag) {
       *abort_flag = 1;
       paged_error(p.c, SSA_DEVICE_TIMEOUT);
     }
@@ -87,13 +86,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
 
   if (warp == kWarps) {
     // ---------------- TMA producer ----------------
-    const int pieces = kKT / min(p.c.page_size, kKT), boxes = pieces * (D / 64);
+    // lane i copies 64 columns of one page piece of K or of V; the page of the
+    // next tile is looked up before this tile's ring entry is waited for
+    const int piece_rows = min(p.c.page_size, kKT), pieces = kKT / piece_rows, boxes = pieces * (D / 64);
+    const int kv = lane / boxes, box = lane - kv * boxes, piece = box & (pieces - 1), half = box / pieces;
+    const uint32_t box_at = ring + kv * G::kTileBytes + half * (kKT * 128) + piece * piece_rows * 128;
     int64_t g = 0;
     while (w.u < w.end) {
       const int last_tok = min(w.tile * tt + tt, w.n) - 1;
       const int lim = p.causal ? max(w.len - w.n + last_tok + 1, 0) : w.len;
       const int64_t end = min(w.end, w.item_first + w.units);
+      int j = static_cast<int>(w.u - w.item_first) * kKT + piece * piece_rows;
+      PageSpot next = page_spot(p.c, w.seq, j, kv < 2 ? lim : 0);
       for (; w.u < end; ++w.u, ++g) {
+        const PageSpot at = next;
+        j += kKT;
+        if (w.u + 1 < end) next = page_spot(p.c, w.seq, j, kv < 2 ? lim : 0);
         const int s = static_cast<int>(g % G::kStages);
         wait(empty + 8 * s, static_cast<uint32_t>((g / G::kStages) & 1) ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) {
@@ -102,11 +110,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
         }
         if (lane == 0) mbar_expect_tx(full + 8 * s, 2 * G::kTileBytes);
         __syncwarp();
-        if (lane < 2 * boxes) {
-          const int kv = lane / boxes, b = lane - kv * boxes;
-          load_box<kKT>(p, mo, kv ? &vmap : &kmap, w.seq, w.head, static_cast<int>(w.u - w.item_first) * kKT, lim,
-                        b & (pieces - 1), b / pieces, ring + (2 * s + kv) * G::kTileBytes, full + 8 * s);
-        }
+        if (kv < 2)
+          tma_load_4d(box_at + 2 * s * G::kTileBytes, kv ? &vmap : &kmap, half * 64, mo.head_first ? w.head : at.row,
+                      mo.head_first ? at.row : w.head, at.page, full + 8 * s);
       }
       if (w.u < w.end) paged_next_item(p, tt, kKT, w);
     }
@@ -303,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
       const int tok = tok0 + r / p.group, head = w.head * p.group + r % p.group;
       const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
       T* out = static_cast<T*>(p.out) + (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh + x0;
-      float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + r) * (D + 2);
+      float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + r) * (D + 4);
 #pragma unroll
       for (int x = 0; x < D / 8; x += 8) {
         float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -325,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
           *reinterpret_cast<uint4*>(out + x) = pk;
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2*>(part + x0 + x + e) = make_float2(a[e], a[e + 1]);
+          for (int e = 0; e < 8; e += 4)
+            *reinterpret_cast<float4*>(part + x0 + x + e) = make_float4(a[e], a[e + 1], a[e + 2], a[e + 3]);
         }
       }
       if ((threadIdx.x & 7) == 0) {

@@ -14,10 +14,6 @@
 //   warps 4-7   stream B
 //   warp 8      TMEM allocation, single-thread MMA issue
 //   warp 9      TMA producer: a lane per page box, K and V tiles in a ring
-//   warps 10-11 nothing: they complete the warpgroup that gives registers up
-//
-// Registers: 384 threads x 168 at launch = 64512; warps 8-11 keep 88 each
-// (128 x 88 = 11264), the streams take 208 (256 x 208 = 53248): 64512 again.
 //
 // TMEM (512 columns): S_A, S_B (128 each; P in the first 64), O_A, O_B (d each).
 //
@@ -53,7 +49,7 @@ using namespace tc;
 
 constexpr int kRows = 256;         // rows of an item
 constexpr int kKT = 128;           // slots per key tile
-constexpr int kThreads = 384;
+constexpr int kThreads = 320;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;      // how far (log2) a tile may exceed the running maximum
@@ -82,23 +78,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
-// Boxes of one K or V tile: lane i < boxes copies 64 columns of one page piece.
-template <int D>
-__device__ __forceinline__ void load_kv(const PagedAttnParams& p, const MapOrder& mo, const void* map, int seq, int head,
-                                        int k0, int lim, uint32_t dst, uint32_t bar) {
-  const int lane = threadIdx.x & 31;
-  const int pieces = kKT / min(p.c.page_size, kKT), boxes = pieces * (D / 64);
-  if (lane == 0) mbar_expect_tx(bar, Geo<D>::kTileBytes);
-  __syncwarp();
-  if (lane < boxes)
-    load_box<kKT>(p, mo, map, seq, head, k0, lim, lane & (pieces - 1), lane / pieces, dst, bar);
-}
-
 // The tile's O += P V for this thread's row over its first `see` slots, on the
 // CUDA cores (P in TMEM columns of S, V swizzled in shared memory).  `fresh`: O
 // holds nothing yet.  The whole stream calls it.
@@ -164,9 +143,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   unsigned char* ring = base + 2 * G::kTileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + G::kStages * G::kTileBytes);
   const uint32_t full = smem_u32(bars), empty = full + 8 * G::kStages;
-  const uint32_t q_full = empty + 8 * G::kStages, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 16;
+  const uint32_t q_full = empty + 8 * G::kStages, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 32;
   const uint32_t v_seen = o_full + 16, drain = v_seen + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * G::kStages + 11);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * G::kStages + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* odd_tile = abort_flag + 1;               // [2] the last tile whose product the stream made itself
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
@@ -178,11 +157,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       mbar_init(empty + 8 * s, 1);
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(q_full + 8 * x, 128);
+      mbar_init(q_full + 8 * x, 4);
       mbar_init(s_full + 8 * x, 1);
-      mbar_init(p_full + 8 * x, 128);
+      mbar_init(p_full + 16 * x, 4);                     // P of slots 0-63, and of 64-127
+      mbar_init(p_full + 16 * x + 8, 4);
       mbar_init(o_full + 8 * x, 1);
-      mbar_init(v_seen + 8 * x, 128);
+      mbar_init(v_seen + 8 * x, 4);
       odd_tile[x] = 0;
     }
     mbar_init(drain, 1);
@@ -201,144 +181,194 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(w) : PagedSplit{};
+  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt) : PagedSplit{};
   auto fail = [&]() {
     *abort_flag = 1;
     paged_error(p.c, SSA_DEVICE_TIMEOUT);
   };
 
-  // a tile is named by its place in the ring, counted from 1
-  auto tile_name = [](int64_t g) { return static_cast<int>(g & 0x3fffffff) + 1; };
+  // a tile is named by its number in the CTA's walk, from 1
+  // (and begins again after a multiple of the ring's period: its entry and
+  // phase follow from it)
+  constexpr int kNames = G::kStages << 20;
+  auto name_next = [](int n) { return n == kNames ? 1 : n + 1; };
 
-  if (warp >= 8) {
-  regs_down<88>();
   if (any && warp == 9) {
     // ---------------- TMA producer ----------------
+    // lane i < boxes copies 64 columns of one page piece; the page of the next
+    // tile is looked up before this tile's ring entries are waited for
+    const int piece_rows = min(p.c.page_size, kKT), pieces = kKT / piece_rows, boxes = pieces * (D / 64);
+    const int piece = lane & (pieces - 1), half = lane / pieces;
+    const uint32_t box_at = half * (kKT * 128) + piece * piece_rows * 128;
     int64_t g = 0;
+    int st = 0;
+    uint32_t par = 1;
     bool stop = false;
     while (w.u < w.end && !stop) {
-      const int tok0 = w.tile * tt, rows = min(tt, w.n - tok0) * p.group;
-      const int last_tok = tok0 + rows / p.group - 1;
+      const int last_tok = min(w.tile * tt + tt, w.n) - 1;
       const int lim = p.causal ? max(w.len - w.n + last_tok + 1, 0) : w.len;
       const int64_t end = min(w.end, w.item_first + w.units);
+      int j = static_cast<int>(w.u - w.item_first) * kKT + piece * piece_rows;
+      PageSpot next = page_spot(p.c, w.seq, j, lane < boxes ? lim : 0);
       for (; w.u < end && !stop; ++w.u) {
-        const int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+        const PageSpot at = next;
+        j += kKT;
+        if (w.u + 1 < end) next = page_spot(p.c, w.seq, j, lane < boxes ? lim : 0);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++g) {
-          const int s = static_cast<int>(g % G::kStages);
-          if (*abort_flag || !mbar_wait(empty + 8 * s, static_cast<uint32_t>((g / G::kStages) & 1) ^ 1u)) stop = true;
-          stop = __any_sync(0xffffffffu, stop);
-          if (stop) {
+          if (!__all_sync(0xffffffffu, mbar_wait_or(empty + 8 * st, par, abort_flag))) {
+            stop = true;
             fail();
             break;
           }
-          load_kv<D>(p, mo, kv ? &vmap : &kmap, w.seq, w.head, k0, lim, smem_u32(ring + s * G::kTileBytes),
-                     full + 8 * s);
+          if (lane == 0) mbar_expect_tx(full + 8 * st, G::kTileBytes);
+          __syncwarp();
+          if (lane < boxes)
+            tma_load_4d(smem_u32(ring) + st * G::kTileBytes + box_at, kv ? &vmap : &kmap, half * 64,
+                        mo.head_first ? w.head : at.row, mo.head_first ? at.row : w.head, at.page, full + 8 * st);
+          if (++st == G::kStages) {
+            st = 0;
+            par ^= 1u;
+          }
         }
       }
-      if (w.u < w.end) paged_next_item(p, tt, kKT, w);
+      if (!stop && w.u < w.end) paged_next_item(p, tt, kKT, w);
     }
     // every issued copy lands before the CTA exits
     if (lane == 0)
       for (int64_t r = g - 1; r >= 0 && r >= g - G::kStages; --r)
         mbar_wait(full + 8 * static_cast<int>(r % G::kStages), static_cast<uint32_t>((r / G::kStages) & 1));
   } else if (any && warp == 8) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      int64_t g = 0;                                     // K tile of the current unit: ring entry g, V: g + 1
-      uint32_t p_ph[2] = {0, 0}, q_ph[2] = {0, 0};
-      bool stop = false, issued = false;
-      auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (stop || *abort_flag || !mbar_wait(bar, parity)) {
-          if (!stop) fail();
-          stop = true;
-        }
-        fence_after();
-        return !stop;
-      };
-      auto ring_at = [&](int64_t i) { return smem_u32(ring + static_cast<int>(i % G::kStages) * G::kTileBytes); };
-      auto wait_full = [&](int64_t i) {
-        return wait(full + 8 * static_cast<int>(i % G::kStages), static_cast<uint32_t>((i / G::kStages) & 1));
-      };
-      auto scores = [&](int x, int64_t i) {              // S_x = Q_x K^T, K in ring entry i
-        const uint32_t kb = ring_at(i), qb = smem_u32(q_tile) + x * G::kTileBytes;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks / 4) * (kKT * 128) + (ks % 4) * 32;
-          mma_f16(tmem + x * 128, sdesc(qb + off, 0, 1024, 2), sdesc(kb + off, 0, 1024, 2), kIdS, ks > 0);
-        }
-        mma_commit(s_full + 8 * x);
-        issued = true;
-      };
-      while (w.u < w.end && !stop) {
-        const int rows = min(tt, w.n - w.tile * tt) * p.group, streams = rows > 128 ? 2 : 1;
-        const int64_t end = min(w.end, w.item_first + w.units);
-        bool fresh[2] = {true, true};
-        if (!wait_full(g)) break;
-        for (int x = 0; x < streams; ++x) {
-          if (!wait(q_full + 8 * x, q_ph[x])) break;
-          q_ph[x] ^= 1u;
-          scores(x, g);
-        }
-        if (stop) break;
-        mma_commit(empty + 8 * static_cast<int>(g % G::kStages));
-        for (; w.u < end && !stop; ++w.u, g += 2) {
-          const bool more = w.u + 1 < end;
-          for (int x = 0; x < streams; ++x) {
-            if (!wait_full(g + 1) || !wait(p_full + 8 * x, p_ph[x])) break;
-            p_ph[x] ^= 1u;
-            if (odd_tile[x] != tile_name(g)) {
-              const uint32_t vb = ring_at(g + 1);
-#pragma unroll
-              for (int ks = 0; ks < kKT / 16; ++ks)      // 16 slots a step; N chunks of 64 columns 16 KB apart
-                mma_f16_ta(tmem + 256 + x * D, tmem + x * 128 + ks * 8, sdesc(vb + ks * 2048, kKT * 128, 1024, 2), kIdO,
-                           (!fresh[x] || ks > 0) ? 1u : 0u);
-            }
-            fresh[x] = false;
-            if (x == streams - 1) mma_commit(empty + 8 * static_cast<int>((g + 1) % G::kStages));
-            if (more) {
-              if (!wait_full(g + 2)) break;
-              scores(x, g + 2);
-              if (x == streams - 1) mma_commit(empty + 8 * static_cast<int>((g + 2) % G::kStages));
-            } else {
-              mma_commit(o_full + 8 * x);
-            }
-          }
-        }
-        if (!stop && w.u < w.end) paged_next_item(p, tt, kKT, w);
-      }
-      // after a failed wait: the commit arrives once every MMA issued before it is done
-      if (issued && stop) {
-        mma_commit(drain);
-        mbar_wait(drain, 0);
-      }
-    }
-  }
-  } else {
-    regs_up<208>();
-    // ---------------- softmax and epilogue of stream x ----------------
-    const int x = warp >> 2, r = (warp & 3) * 32 + lane;  // row of the stream, its TMEM lane
-    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lane_base + x * 128, o_addr = tmem + lane_base + 256 + x * D;
-    const float c = p.inv_scale * kLog2e;
-    uint32_t s_ph = 0, o_ph = 0, v_ph = 0;
-    int64_t g = 0;                                        // ring entry of the current unit's K
+    // ---------------- MMA issuer: the warp decides, one lane issues ----------------
+    constexpr uint32_t kTileDesc = G::kTileBytes >> 4, kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    const uint32_t q_lo = smem_u32(q_tile) >> 4, ring_lo = smem_u32(ring) >> 4;
+    // descriptors: SWIZZLE_128B, groups of 8 rows 1024 bytes apart; V (MN-major): 64-column chunks 16 KB apart
+    auto desc = [](uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | (lo & 0x3fffu); };
+    auto desc_v = [](uint32_t lo) {
+      return (static_cast<uint64_t>(kDescHi) << 32) | ((kKT * 128u >> 4) << 16) | (lo & 0x3fffu);
+    };
+    uint32_t p_ph = 0, q_ph = 0;                         // bit x: stream x
+    int ks = 0, name = 1;                     // ring entry of the current unit's K
+    uint32_t kpar = 0;
     bool stop = false;
-    // the same answer in every lane: what follows is done by whole warps
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      const bool ok = !*abort_flag && mbar_wait(bar, parity);
-      if (!__all_sync(0xffffffffu, ok)) {
+      if (!stop && !__all_sync(0xffffffffu, mbar_wait_or(bar, parity, abort_flag))) {
         fail();
         stop = true;
       }
       fence_after();
       return !stop;
     };
-    for (int slot = 0; any && w.u < w.end && !stop; slot = 1) {
+    auto scores = [&](int x, int st) {                   // S_x = Q_x K^T, K in ring entry st
+      if (elect_one()) {
+        const uint32_t kb = ring_lo + st * kTileDesc, qb = q_lo + x * kTileDesc;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k / 4) * (kKT * 128) + (k % 4) * 32) >> 4;
+          mma_f16(tmem + x * 128, desc(qb + off), desc(kb + off), kIdS, k > 0);
+        }
+        mma_commit(s_full + 8 * x);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int st) {
+      if (elect_one()) mma_commit(empty + 8 * st);
+      __syncwarp();
+    };
+    while (w.u < w.end && !stop) {
+      const int rows = min(tt, w.n - w.tile * tt) * p.group;
+      const int streams = __shfl_sync(0xffffffffu, rows > 128 ? 2 : 1, 0);
+      const int64_t end = min(w.end, w.item_first + w.units);
+      const int units = __shfl_sync(0xffffffffu, static_cast<int>(end - w.u), 0);
+      uint32_t fresh = 3;
+      wait(full + 8 * ks, kpar);
+      for (int x = 0; x < streams && !stop; ++x) {
+        if (!wait(q_full + 8 * x, (q_ph >> x) & 1u)) break;
+        q_ph ^= 1u << x;
+        scores(x, ks);
+      }
+      if (stop) break;
+      release(ks);
+      for (int i = 0; i < units && !stop; ++i) {
+        int vs = ks + 1;
+        uint32_t vpar = kpar;
+        if (vs == G::kStages) { vs = 0; vpar ^= 1u; }
+        int ns = vs + 1;                                 // the next unit's K
+        uint32_t npar = vpar;
+        if (ns == G::kStages) { ns = 0; npar ^= 1u; }
+        const bool more = i + 1 < units;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (x >= streams) break;
+          if (x == 0) wait(full + 8 * vs, vpar);
+          const uint32_t pp = (p_ph >> x) & 1u;
+          if (!wait(p_full + 16 * x, pp)) break;
+          p_ph ^= 1u << x;
+          const bool made = __shfl_sync(0xffffffffu, odd_tile[x] == name, 0);
+          const uint32_t vb = ring_lo + vs * kTileDesc, acc = ((fresh >> x) & 1u) ^ 1u;
+          auto product = [&](int k0) {                   // four steps of 16 slots
+#pragma unroll
+            for (int k = k0; k < k0 + 4; ++k)
+              mma_f16_ta(tmem + 256 + x * D, tmem + x * 128 + k * 8, desc_v(vb + (k * 2048 >> 4)), kIdO, k > 0 ? 1u : acc);
+          };
+          if (!made && elect_one()) product(0);
+          __syncwarp();
+          if (!wait(p_full + 16 * x + 8, pp)) break;
+          if (elect_one()) {
+            if (!made) product(4);
+            if (x == streams - 1) mma_commit(empty + 8 * vs);
+            if (!more) mma_commit(o_full + 8 * x);
+          }
+          __syncwarp();
+          fresh &= ~(1u << x);
+          if (more) {
+            if (x == 0 && !wait(full + 8 * ns, npar)) break;
+            scores(x, ns);
+            if (x == streams - 1) release(ns);
+          }
+        }
+        ks = ns;
+        kpar = npar;
+        name = name_next(name);
+      }
+      w.u = end;
+      if (!stop && w.u < w.end) paged_next_item(p, tt, kKT, w);
+    }
+    // after a failed wait: the commit arrives once every MMA issued before it is done
+    if (stop) {
+      if (elect_one()) mma_commit(drain);
+      __syncwarp();
+      mbar_wait(drain, 0);
+    }
+  } else if (any && warp < 8) {
+    // ---------------- softmax and epilogue of stream x ----------------
+    const int x = warp >> 2, r = (warp & 3) * 32 + lane;  // row of the stream, its TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lane_base + x * 128, o_addr = tmem + lane_base + 256 + x * D;
+    const float c = p.inv_scale * kLog2e;
+    uint32_t s_ph = 0, o_ph = 0, v_ph = 0;
+    int name = 1;
+    bool stop = false;
+    // the same answer in every lane: what follows is done by whole warps
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (!__all_sync(0xffffffffu, mbar_wait_or(bar, parity, abort_flag))) {
+        fail();
+        stop = true;
+      }
+      fence_after();
+      return !stop;
+    };
+    auto arrive = [&](uint32_t bar) {                     // once a warp
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    for (int slot = 0; w.u < w.end && !stop; slot = 1) {
       const int tok0 = w.tile * tt, rows = min(tt, w.n - tok0) * p.group;
-      const int64_t from = w.u, end = min(w.end, w.item_first + w.units);
+      const int64_t end = min(w.end, w.item_first + w.units);
+      const int units = static_cast<int>(end - w.u);
+      const bool whole = w.u == w.item_first && end == w.item_first + w.units;
       if (x == 1 && rows <= 128) {                        // nothing for this stream here
-        g += 2 * (end - from);
+        for (int i = 0; i < units; ++i) name = name_next(name);
         w.u = end;
         if (w.u < w.end) paged_next_item(p, tt, kKT, w);
         continue;
@@ -360,39 +390,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         fence_proxy_async();
         fence_before();
-        mbar_arrive(q_full + 8 * x);
+        arrive(q_full + 8 * x);
       }
       float m = -INFINITY, l = 0.f;
-      for (; w.u < end; ++w.u, g += 2) {
-        const int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+      int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+      for (int i = 0; i < units; ++i, k0 += kKT, name = name_next(name)) {
         if (!wait(s_full + 8 * x, s_ph)) break;
         s_ph ^= 1u;
-        float s[kKT];
-        {
-          uint32_t v[4][32];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32_async(s_addr + 32 * i, v[i]);
-          tmem_wait();
-#pragma unroll
-          for (int j = 0; j < kKT; ++j) s[j] = __uint_as_float(v[j / 32][j % 32]);
-        }
         const bool masked = k0 + kKT > lim0;              // the same for the whole stream
-        if (masked) {
-          const int see = lim - k0;
+        const int see = masked ? lim - k0 : kKT;
+        uint32_t v[2][32];
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld32_async(s_addr, v[0]);
 #pragma unroll
-          for (int j = 0; j < kKT; ++j) s[j] = j < see ? s[j] : -INFINITY;
+        for (int q = 0; q < 4; ++q) {
+          tmem_wait();
+          tmem_ld32_async(s_addr + 32 * ((q + 1) & 3), v[(q + 1) & 1]);
+          uint32_t (&u)[32] = v[q & 1];
+          if (masked) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] = 32 * q + j < see ? u[j] : __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(u[j + e]), __uint_as_float(u[j + 4 + e]));
         }
-        float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int j = 4; j < kKT; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c;
         const bool raise = top > m + kSlack;
         if (__any_sync(0xffffffffu, raise)) {
           const float mn = raise ? top : m;
           const float f = m == -INFINITY ? 0.f : ex2_approx(m - mn);       // 1 where the row keeps its maximum
           m = mn;
           l *= f;
-          if (w.u > from) {                               // the PV of the tile before is done: S of this one came after it
+          if (i > 0) {                               // the PV of the tile before is done: S of this one came after it
 #pragma unroll
             for (int c0 = 0; c0 < D; c0 += 16) {
               uint32_t o[16];
@@ -406,49 +437,72 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           }
         }
         const float off = (m == -INFINITY ? 0.f : m) - kShift;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t c2 = pair(c, c), off2 = pair(-off, -off);
+        uint64_t sum[2] = {0, 0};
+        auto exps = [&](auto masked_tile) {
+          constexpr bool kMasked = decltype(masked_tile)::value;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t pk[16];
+          for (int q = 0; q < 4; ++q) {
+            tmem_wait();
+            if (q < 3) tmem_ld32_async(s_addr + 32 * (q + 1), v[(q + 1) & 1]);
+            uint32_t (&u)[32] = v[q & 1];
+            if (kMasked) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float a = ex2_approx(fmaf(s[32 * i + 2 * j], c, -off));
-            const float b = ex2_approx(fmaf(s[32 * i + 2 * j + 1], c, -off));
-            sum[j & 3] += a + b;
-            pk[j] = pack2<T>(a, b);
+              for (int j = 0; j < 32; ++j) u[j] = 32 * q + j < see ? u[j] : __float_as_uint(-INFINITY);
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float a, b;
+              unpair(fma_pair(pair(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1])), c2, off2), a, b);
+              a = ex2_approx(a);
+              b = ex2_approx(b);
+              sum[j & 1] = add_pair(sum[j & 1], pair(a, b));
+              pk[j] = pack2<T>(a, b);
+            }
+            tmem_st16(s_addr + 16 * q, pk);
+            if (!kMasked && q == 1) {                     // the tensor cores may begin
+              tmem_wait_st();
+              fence_before();
+              arrive(p_full + 16 * x);
+            }
           }
-          tmem_st16(s_addr + 16 * i, pk);
+        };
+        if (masked) exps(std::true_type{});
+        else exps(std::false_type{});
+        {
+          float a, b;
+          unpair(add_pair(sum[0], sum[1]), a, b);
+          l += a + b;
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_wait_st();
         if (masked) {
           // a non-finite value in V, perhaps hidden from this row or another?
-          const int64_t e = g + 1;
-          const int st = static_cast<int>(e % G::kStages);
-          if (!wait(full + 8 * st, static_cast<uint32_t>((e / G::kStages) & 1))) break;
+          const int e = 2 * (name - 1) + 1, st = e % G::kStages;
+          if (!wait(full + 8 * st, static_cast<uint32_t>(e / G::kStages) & 1u)) break;
           const unsigned char* v = ring + st * G::kTileBytes;
           uint32_t odd = 0;
-          for (int i = r; i < G::kTileBytes / 16; i += 128) {
-            const uint4 a = *reinterpret_cast<const uint4*>(v + i * 16);
+          for (int y = r; y < G::kTileBytes / 16; y += 128) {
+            const uint4 a = *reinterpret_cast<const uint4*>(v + y * 16);
             odd |= odd_bits<T>(a.x) | odd_bits<T>(a.y) | odd_bits<T>(a.z) | odd_bits<T>(a.w);
           }
-          if (odd) odd_tile[x] = tile_name(g);
-          mbar_arrive(v_seen + 8 * x);
+          if (odd) odd_tile[x] = name;
+          arrive(v_seen + 8 * x);
           if (!wait(v_seen + 8 * x, v_ph)) break;
           v_ph ^= 1u;
-          if (odd_tile[x] == tile_name(g)) visible_product<T, D>(s_addr, o_addr, v, lim - k0, w.u == from);
+          if (odd_tile[x] == name) visible_product<T, D>(s_addr, o_addr, v, lim - k0, i == 0);
         }
         fence_before();
-        mbar_arrive(p_full + 8 * x);
+        if (masked) arrive(p_full + 16 * x);
+        arrive(p_full + 16 * x + 8);
       }
       if (stop) break;
       // ---- epilogue ----
       if (!wait(o_full + 8 * x, o_ph)) break;
       o_ph ^= 1u;
-      const bool whole = from == w.item_first && end == w.item_first + w.units;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       T* out = static_cast<T*>(p.out) + (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh;
-      float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + row) * (D + 2);
+      float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + row) * (D + 4);
 #pragma unroll
       for (int c0 = 0; c0 < D; c0 += 32) {
         uint32_t o[32];
@@ -467,8 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            *reinterpret_cast<float2*>(part + c0 + i) = make_float2(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(part + c0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
         }
       }
       if (live) {
@@ -482,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           part[D + 1] = l;
         }
       }
+      w.u = end;
       if (w.u < w.end) paged_next_item(p, tt, kKT, w);
     }
   }

@@ -26,23 +26,20 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x
       : "memory");
 }
 
-// The box of one 64-column half of one page piece of a tile of KT slots
-// (shared layout [D / 64][KT][128 bytes], SWIZZLE_128B).  Slots from `lim` on
-// that lie in no page of the sequence, and bad pages, read as zeros (a page
-// coordinate out of range).
-template <int KT>
-__device__ __forceinline__ void load_box(const PagedAttnParams& p, const MapOrder& mo, const void* map, int seq,
-                                         int head, int k0, int lim, int piece, int half, uint32_t dst, uint32_t bar) {
-  const int rows = min(p.c.page_size, KT);
-  const int j = k0 + piece * rows;
-  int pg = -1, row = 0;
+// Where slot j of a sequence lies, for a box that starts there.  Slots from
+// `lim` on, and bad pages, get a page coordinate out of range: the copy reads
+// zeros.
+struct PageSpot {
+  int page, row;
+};
+__device__ __forceinline__ PageSpot page_spot(const PagedCacheParams& c, int seq, int j, int lim) {
+  PageSpot s{-1, 0};
   if (j < lim) {
     int lp;
-    page_of(p.c, j, lp, row);
-    pg = static_cast<int>(physical_page(p.c, p.c.table, p.c.table_stride, seq, lp));
+    page_of(c, j, lp, s.row);
+    s.page = static_cast<int>(physical_page(c, c.table, c.table_stride, seq, lp));
   }
-  tma_load_4d(dst + half * (KT * 128) + piece * rows * 128, map, half * 64, mo.head_first ? head : row,
-              mo.head_first ? row : head, pg, bar);
+  return s;
 }
 
 // Non-finite 16-bit values: all exponent bits set.  (x & kExp) + kOne carries

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   fence_after();
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (!*abort_flag && !mbar_wait(bar, parity)) {
+    if (!mbar_wait_or(bar, parity, abort_flag) && !*abort_flag) {
       *abort_flag = 1;
       paged_error(p.c, SSA_DEVICE_TIMEOUT);
     }
@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
 
   if (warp == 9) {
     // ---------------- producer ----------------
-    const int pieces = kSlots / min(p.c.page_size, kSlots), boxes = pieces * (D / 64);
+    const int piece_rows = min(p.c.page_size, kSlots), pieces = kSlots / piece_rows, boxes = pieces * (D / 64);
+    const int piece = lane & (pieces - 1), half = lane / pieces;
     const int64_t h_q = static_cast<int64_t>(p.c.h_kv) * g;
     const uint32_t q_bytes = static_cast<uint32_t>(tt * g) * 128 * (D / 64);
     bool stop = false;
@@ -152,9 +153,12 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       __syncwarp();
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        if (lane < boxes)
-          load_box<kSlots>(p, mo, &kmap, it.seq, head, k0 + x * kSlots, it.q.len, lane & (pieces - 1), lane / pieces,
-                           smem_u32(base) + (2 * b + x) * G::kTileBytes, k_full + 8 * b);
+        if (lane < boxes) {
+          const PageSpot at = page_spot(p.c, it.seq, k0 + x * kSlots + piece * piece_rows, it.q.len);
+          tma_load_4d(smem_u32(base) + (2 * b + x) * G::kTileBytes + half * (kSlots * 128) + piece * piece_rows * 128,
+                      &kmap, half * 64, mo.head_first ? head : at.row, mo.head_first ? at.row : head, at.page,
+                      k_full + 8 * b);
+        }
       for (int r = first_token(p, it.q, k0) / tt; r * tt < it.q.n; ++r, ++t) {
         const int s = static_cast<int>(t % kQStages);
         wait(q_empty + 8 * s, static_cast<uint32_t>((t / kQStages) & 1) ^ 1u);
@@ -185,38 +189,49 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     for (int64_t r = t - 1; lane == 0 && r >= 0 && r >= t - kQStages; --r)
       mbar_wait(q_full + 8 * static_cast<int>(r % kQStages), static_cast<uint32_t>((r / kQStages) & 1));
   } else if (warp == 8) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      for (int64_t i = blockIdx.x; !*abort_flag && seek(p, it, i); i += gridDim.x, ++n) {
-        const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots;
-        const int b = static_cast<int>(n & 1);
-        wait(k_full + 8 * b, static_cast<uint32_t>((n >> 1) & 1));
-        for (int r = first_token(p, it.q, k0) / tt; r * tt < it.q.n && !*abort_flag; ++r, ++t) {
-          const int s = static_cast<int>(t % kQStages), sb = static_cast<int>(t & 1);
-          wait(q_full + 8 * s, static_cast<uint32_t>((t / kQStages) & 1));
-          const uint32_t qb = smem_u32(q_ring + s * G::kTileBytes);
+    // ---------------- MMA issuer: the warp decides, one lane issues ----------------
+    constexpr uint32_t kTileDesc = G::kTileBytes >> 4, kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    const uint32_t k_lo = smem_u32(base) >> 4, q_lo = smem_u32(q_ring) >> 4;
+    auto desc = [](uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | (lo & 0x3fffu); };
+    int s = 0;
+    uint32_t qpar = 0;
+    for (int64_t i = blockIdx.x; !__any_sync(0xffffffffu, *abort_flag) && seek(p, it, i); i += gridDim.x, ++n) {
+      const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots;
+      const int b = static_cast<int>(n & 1), r0 = first_token(p, it.q, k0) / tt;
+      const int tiles = __shfl_sync(0xffffffffu, max((it.q.n + tt - 1) / tt - r0, 0), 0);
+      wait(k_full + 8 * b, static_cast<uint32_t>((n >> 1) & 1));
+      for (int j = 0; j < tiles; ++j, ++t) {
+        const int sb = static_cast<int>(t & 1);
+        wait(q_full + 8 * s, qpar);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            wait(s_empty + 8 * (2 * x + sb), static_cast<uint32_t>((t >> 1) & 1) ^ 1u);
-            if (*abort_flag) break;
-            fence_after();
-            const uint32_t kb = smem_u32(base) + (2 * b + x) * G::kTileBytes;
+        for (int x = 0; x < 2; ++x) {
+          wait(s_empty + 8 * (2 * x + sb), static_cast<uint32_t>((t >> 1) & 1) ^ 1u);
+          __syncwarp();
+          fence_after();
+          if (elect_one()) {
+            const uint32_t kb = k_lo + (2 * b + x) * kTileDesc, qb = q_lo + s * kTileDesc;
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-              const uint32_t off = (ks / 4) * (128 * 128) + (ks % 4) * 32;
-              mma_f16(tmem + (2 * x + sb) * 128, sdesc(kb + off, 0, 1024, 2), sdesc(qb + off, 0, 1024, 2), kId, ks > 0);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = ((k / 4) * (128 * 128) + (k % 4) * 32) >> 4;
+              mma_f16(tmem + (2 * x + sb) * 128, desc(kb + off), desc(qb + off), kId, k > 0);
             }
             mma_commit(s_full + 8 * (2 * x + sb));
+            if (x == 1) mma_commit(q_empty + 8 * s);
           }
-          mma_commit(q_empty + 8 * s);
+          __syncwarp();
         }
-        mma_commit(k_empty + 8 * b);
+        if (++s == kQStages) {
+          s = 0;
+          qpar ^= 1u;
+        }
       }
-      // the last commits arrive once every MMA is done; both buffers of K are
-      // then free (an item's k_empty is its n-th phase)
-      for (int64_t r = n - 1; r >= 0 && r >= n - 2; --r)
-        mbar_wait(k_empty + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
+      if (elect_one()) mma_commit(k_empty + 8 * b);
+      __syncwarp();
     }
+    // the last commits arrive once every MMA is done; both buffers of K are
+    // then free (an item's k_empty is its n-th phase)
+    for (int64_t r = n - 1; r >= 0 && r >= n - 2; --r)
+      mbar_wait(k_empty + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
   } else {
     // ---------------- stream x: a slot per thread ----------------
     const int x = warp >> 2, r0 = (warp & 3) * 32 + lane;
