@@ -124,35 +124,43 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedCacheParams& c, const i
   return r;
 }
 
-// sum_{i < n} floor((a i + b) / m) for non-negative a, b, n and m > 0, by the
-// Euclidean reduction of lattice points under a line.
-__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+// sum_{i < n} floor((a i + b) / m) for m > 0 and a n + b < 2^32, by the Euclidean
+// reduction of lattice points under a line (32-bit divisions: every CTA starts
+// with a few of these).
+__host__ __device__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   int64_t ans = 0;
   while (n > 0) {
     if (a >= m) {
-      ans += n * (n - 1) / 2 * (a / m);
-      a %= m;
+      const uint32_t q = a / m;
+      ans += static_cast<int64_t>(n) * (n - 1) / 2 * q;
+      a -= q * m;
     }
     if (b >= m) {
-      ans += n * (b / m);
-      b %= m;
+      const uint32_t q = b / m;
+      ans += static_cast<int64_t>(n) * q;
+      b -= q * m;
     }
-    const int64_t y = a * n + b;
+    const uint32_t y = a * n + b;
     if (y < m) break;
     n = y / m;
-    b = y % m;
-    const int64_t t = m;
+    b = y - n * m;
+    const uint32_t t = m;
     m = a;
     a = t;
   }
   return ans;
+}
+// a * b / c, a * b mostly below 2^32
+__host__ __device__ inline int64_t mul_div(int64_t a, int64_t b, int64_t c) {
+  const int64_t x = a * b;
+  return x < (1ll << 32) ? static_cast<uint32_t>(x) / static_cast<uint32_t>(c) : x / c;
 }
 
 // The tiles of one sequence: `tiles` of them, `tt` tokens each, and their units.
 struct TileCosts {
   int n, len, tt, kt, causal, tiles;
   __host__ __device__ TileCosts(int n_, int len_, int tt_, int kt_, int causal_)
-      : n(n_), len(len_), tt(tt_), kt(kt_), causal(causal_), tiles(n_ > 0 ? (n_ + tt_ - 1) / tt_ : 0) {}
+      : n(n_), len(len_), tt(tt_), kt(kt_), causal(causal_), tiles(n_ > 0 ? static_cast<int>((static_cast<uint32_t>(n_) + tt_ - 1) / static_cast<uint32_t>(tt_)) : 0) {}
   // slots the tile's last row sees
   __host__ __device__ int seen(int r) const {
     if (!causal) return len;
@@ -161,7 +169,7 @@ struct TileCosts {
     return e > 0 ? static_cast<int>(e) : 0;
   }
   __host__ __device__ int units(int r) const {
-    const int u = (seen(r) + kt - 1) / kt;
+    const int u = static_cast<int>((static_cast<uint32_t>(seen(r)) + kt - 1) / static_cast<uint32_t>(kt));
     return u > 0 ? u : 1;
   }
   // units of tiles 0 .. r-1
@@ -173,18 +181,33 @@ struct TileCosts {
       --r;
     }
     // tile i < tiles - 1 sees base + (i + 1) tt slots; one unit while that is at most kt
-    const int64_t base = static_cast<int64_t>(len) - n;
-    int64_t one = base >= kt ? 0 : (kt - base) / tt;
+    const int base = len - n;
+    int one = base >= kt ? 0 : static_cast<int>(static_cast<uint32_t>(kt - base) / static_cast<uint32_t>(tt));
     if (one > r) one = r;
-    return extra + one + floor_sum(r - one, kt, tt, base + (one + 1) * tt + kt - 1);
+    // sum_{i < m} floor((a i + b) / kt); kt is a constant power of two in every
+    // kernel, so this first step of floor_sum has no division
+    const uint32_t m = r - one, k = kt;
+    uint32_t a = tt, b = static_cast<uint32_t>(base + (static_cast<int64_t>(one) + 1) * tt + kt - 1);
+    if (m == 0) return extra + one;
+    int64_t sum = extra + one + static_cast<int64_t>(m) * (m - 1) / 2 * (a / k) + static_cast<int64_t>(m) * (b / k);
+    a %= k;
+    b %= k;
+    const uint32_t y = a * m + b;
+    return sum + (a && y >= k ? floor_sum(y / k, a, k, y % k) : 0);
   }
-  // the tile unit u (of the sequence's units of one head) lies in
-  __host__ __device__ int find(int64_t u) const {
-    int lo = 0, hi = tiles - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (before(mid) <= u) lo = mid;
-      else hi = mid - 1;
+  // The tile that unit u (of the sequence's units of one head) lies in, and the
+  // units before it: a 32-way search by a full warp.
+  __device__ int find(int64_t u, int64_t& first) const {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, width = tiles;                 // the tile is in [lo, lo + width)
+    first = 0;
+    while (width > 1) {
+      const int step = (width + 31) / 32, t = lo + lane * step;
+      const int64_t b = lane * step < width ? before(t) : u + 1;
+      const int hit = 31 - __clz(__ballot_sync(0xffffffffu, b <= u));
+      first = __shfl_sync(0xffffffffu, b, hit);
+      width = min(step, lo + width - (lo + hit * step));
+      lo += hit * step;
     }
     return lo;
   }
@@ -206,29 +229,35 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
                                       int64_t grid, PagedWalk& w) {
   const int lane = threadIdx.x & 31;
   const int hk = p.c.h_kv;
-  int64_t mine = 0;
+  // the first 32 sequences stay in registers for the second look
+  PagedSeq q_first{0, 0, 0};
+  int64_t mine = 0, cost_first = 0;
   for (int s = lane; s < p.c.batch; s += 32) {
     const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, s);
     const TileCosts t(q.n, q.len, tt, kt, p.causal);
-    mine += t.before(t.tiles) * hk;
+    const int64_t cost = t.before(t.tiles) * hk;
+    if (s < 32) {
+      q_first = q;
+      cost_first = cost;
+    }
+    mine += cost;
   }
   int64_t total = mine;
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  int64_t ctas = (total + min_units - 1) / min_units;
-  if (ctas > grid) ctas = grid;
+  int64_t ctas = total >= grid * min_units ? grid : mul_div(total + min_units - 1, 1, min_units);
   w.total = total;
   w.ctas = ctas;
   if (cta >= ctas) return false;
-  w.u = cta * total / ctas;
-  w.end = (cta + 1) * total / ctas;
+  w.u = mul_div(cta, total, ctas);
+  w.end = mul_div(cta + 1, total, ctas);
   // the sequence holding unit w.u: running totals over groups of 32 sequences
   int64_t base = 0;
   for (int s0 = 0;; s0 += 32) {
     const int s = s0 + lane;
-    int64_t cost = 0;
-    PagedSeq q{0, 0, 0};
-    if (s < p.c.batch) {
+    int64_t cost = s0 == 0 ? cost_first : 0;
+    PagedSeq q = q_first;
+    if (s0 > 0 && s < p.c.batch) {
       q = paged_seq(p.c, p.q_starts, p.rows, s);
       const TileCosts t(q.n, q.len, tt, kt, p.causal);
       cost = t.before(t.tiles) * hk;
@@ -250,10 +279,10 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
       w.q0 = __shfl_sync(0xffffffffu, q.q0, src);
       const TileCosts t(w.n, w.len, tt, kt, p.causal);
       const int64_t per = t.before(t.tiles), off = w.u - first;
-      w.head = static_cast<int>(off / per);
-      const int64_t in_head = off - w.head * per;
-      w.tile = t.find(in_head);
-      w.item_first = first + w.head * per + t.before(w.tile);
+      w.head = static_cast<int>(mul_div(off, 1, per));
+      int64_t in_tiles;
+      w.tile = t.find(off - w.head * per, in_tiles);
+      w.item_first = first + w.head * per + in_tiles;
       w.units = t.units(w.tile);
       return true;
     }
@@ -286,7 +315,8 @@ __device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt,
 
 // The CTA that holds unit u: the last c with floor(c W / G) <= u.
 __device__ __forceinline__ int unit_cta(const PagedWalk& w, int64_t u) {
-  return static_cast<int>(((u + 1) * w.ctas - 1) / w.total);
+  const int64_t x = (u + 1) * w.ctas - 1;
+  return static_cast<int>(x < (1ll << 32) ? static_cast<uint32_t>(x) / static_cast<uint32_t>(w.total) : x / w.total);
 }
 __device__ __forceinline__ PagedSplit paged_split(const PagedAttnParams& p, const PagedWalk& w, int tt) {
   const int tok0 = w.tile * tt;

@@ -345,6 +345,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int x = warp >> 2, r = (warp & 3) * 32 + lane;  // row of the stream, its TMEM lane
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lane_base + x * 128, o_addr = tmem + lane_base + 256 + x * D;
+    // the warp's rows of its stream's Q tile: 16-byte piece pc of row rr
+    constexpr int kPieces = D / 8;
+    unsigned char* stage = q_tile + x * G::kTileBytes + (warp & 3) * 32 * 128;
+    auto stage_at = [](int rr, int pc) { return (pc / 8) * (kKT * 128) + rr * 128 + (((pc % 8) ^ (rr & 7)) << 4); };
     const float c = p.inv_scale * kLog2e;
     uint32_t s_ph = 0, o_ph = 0, v_ph = 0;
     int name = 1;
@@ -378,20 +382,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const int tok = tok0 + min(row, rows - 1) / p.group, head = w.head * p.group + row % p.group;
       const int lim = p.causal ? max(w.len - w.n + tok + 1, 0) : w.len;     // slots this row sees
       const int lim0 = p.causal ? max(w.len - w.n + tok0 + (x * 128) / p.group + 1, 0) : w.len;   // the stream's first row
-      // ---- Q ----
-      {
-        unsigned char* dst = q_tile + x * G::kTileBytes + r * 128;
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (w.q0 + tok) * p.q_sn +
-                                                          static_cast<int64_t>(head) * p.q_sh);
+      // ---- Q: a warp brings its own 32 rows, whole rows side by side ----
+      const int64_t q_at = (w.q0 + tok) * p.q_sn + static_cast<int64_t>(head) * p.q_sh;
+      const unsigned alive = __ballot_sync(0xffffffffu, live);
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 f = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-          *reinterpret_cast<uint4*>(dst + (i / 8) * (kKT * 128) + (((i % 8) ^ (r & 7)) << 4)) = f;
-        }
-        fence_proxy_async();
-        fence_before();
-        arrive(q_full + 8 * x);
+      for (int it = 0; it < kPieces; ++it) {
+        const int rr = it * (32 / kPieces) + lane / kPieces, pc = lane % kPieces;
+        const T* src = static_cast<const T*>(p.q) + __shfl_sync(0xffffffffu, q_at, rr) + pc * 8;
+        unsigned char* dst = stage + stage_at(rr, pc);
+        if ((alive >> rr) & 1u) cp_async16(smem_u32(dst), src);
+        else *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
       }
+      cp_commit();
+      cp_wait<0>();
+      fence_proxy_async();
+      fence_before();
+      arrive(q_full + 8 * x);
       float m = -INFINITY, l = 0.f;
       int k0 = static_cast<int>(w.u - w.item_first) * kKT;
       for (int i = 0; i < units; ++i, k0 += kKT, name = name_next(name)) {
@@ -501,28 +507,57 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (!wait(o_full + 8 * x, o_ph)) break;
       o_ph ^= 1u;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* out = static_cast<T*>(p.out) + (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh;
+      // through the warp's own rows of the Q tile, which no product reads any
+      // more, so that whole rows are stored side by side
+      const int64_t o_at = (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh;
       float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + row) * (D + 4);
+      if (whole) {
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t o[32];
-        tmem_ld32_async(o_addr + c0, o);
-        tmem_wait();
-        if (!live) continue;
-        if (whole) {
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32_async(o_addr + c0, o);
+          tmem_wait();
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
+          for (int e = 0; e < 32; e += 8) {
             uint4 f;
-            f.x = pack2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-            f.y = pack2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-            f.z = pack2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-            f.w = pack2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + c0 + i) = f;
+            f.x = pack2<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+            f.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            f.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+            f.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+            *reinterpret_cast<uint4*>(stage + stage_at(lane, (c0 + e) / 8)) = f;
           }
-        } else {
+        }
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(part + c0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        for (int it = 0; it < kPieces; ++it) {
+          const int rr = it * (32 / kPieces) + lane / kPieces, pc = lane % kPieces;
+          T* dst = static_cast<T*>(p.out) + __shfl_sync(0xffffffffu, o_at, rr) + pc * 8;
+          if ((alive >> rr) & 1u) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(stage + stage_at(rr, pc));
+        }
+        __syncwarp();
+      } else {
+        // D / 2 columns in fp32 fill a staged row
+        float* rows0 = part - static_cast<int64_t>(lane) * (D + 4);
+#pragma unroll
+        for (int h0 = 0; h0 < D; h0 += D / 2) {
+#pragma unroll
+          for (int c0 = 0; c0 < D / 2; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld32_async(o_addr + h0 + c0, o);
+            tmem_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(stage + stage_at(lane, (c0 + e) / 4)) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int it = 0; it < kPieces; ++it) {
+            const int rr = it * (32 / kPieces) + lane / kPieces, pc = lane % kPieces;
+            if ((alive >> rr) & 1u)
+              *reinterpret_cast<uint4*>(rows0 + rr * (D + 4) + h0 + pc * 4) =
+                  *reinterpret_cast<const uint4*>(stage + stage_at(rr, pc));
+          }
+          __syncwarp();
         }
       }
       if (live) {
