@@ -4,7 +4,10 @@
 // Attention work is a line of units.  An item is (sequence, KV head, tile of
 // query rows): the g heads of a KV group at `tokens` consecutive new tokens
 // are the rows of one tile.  Its units are the key tiles of KT slots its last
-// row sees (one unit where it sees none, so that its zero rows are written).
+// row sees (one where it sees none, so that its zero rows are written), after
+// `extra` units that stand for what an item costs besides its tiles (its query
+// rows, its results, the pipeline's first and last steps): without them a CTA
+// whose share is many short items would run long.
 // Items follow one another by sequence, head, tile.  CTA c of G takes units
 // [c W / G, (c + 1) W / G) of the W there are, whatever the lengths of the
 // batch: ragged batches and long contexts of few rows spread evenly, with no
@@ -158,9 +161,9 @@ __host__ __device__ inline int64_t mul_div(int64_t a, int64_t b, int64_t c) {
 
 // The tiles of one sequence: `tiles` of them, `tt` tokens each, and their units.
 struct TileCosts {
-  int n, len, tt, kt, causal, tiles;
-  __host__ __device__ TileCosts(int n_, int len_, int tt_, int kt_, int causal_)
-      : n(n_), len(len_), tt(tt_), kt(kt_), causal(causal_), tiles(n_ > 0 ? static_cast<int>((static_cast<uint32_t>(n_) + tt_ - 1) / static_cast<uint32_t>(tt_)) : 0) {}
+  int n, len, tt, kt, more, causal, tiles;
+  __host__ __device__ TileCosts(int n_, int len_, int tt_, int kt_, int extra, int causal_)
+      : n(n_), len(len_), tt(tt_), kt(kt_), more(extra), causal(causal_), tiles(n_ > 0 ? static_cast<int>((static_cast<uint32_t>(n_) + tt_ - 1) / static_cast<uint32_t>(tt_)) : 0) {}
   // slots the tile's last row sees
   __host__ __device__ int seen(int r) const {
     if (!causal) return len;
@@ -168,16 +171,19 @@ struct TileCosts {
     const int64_t e = static_cast<int64_t>(len) - n + last;
     return e > 0 ? static_cast<int>(e) : 0;
   }
-  __host__ __device__ int units(int r) const {
+  // its key tiles, and its units
+  __host__ __device__ int key_tiles(int r) const {
     const int u = static_cast<int>((static_cast<uint32_t>(seen(r)) + kt - 1) / static_cast<uint32_t>(kt));
     return u > 0 ? u : 1;
   }
+  __host__ __device__ int units(int r) const { return key_tiles(r) + more; }
   // units of tiles 0 .. r-1
-  __host__ __device__ int64_t before(int r) const {
-    if (!causal) return static_cast<int64_t>(r) * units(0);
+  __host__ __device__ int64_t before(int r) const { return key_tiles_before(r) + static_cast<int64_t>(r) * more; }
+  __host__ __device__ int64_t key_tiles_before(int r) const {
+    if (!causal) return static_cast<int64_t>(r) * key_tiles(0);
     int64_t extra = 0;
     if (r == tiles && r > 0) {                 // the last tile may be short
-      extra = units(r - 1);
+      extra = key_tiles(r - 1);
       --r;
     }
     // tile i < tiles - 1 sees base + (i + 1) tt slots; one unit while that is at most kt
@@ -225,7 +231,7 @@ struct PagedWalk {
 // Total units, and the walk of CTA `cta` of `grid` (CTAs of less than
 // `min_units` each are not made: the rest stay idle).  Called by one full
 // warp; every lane gets the result.  False: no work.
-__device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int min_units, int64_t cta,
+__device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int extra, int min_units, int64_t cta,
                                       int64_t grid, PagedWalk& w) {
   const int lane = threadIdx.x & 31;
   const int hk = p.c.h_kv;
@@ -234,7 +240,7 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
   int64_t mine = 0, cost_first = 0;
   for (int s = lane; s < p.c.batch; s += 32) {
     const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, s);
-    const TileCosts t(q.n, q.len, tt, kt, p.causal);
+    const TileCosts t(q.n, q.len, tt, kt, extra, p.causal);
     const int64_t cost = t.before(t.tiles) * hk;
     if (s < 32) {
       q_first = q;
@@ -259,7 +265,7 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
     PagedSeq q = q_first;
     if (s0 > 0 && s < p.c.batch) {
       q = paged_seq(p.c, p.q_starts, p.rows, s);
-      const TileCosts t(q.n, q.len, tt, kt, p.causal);
+      const TileCosts t(q.n, q.len, tt, kt, extra, p.causal);
       cost = t.before(t.tiles) * hk;
     }
     int64_t incl = cost;
@@ -277,7 +283,7 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
       w.n = __shfl_sync(0xffffffffu, q.n, src);
       w.len = __shfl_sync(0xffffffffu, q.len, src);
       w.q0 = __shfl_sync(0xffffffffu, q.q0, src);
-      const TileCosts t(w.n, w.len, tt, kt, p.causal);
+      const TileCosts t(w.n, w.len, tt, kt, extra, p.causal);
       const int64_t per = t.before(t.tiles), off = w.u - first;
       w.head = static_cast<int>(mul_div(off, 1, per));
       int64_t in_tiles;
@@ -293,9 +299,9 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
 
 // The item after the current one (w.u is its first unit).  Every lane of a
 // warp, or a single thread, may call it: no exchange between lanes.
-__device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt, PagedWalk& w) {
+__device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt, int extra, PagedWalk& w) {
   w.item_first += w.units;
-  TileCosts t(w.n, w.len, tt, kt, p.causal);
+  TileCosts t(w.n, w.len, tt, kt, extra, p.causal);
   if (++w.tile >= t.tiles) {
     w.tile = 0;
     if (++w.head >= p.c.h_kv) {
@@ -307,7 +313,7 @@ __device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt,
         w.len = q.len;
         w.q0 = q.q0;
       } while (w.n == 0);
-      t = TileCosts(w.n, w.len, tt, kt, p.causal);
+      t = TileCosts(w.n, w.len, tt, kt, extra, p.causal);
     }
   }
   w.units = t.units(w.tile);
@@ -318,10 +324,32 @@ __device__ __forceinline__ int unit_cta(const PagedWalk& w, int64_t u) {
   const int64_t x = (u + 1) * w.ctas - 1;
   return static_cast<int>(x < (1ll << 32) ? static_cast<uint32_t>(x) / static_cast<uint32_t>(w.total) : x / w.total);
 }
-__device__ __forceinline__ PagedSplit paged_split(const PagedAttnParams& p, const PagedWalk& w, int tt) {
+__device__ __forceinline__ PagedSplit paged_split(const PagedAttnParams& p, const PagedWalk& w, int tt, int extra) {
   const int tok0 = w.tile * tt;
   return PagedSplit{w.item_first, w.q0 + tok0, w.head, (w.n - tok0 < tt ? w.n - tok0 : tt) * p.group,
-                    unit_cta(w, w.item_first), unit_cta(w, w.item_first + w.units - 1), 1};
+                    unit_cta(w, w.item_first + extra), unit_cta(w, w.item_first + w.units - 1), 1};
+}
+// The key tiles [first, last) of the current item that are this CTA's (none
+// where its share holds only units of `extra`), and whether that is all of them.
+struct PagedSegment {
+  int first, last;
+  bool whole;
+};
+__device__ __forceinline__ PagedSegment paged_segment(const PagedWalk& w, int extra) {
+  const int64_t item_end = w.item_first + w.units, end = w.end < item_end ? w.end : item_end;
+  const int64_t a = w.u - w.item_first - extra, b = end - w.item_first - extra;
+  PagedSegment s;
+  s.first = a > 0 ? static_cast<int>(a) : 0;
+  s.last = b > 0 ? static_cast<int>(b) : 0;
+  s.whole = s.first == 0 && end == item_end;
+  return s;
+}
+// To the first unit past the current item; false if that is not this CTA's.
+__device__ __forceinline__ bool paged_advance(const PagedAttnParams& p, int tt, int kt, int extra, PagedWalk& w) {
+  w.u = w.item_first + w.units;
+  if (w.u >= w.end) return false;
+  paged_next_item(p, tt, kt, extra, w);
+  return true;
 }
 
 __host__ __device__ inline int tile_tokens(int tile_rows, int group) { return tile_rows / group; }

@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kKT = 64;            // slots per key tile
 constexpr int kThreads = 256;
+constexpr int kExtra = 1;          // units an item costs besides its tiles
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -156,13 +157,16 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int tt = tile_tokens(R, p.group), d = p.c.d;
   PagedWalk w;
-  const bool any = paged_schedule(p, tt, kKT, 1, blockIdx.x, gridDim.x, w);
+  const bool any = paged_schedule(p, tt, kKT, kExtra, 1, blockIdx.x, gridDim.x, w);
   if (!any) {
     if (tid == 0) p.split[blockIdx.x].valid = 0;
     return;
   }
-  if (tid == 0) p.split[blockIdx.x] = paged_split(p, w, tt);
-  for (int slot = 0; w.u < w.end; slot = 1) {
+  if (tid == 0) p.split[blockIdx.x] = paged_split(p, w, tt, kExtra);
+  bool going = true;
+  for (int slot = 0; going; slot = 1, going = paged_advance(p, tt, kKT, kExtra, w)) {
+    const PagedSegment seg = paged_segment(w, kExtra);
+    if (seg.first == seg.last) continue;
     const TileRows t = tile_rows(w, tt, p.group);
     __syncthreads();
     load_rows<T>(p, w.q0, w.head, t, R, G::QS, qs);
@@ -180,9 +184,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
     }
     const int tile_min = seen_slots(p, w.n, w.len, t.tok0);                              // every row sees these
     const int tile_max = seen_slots(p, w.n, w.len, t.tok0 + t.rows / p.group - 1);       // some row sees these
-    const int64_t from = w.u, stop = min(w.end, w.item_first + w.units);
-    for (; w.u < stop; ++w.u) {
-      const int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+    for (int kt = seg.first; kt < seg.last; ++kt) {
+      const int k0 = kt * kKT;
       tile_offsets(p.c, w.seq, w.head, k0, tile_max, koff, voff);
       __syncthreads();
       load_tile<T>(p.c.k, koff, d, d, G::QS, ks);
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
       }
       __syncthreads();
     }
-    const bool whole = from == w.item_first && stop == w.item_first + w.units;
+    const bool whole = seg.whole;
 #pragma unroll
     for (int i = 0; i < RI; ++i) {
 #pragma unroll
@@ -296,20 +299,19 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
         }
       }
     }
-    if (w.u < w.end) paged_next_item(p, tt, kKT, w);
   }
 }
 
 // ---------------------------------------------------------------------------
 // join of the items cut by CTA boundaries.  Block b looks at the boundary
-// before CTA b + 1: if it is the first one inside its item, the block joins the
-// item's rows, a warp per row, over the CTAs that hold parts of it, in CTA
+// before CTA b + 1: if it is the first one inside its item, the blocks (b, y) join
+// the item's rows, a warp per row, over the CTAs that hold parts of it, in CTA
 // order, in one pass with a running maximum.  A matter of latency: everything
 // it needs to find its rows is in the two split records, and the parts of a
 // row are loaded four at a time.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(1024) combine_kernel(PagedAttnParams p, int R) {
+__global__ void __launch_bounds__(256) combine_kernel(PagedAttnParams p, int R) {
   const int b = blockIdx.x + 1;
   const PagedSplit it = p.split[b];
   const int64_t before = p.split[b - 1].item_first;
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(1024) combine_kernel(PagedAttnParams p, int R)
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int64_t step = static_cast<int64_t>(2) * R * pd;
   const int x0 = 4 * lane, x1 = x0 + 128;                           // this lane's columns
-  for (int r = warp; r < it.rows; r += blockDim.x / kWarp) {
+  for (int r = blockIdx.y * (blockDim.x / kWarp) + warp; r < it.rows; r += gridDim.y * (blockDim.x / kWarp)) {
     const float* src = p.part + (static_cast<int64_t>(b - 1) * 2 * R + r) * pd;
     float m = -INFINITY, l = 0.f;
     float4 o0 = make_float4(0.f, 0.f, 0.f, 0.f), o1 = o0;
@@ -506,11 +508,12 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
       e = a.rows == 64 ? launch_simt_t<64>(p, dt, a.grid, false, st) : launch_simt_t<16>(p, dt, a.grid, false, st);
   }
   if (e != cudaSuccess) return e;
-  const int threads = a.rows == 16 ? 512 : 1024;
+  // one wave of blocks: two warps' rows each for few rows, four for many
+  const dim3 grid(a.grid - 1, a.rows == 256 ? 8 : a.rows / 8);
   switch (dt) {
-    case SSA_F32: combine_kernel<float><<<a.grid - 1, threads, 0, st>>>(p, a.rows); break;
-    case SSA_BF16: combine_kernel<__nv_bfloat16><<<a.grid - 1, threads, 0, st>>>(p, a.rows); break;
-    default: combine_kernel<__half><<<a.grid - 1, threads, 0, st>>>(p, a.rows); break;
+    case SSA_F32: combine_kernel<float><<<grid, 256, 0, st>>>(p, a.rows); break;
+    case SSA_BF16: combine_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, a.rows); break;
+    default: combine_kernel<__half><<<grid, 256, 0, st>>>(p, a.rows); break;
   }
   e = cudaGetLastError();
   if (e != cudaSuccess || !p.c.w) return e;

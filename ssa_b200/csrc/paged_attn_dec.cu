@@ -33,6 +33,7 @@ using namespace tc;
 
 constexpr int kRows = 16;
 constexpr int kKT = 64;
+constexpr int kExtra = 2;          // units an item costs besides its tiles
 constexpr int kWarps = 4;          // consumers, 16 slots of a tile each
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr float kLog2e = 1.4426950408889634f;
@@ -73,8 +74,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
     prefetch_tensormap(&vmap);
   }
   PagedWalk w;
-  const bool any = paged_schedule(p, tt, kKT, 1, blockIdx.x, gridDim.x, w);
-  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt) : PagedSplit{};
+  const bool any = paged_schedule(p, tt, kKT, kExtra, 1, blockIdx.x, gridDim.x, w);
+  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
   __syncthreads();
   if (!any) return;
   auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -92,20 +93,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
     const int kv = lane / boxes, box = lane - kv * boxes, piece = box & (pieces - 1), half = box / pieces;
     const uint32_t box_at = ring + kv * G::kTileBytes + half * (kKT * 128) + piece * piece_rows * 128;
     int64_t g = 0;
-    while (w.u < w.end) {
+    bool going = true;
+    for (; going; going = going && paged_advance(p, tt, kKT, kExtra, w)) {
+      const PagedSegment seg = paged_segment(w, kExtra);
+      if (seg.first == seg.last) continue;
       const int last_tok = min(w.tile * tt + tt, w.n) - 1;
       const int lim = p.causal ? max(w.len - w.n + last_tok + 1, 0) : w.len;
-      const int64_t end = min(w.end, w.item_first + w.units);
-      int j = static_cast<int>(w.u - w.item_first) * kKT + piece * piece_rows;
+      int j = seg.first * kKT + piece * piece_rows;
       PageSpot next = page_spot(p.c, w.seq, j, kv < 2 ? lim : 0);
-      for (; w.u < end; ++w.u, ++g) {
+      for (int t = seg.first; t < seg.last; ++t, ++g) {
         const PageSpot at = next;
         j += kKT;
-        if (w.u + 1 < end) next = page_spot(p.c, w.seq, j, kv < 2 ? lim : 0);
+        if (t + 1 < seg.last) next = page_spot(p.c, w.seq, j, kv < 2 ? lim : 0);
         const int s = static_cast<int>(g % G::kStages);
         wait(empty + 8 * s, static_cast<uint32_t>((g / G::kStages) & 1) ^ 1u);
         if (__any_sync(0xffffffffu, *abort_flag)) {
-          w.u = w.end;
+          going = false;
           break;
         }
         if (lane == 0) mbar_expect_tx(full + 8 * s, 2 * G::kTileBytes);
@@ -114,7 +117,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
           tma_load_4d(box_at + 2 * s * G::kTileBytes, kv ? &vmap : &kmap, half * 64, mo.head_first ? w.head : at.row,
                       mo.head_first ? at.row : w.head, at.page, full + 8 * s);
       }
-      if (w.u < w.end) paged_next_item(p, tt, kKT, w);
     }
     // every issued copy lands before the CTA exits
     if (lane == 0)
@@ -131,9 +133,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
   const int kk = (lane >> 4) * 8 + (lane & 7), kp = (lane >> 3) & 1;
   const int vk = ((lane >> 3) & 1) * 8 + (lane & 7), vp = lane >> 4;
   int64_t g = 0;
-  for (int slot = 0; w.u < w.end; slot = 1) {
+  bool going = true;
+  for (int slot = 0; going; slot = 1, going = paged_advance(p, tt, kKT, kExtra, w)) {
+    const PagedSegment seg = paged_segment(w, kExtra);
+    if (seg.first == seg.last) continue;
     const int tok0 = w.tile * tt, rows = min(tt, w.n - tok0) * p.group;
-    const int64_t from = w.u, end = min(w.end, w.item_first + w.units);
     uint32_t q[KS][4];
     int lim[2];
     float* sc[2];
@@ -157,9 +161,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
-    for (; w.u < end; ++w.u, ++g) {
+    for (int t = seg.first; t < seg.last; ++t, ++g) {
       const int st = static_cast<int>(g % G::kStages);
-      const int k0 = static_cast<int>(w.u - w.item_first) * kKT + warp * 16;
+      const int k0 = t * kKT + warp * 16;
       wait(full + 8 * st, static_cast<uint32_t>((g / G::kStages) & 1));
       __syncwarp();
       const uint32_t kb = ring + 2 * st * G::kTileBytes, vb = kb + G::kTileBytes;
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
         fy[y] = ex2_approx(src[D] - off);
         sum = fmaf(fy[y], src[D + 1], sum);
       }
-      const bool whole = from == w.item_first && end == w.item_first + w.units;
+      const bool whole = seg.whole;
       const int tok = tok0 + r / p.group, head = w.head * p.group + r % p.group;
       const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
       T* out = static_cast<T*>(p.out) + (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh + x0;
@@ -348,7 +352,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
       }
     }
     asm volatile("barrier.cta.sync 1, 128;" ::: "memory");   // before the next item's partials overwrite these
-    if (w.u < w.end) paged_next_item(p, tt, kKT, w);
   }
 }
 

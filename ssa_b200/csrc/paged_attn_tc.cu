@@ -49,6 +49,7 @@ using namespace tc;
 
 constexpr int kRows = 256;         // rows of an item
 constexpr int kKT = 128;           // slots per key tile
+constexpr int kExtra = 4;          // units an item costs besides its tiles
 constexpr int kThreads = 320;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -176,12 +177,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   PagedWalk w;
-  const bool any = paged_schedule(p, tt, kKT, 1, blockIdx.x, gridDim.x, w);
+  const bool any = paged_schedule(p, tt, kKT, kExtra, 1, blockIdx.x, gridDim.x, w);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt) : PagedSplit{};
+  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
   auto fail = [&]() {
     *abort_flag = 1;
     paged_error(p.c, SSA_DEVICE_TIMEOUT);
@@ -204,16 +205,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     int st = 0;
     uint32_t par = 1;
     bool stop = false;
-    while (w.u < w.end && !stop) {
+    for (bool going = true; going && !stop; going = !stop && paged_advance(p, tt, kKT, kExtra, w)) {
+      const PagedSegment seg = paged_segment(w, kExtra);
+      if (seg.first == seg.last) continue;
       const int last_tok = min(w.tile * tt + tt, w.n) - 1;
       const int lim = p.causal ? max(w.len - w.n + last_tok + 1, 0) : w.len;
-      const int64_t end = min(w.end, w.item_first + w.units);
-      int j = static_cast<int>(w.u - w.item_first) * kKT + piece * piece_rows;
+      int j = seg.first * kKT + piece * piece_rows;
       PageSpot next = page_spot(p.c, w.seq, j, lane < boxes ? lim : 0);
-      for (; w.u < end && !stop; ++w.u) {
+      for (int t = seg.first; t < seg.last && !stop; ++t) {
         const PageSpot at = next;
         j += kKT;
-        if (w.u + 1 < end) next = page_spot(p.c, w.seq, j, lane < boxes ? lim : 0);
+        if (t + 1 < seg.last) next = page_spot(p.c, w.seq, j, lane < boxes ? lim : 0);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++g) {
           if (!__all_sync(0xffffffffu, mbar_wait_or(empty + 8 * st, par, abort_flag))) {
@@ -232,7 +234,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           }
         }
       }
-      if (!stop && w.u < w.end) paged_next_item(p, tt, kKT, w);
     }
     // every issued copy lands before the CTA exits
     if (lane == 0)
@@ -275,11 +276,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       if (elect_one()) mma_commit(empty + 8 * st);
       __syncwarp();
     };
-    while (w.u < w.end && !stop) {
+    for (bool going = true; going && !stop; going = !stop && paged_advance(p, tt, kKT, kExtra, w)) {
+      const PagedSegment seg = paged_segment(w, kExtra);
+      const int units = __shfl_sync(0xffffffffu, seg.last - seg.first, 0);
+      if (units == 0) continue;
       const int rows = min(tt, w.n - w.tile * tt) * p.group;
       const int streams = __shfl_sync(0xffffffffu, rows > 128 ? 2 : 1, 0);
-      const int64_t end = min(w.end, w.item_first + w.units);
-      const int units = __shfl_sync(0xffffffffu, static_cast<int>(end - w.u), 0);
       uint32_t fresh = 3;
       wait(full + 8 * ks, kpar);
       for (int x = 0; x < streams && !stop; ++x) {
@@ -331,8 +333,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         kpar = npar;
         name = name_next(name);
       }
-      w.u = end;
-      if (!stop && w.u < w.end) paged_next_item(p, tt, kKT, w);
     }
     // after a failed wait: the commit arrives once every MMA issued before it is done
     if (stop) {
@@ -366,15 +366,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    for (int slot = 0; w.u < w.end && !stop; slot = 1) {
+    bool going = true;
+    for (int slot = 0; going && !stop; slot = 1, going = !stop && paged_advance(p, tt, kKT, kExtra, w)) {
+      const PagedSegment seg = paged_segment(w, kExtra);
+      const int units = seg.last - seg.first;
+      if (units == 0) continue;
       const int tok0 = w.tile * tt, rows = min(tt, w.n - tok0) * p.group;
-      const int64_t end = min(w.end, w.item_first + w.units);
-      const int units = static_cast<int>(end - w.u);
-      const bool whole = w.u == w.item_first && end == w.item_first + w.units;
+      const bool whole = seg.whole;
       if (x == 1 && rows <= 128) {                        // nothing for this stream here
         for (int i = 0; i < units; ++i) name = name_next(name);
-        w.u = end;
-        if (w.u < w.end) paged_next_item(p, tt, kKT, w);
         continue;
       }
       const int row = x * 128 + r;
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       fence_before();
       arrive(q_full + 8 * x);
       float m = -INFINITY, l = 0.f;
-      int k0 = static_cast<int>(w.u - w.item_first) * kKT;
+      int k0 = seg.first * kKT;
       for (int i = 0; i < units; ++i, k0 += kKT, name = name_next(name)) {
         if (!wait(s_full + 8 * x, s_ph)) break;
         s_ph ^= 1u;
@@ -571,8 +571,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           part[D + 1] = l;
         }
       }
-      w.u = end;
-      if (w.u < w.end) paged_next_item(p, tt, kKT, w);
     }
   }
   fence_before();

@@ -41,7 +41,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 template <int D>
 struct Geo {
   static constexpr int kTileBytes = 128 * D * 2;
-  static constexpr size_t kSmem = 1024 + (4 + kQStages) * static_cast<size_t>(kTileBytes) + kQStages * kRows * 4 + 256;
+  static constexpr size_t kSmem = 1024 + (4 + kQStages) * static_cast<size_t>(kTileBytes) + kQStages * kRows * 4 + kRows * 2 + 192;
 };
 
 struct QueryMap {
@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* q_ring = base + 4 * G::kTileBytes;      // base: K [2 items][2 streams]
   float* z_ring = reinterpret_cast<float*>(q_ring + kQStages * G::kTileBytes);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(z_ring + kQStages * kRows);
+  short* row_token = reinterpret_cast<short*>(z_ring + kQStages * kRows);   // token of a row in its tile
+  uint64_t* bars = reinterpret_cast<uint64_t*>(row_token + kRows);
   const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, q_full = k_empty + 16, q_empty = q_full + 8 * kQStages;
   const uint32_t s_full = q_empty + 8 * kQStages, s_empty = s_full + 32;     // [stream][buffer]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 2 * kQStages + 8);
@@ -99,6 +100,10 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   // rows of a Q slot that no box fills (tokens * g < 128) read as zero queries
   for (int i = threadIdx.x; i < kQStages * G::kTileBytes / 16; i += kThreads)
     reinterpret_cast<uint4*>(q_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+  if (threadIdx.x < kRows) {
+    const int row = threadIdx.x, a = qm.head_first ? row / g : row % tt, h = qm.head_first ? row % g : row / tt;
+    row_token[row] = static_cast<short>(h < g && a < tt ? a : kRows);       // kRows: no row
+  }
   fence_proxy_async();
   if (threadIdx.x == 0) {
     for (int b = 0; b < 2; ++b) {
@@ -140,6 +145,15 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     const int piece_rows = min(p.c.page_size, kSlots), pieces = kSlots / piece_rows, boxes = pieces * (D / 64);
     const int piece = lane & (pieces - 1), half = lane / pieces;
     const int64_t h_q = static_cast<int64_t>(p.c.h_kv) * g;
+    // token and head of this lane's four rows of a Q tile (token `kRows`: no row)
+    int row_tok[4], row_head[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = lane + 32 * e;
+      row_tok[e] = qm.head_first ? row / g : row % tt;
+      row_head[e] = qm.head_first ? row % g : row / tt;
+      if (row_head[e] >= g || row_tok[e] >= tt) row_tok[e] = kRows;
+    }
     const uint32_t q_bytes = static_cast<uint32_t>(tt * g) * 128 * (D / 64);
     bool stop = false;
     for (int64_t i = blockIdx.x; !stop && seek(p, it, i); i += gridDim.x, ++n) {
@@ -159,28 +173,34 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
                       &kmap, half * 64, mo.head_first ? head : at.row, mo.head_first ? at.row : head, at.page,
                       k_full + 8 * b);
         }
-      for (int r = first_token(p, it.q, k0) / tt; r * tt < it.q.n; ++r, ++t) {
+      // lse2 of the next tile's rows is on its way while this tile's ring entry
+      // is waited for
+      int r = first_token(p, it.q, k0) / tt;
+      float z[4];
+      auto fetch = [&](int tile) {
+        const int64_t tok = it.q.q0 + static_cast<int64_t>(tile) * tt;
+        const int tokens = min(tt, it.q.n - tile * tt);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          z[e] = row_tok[e] < tokens ? __ldg(p.lse2 + (tok + row_tok[e]) * h_q + head * g + row_head[e]) : INFINITY;
+      };
+      if (r * tt < it.q.n) fetch(r);
+      for (; r * tt < it.q.n; ++r, ++t) {
         const int s = static_cast<int>(t % kQStages);
         wait(q_empty + 8 * s, static_cast<uint32_t>((t / kQStages) & 1) ^ 1u);
         stop = __any_sync(0xffffffffu, *abort_flag);
         if (stop) break;
         if (lane == 0) mbar_expect_tx(q_full + 8 * s, q_bytes);
         __syncwarp();
-        const int64_t tok = it.q.q0 + static_cast<int64_t>(r) * tt;
         if (lane < D / 64) {
-          const int y = head * g, zc = static_cast<int>(tok);
+          const int y = head * g, zc = static_cast<int>(it.q.q0) + r * tt;
           tma_load_3d(smem_u32(q_ring + s * G::kTileBytes) + lane * (kRows * 128), &qmap, lane * 64,
                       qm.head_first ? y : zc, qm.head_first ? zc : y, q_full + 8 * s);
         }
-        const int rows = min(tt, it.q.n - r * tt) * g;
 #pragma unroll
-        for (int e = lane; e < kRows; e += 32) {
-          const int a = qm.head_first ? e / g : e % tt, j = qm.head_first ? e % g : e / tt;
-          float z = INFINITY;                            // exp2(s - inf) = 0: no row
-          if (a * g < rows && j < g) z = p.lse2[(tok + a) * h_q + head * g + j];
-          z_ring[s * kRows + e] = z;
-        }
+        for (int e = 0; e < 4; ++e) z_ring[s * kRows + lane + 32 * e] = z[e];   // exp2(s - inf) = 0 where there is no row
         mbar_arrive(q_full + 8 * s);
+        if ((r + 1) * tt < it.q.n) fetch(r + 1);
       }
     }
     // every issued copy lands before the CTA exits
@@ -247,9 +267,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         wait(s_full + 8 * (2 * x + sb), static_cast<uint32_t>((t >> 1) & 1));
         __syncwarp();
         fence_after();
-        const int rows = min(tt, it.q.n - r * tt) * g;
         const int64_t lim0 = p.causal ? static_cast<int64_t>(it.q.len) - it.q.n + r * tt + 1 : it.q.len;
-        const bool masked = lim0 < k0 + (x + 1) * kSlots || rows < tt * g;
+        const bool masked = lim0 < k0 + (x + 1) * kSlots || it.q.n - r * tt < tt;
         const float4* zs = reinterpret_cast<const float4*>(z_ring + s * kRows);
         const uint32_t ta = tmem + lane_base + (2 * x + sb) * 128;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -269,14 +288,21 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
               sum[3] += ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 3]), c, -z.w));
             }
           } else {
-            const float* z1 = z_ring + s * kRows + 32 * q4;
+            // a row of token a sees the slot from token `from` on
+            const short4* ts = reinterpret_cast<const short4*>(row_token);
+            const int from = p.causal ? slot - (it.q.len - it.q.n) - r * tt : -1, tokens = min(tt, it.q.n - r * tt);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int e = 32 * q4 + j, a = qm.head_first ? e / g : e % tt, hh = qm.head_first ? e % g : e / tt;
-              const bool row = a * g < rows && hh < g;
-              const bool sees = row && (!p.causal || slot < it.q.len - it.q.n + r * tt + a + 1);
-              const float ex = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][j]), c, -z1[j]));
-              sum[j & 3] += sees ? ex : 0.f;
+            for (int j = 0; j < 8; ++j) {
+              const float4 z = zs[q4 * 8 + j];
+              const short4 a = ts[q4 * 8 + j];
+              const float e0 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j]), c, -z.x));
+              const float e1 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 1]), c, -z.y));
+              const float e2 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 2]), c, -z.z));
+              const float e3 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 3]), c, -z.w));
+              sum[0] += a.x >= from && a.x < tokens ? e0 : 0.f;
+              sum[1] += a.y >= from && a.y < tokens ? e1 : 0.f;
+              sum[2] += a.z >= from && a.z < tokens ? e2 : 0.f;
+              sum[3] += a.w >= from && a.w < tokens ? e3 : 0.f;
             }
           }
         }
