@@ -112,7 +112,8 @@ def _device_index(dev: torch.device) -> int:
 
 def host_word(dev: torch.device, op: int) -> Optional[int]:
     """Address of the error word of op number ``op`` (in ``_HostWords.OPS``), or
-    None with ``SSA_CHECKED=0``; raises for an error already found."""
+    None with ``SSA_CHECKED=0``; raises for an error already found.  To be
+    followed by :func:`host_word_done` where :func:`mode` is ``sync``."""
     if mode() == "off":
         return None
     key = _device_index(dev)
@@ -120,15 +121,15 @@ def host_word(dev: torch.device, op: int) -> Optional[int]:
     if w is None:
         with _lock:
             w = _words.setdefault(key, _HostWords())
-    elif any(w.view):
+    elif w.view[0] or w.view[1] or w.view[2]:
         _poll_words(dev)
     w.used = True
     return w.base + 4 * op
 
 
 def host_word_done(dev: torch.device) -> None:
-    """After the launch: with ``SSA_CHECKED=sync`` wait for it and raise now."""
-    if mode() == "sync" and not torch.cuda.is_current_stream_capturing():
+    """After the launch, with ``SSA_CHECKED=sync``: wait for it and raise now."""
+    if not torch.cuda.is_current_stream_capturing():
         torch.cuda.current_stream(dev).synchronize()
         _poll_words(dev)
 

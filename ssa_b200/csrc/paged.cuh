@@ -19,6 +19,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ssa {
@@ -353,6 +355,24 @@ __device__ __forceinline__ bool paged_advance(const PagedAttnParams& p, int tt, 
 }
 
 __host__ __device__ inline int tile_tokens(int tile_rows, int group) { return tile_rows / group; }
+
+// Allows a kernel its dynamic shared memory, once per device (one of these, static, per kernel).
+class SmemOptIn {
+ public:
+  cudaError_t operator()(const void* kernel, size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done_.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e == cudaSuccess) done_.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, ssa_dtype dt, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictParams& p, ssa_dtype dt, cudaStream_t st);

@@ -433,13 +433,15 @@ cudaError_t launch_simt(const PagedAttnParams& p, int grid, bool weights, cudaSt
   const int smem = static_cast<int>(SimtGeo<R, DP>::kSmem);
   if (!weights) {
     auto kern = attn_simt_kernel<T, R, DP>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemOptIn opt_in;
+    const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), smem);
     if (e != cudaSuccess) return e;
     kern<<<grid, kThreads, smem, st>>>(p);
     return cudaGetLastError();
   }
   auto kern = weights_simt_kernel<T, R, DP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static SmemOptIn opt_in;
+  const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), smem);
   if (e != cudaSuccess) return e;
   const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
   if (slots == 0) return cudaSuccess;

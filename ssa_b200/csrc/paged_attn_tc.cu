@@ -589,8 +589,8 @@ cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStrea
       !page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, kKT, &vm, &vo) || mo.head_first != vo.head_first)
     return cudaErrorInvalidValue;
   auto kern = attn_tc_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(Geo<D>::kSmem));
+  static SmemOptIn opt_in;
+  const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), Geo<D>::kSmem);
   if (e != cudaSuccess) return e;
   kern<<<grid, kThreads, Geo<D>::kSmem, st>>>(km, vm, p, mo);
   return cudaGetLastError();

@@ -55,121 +55,194 @@ __global__ void __launch_bounds__(256) append_kernel(PagedAppendParams p, int el
 // Order-preserving key of a weight; NaN ranks with -inf, below every number.
 __device__ __forceinline__ uint32_t weight_key(float w) { return float_key(w != w ? -INFINITY : w); }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
+constexpr int kSelBins = 2048;
+constexpr int kSelKeys = 49152;    // keys held in shared memory (192 KB); longer sequences are read again
 
 // One CTA per (sequence, KV head).  The n_keep heaviest of the first `older`
 // slots are those whose key exceeds the n_keep-th largest, T, and the first
-// few that equal it: T is found from its top byte down, each pass counting the
-// next byte of the keys that agree with T so far; then one pass in slot order
-// writes the kept slots.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(PagedEvictParams p) {
+// few that equal it.  The weights are read once into shared memory, eight
+// loads in flight a thread; T is found from its top bits down in three passes
+// of 11, 11 and 10 bits, each counting the next digit of the keys that agree
+// with T so far and finding the digit by a sum from the top over the 2048
+// counts; then every warp counts and writes the kept slots of its own run of
+// slots, in order.  Bound by latency: a dozen block-wide steps.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(PagedEvictParams p, int held) {
   const PagedCacheParams& c = p.c;
   const int s = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __shared__ int hist[256];
-  __shared__ uint32_t sh_prefix;
-  __shared__ int sh_left;
-  __shared__ int wsum[32][2];
+  extern __shared__ uint32_t sel_keys[];
+  __shared__ int hist[kSelBins];
+  __shared__ int wsum[kSelWarps][2];
+  __shared__ int found[2];
   const int len = max(paged_len(c, s), 0);
   const int size = min(len, p.budget), recent = min(p.recent, size), older = len - recent, n_keep = size - recent;
   int32_t* kept = p.kept + (static_cast<int64_t>(s) * c.h_kv + h) * p.budget;
   if (tid == 0 && h == 0) p.new_lens[s] = size;
-  auto key_of = [&](int j) -> uint32_t {
+  for (int j = size + tid; j < p.budget; j += kSelThreads) kept[j] = -1;
+  if (size == len) {
+    for (int j = tid; j < len; j += kSelThreads) kept[j] = j;
+    return;
+  }
+  auto read_key = [&](int j) -> uint32_t {
     int page, row;
     page_of(c, j, page, row);
     const int64_t pg = physical_page(c, c.table, c.table_stride, s, page);
     return pg < 0 ? 0u : weight_key(c.w[pg * c.w_sp + row * c.w_sn + h * c.w_sh]);
   };
-  uint32_t prefix = 0;
-  int left = n_keep;                       // of the keys that agree with the prefix, how many are kept
-  if (size < len) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int b = tid; b < 256; b += kSelThreads) hist[b] = 0;
-      __syncthreads();
-      for (int j = tid; j < older; j += kSelThreads) {
-        const uint32_t k = key_of(j);
-        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int l = left, b = 255;
-        while (b > 0 && hist[b] < l) l -= hist[b--];
-        sh_prefix = prefix | (static_cast<uint32_t>(b) << shift);
-        sh_left = l;
-      }
-      __syncthreads();
-      prefix = sh_prefix;
-      left = sh_left;
-      __syncthreads();
+  const bool hold = older <= held;
+  if (hold) {
+    for (int j0 = tid; j0 < older; j0 += 8 * kSelThreads) {
+      uint32_t k[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[e] = j0 + e * kSelThreads < older ? read_key(j0 + e * kSelThreads) : 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j0 + e * kSelThreads < older) sel_keys[j0 + e * kSelThreads] = k[e];
     }
   }
-  // slots in order: kept if above T, if among the first `left` equal to T, or recent
-  int out = 0, equal = 0;
-  for (int j0 = 0; j0 < len; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    bool gt = false, eq = false;
-    if (j < len) {
-      if (size == len || j >= older) gt = true;
-      else {
-        const uint32_t k = key_of(j);
-        gt = k > prefix;
-        eq = k == prefix;
+  __syncthreads();
+  auto key_of = [&](int j) -> uint32_t { return hold ? sel_keys[j] : read_key(j); };
+  uint32_t prefix = 0, known = 0;          // the bits of T found so far, and which
+  int left = n_keep;                       // of the keys that agree with them, how many are kept
+  for (int pass = 0; pass < 3 && n_keep > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
+    __syncthreads();
+    for (int j = tid; j - lane < older; j += kSelThreads) {
+      const uint32_t k = j < older ? key_of(j) : 0u;
+      const bool in = j < older && (k & known) == prefix;
+      const int bin = in ? static_cast<int>((k >> shift) & (bins - 1)) : -1;
+      // equal weights (a cache's first steps) would queue 32 deep on one counter
+      int same;
+      __match_all_sync(0xffffffffu, bin, &same);
+      if (same) {
+        if (lane == 0 && bin >= 0) atomicAdd(&hist[bin], 32);
+      } else if (in) {
+        atomicAdd(&hist[bin], 1);
       }
-    }
-    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) {
-      wsum[warp][0] = __popc(bg);
-      wsum[warp][1] = __popc(be);
     }
     __syncthreads();
-    const unsigned below = (1u << lane) - 1u;
-    int g0 = out + __popc(bg & below), e0 = equal + __popc(be & below), tg = 0, te = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) {
-      if (w < warp) {
-        g0 += wsum[w][0];
-        e0 += wsum[w][1];
-      }
-      tg += wsum[w][0];
-      te += wsum[w][1];
+    // the largest digit b with (keys of digits >= b) >= left: a thread has two
+    // digits, from the top
+    const int b0 = kSelBins - 1 - 2 * tid, c0 = hist[b0], c1 = hist[b0 - 1];
+    int incl = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
     }
+    if (lane == 31) wsum[warp][0] = incl;
+    __syncthreads();
+    int above = incl - c0 - c1;
+    for (int w = 0; w < warp; ++w) above += wsum[w][0];
+    if (above < left && left <= above + c0 + c1) {
+      const bool first = left <= above + c0;
+      found[0] = first ? b0 : b0 - 1;
+      found[1] = first ? left - above : left - above - c0;
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(found[0]) << shift;
+    known |= static_cast<uint32_t>(bins - 1) << shift;
+    left = found[1];
+  }
+  if (n_keep == 0) prefix = 0xffffffffu;   // no key exceeds it, and none that equals it is kept
+  // each warp's run of slots: kept if above T, if among the first `left` equal to T, or recent
+  const int run = ((len + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, lo = warp * run, hi = min(lo + run, len);
+  auto kind = [&](int j, bool& gt, bool& eq) {
+    gt = eq = false;
+    if (j >= hi) return;
+    if (j >= older) {
+      gt = true;
+    } else {
+      const uint32_t k = key_of(j);
+      gt = k > prefix;
+      eq = k == prefix;
+    }
+  };
+  int ng = 0, ne = 0;
+  for (int j = lo + lane; j - lane < hi; j += 32) {
+    bool gt, eq;
+    kind(j, gt, eq);
+    ng += __popc(__ballot_sync(0xffffffffu, gt));
+    ne += __popc(__ballot_sync(0xffffffffu, eq));
+  }
+  __syncthreads();
+  if (lane == 0) {
+    wsum[warp][0] = ng;
+    wsum[warp][1] = ne;
+  }
+  __syncthreads();
+  int out = 0, equal = 0;                  // slots above T, and equal to it, before this warp's run
+  {
+    const int g = lane < warp ? wsum[lane][0] : 0, e = lane < warp ? wsum[lane][1] : 0;
+    out = __reduce_add_sync(0xffffffffu, g);
+    equal = __reduce_add_sync(0xffffffffu, e);
+  }
+  const unsigned below = (1u << lane) - 1u;
+  for (int j = lo + lane; j - lane < hi; j += 32) {
+    bool gt, eq;
+    kind(j, gt, eq);
+    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+    const int g0 = out + __popc(bg & below), e0 = equal + __popc(be & below);
     if (gt) kept[g0 + min(e0, left)] = j;
     else if (eq && e0 < left) kept[g0 + e0] = j;
-    out += tg;
-    equal += te;
-    __syncthreads();
+    out += __popc(bg);
+    equal += __popc(be);
   }
-  for (int j = size + tid; j < p.budget; j += kSelThreads) kept[j] = -1;
 }
 
-// Kept slots' keys, values and weights to the new pages: one 16-byte piece of
-// K and of V per thread.
+// Kept slots' keys, values and weights to the new pages.  A thread moves one
+// 16-byte piece of K and of V of four slots, all of their loads in flight
+// together (the slot, its page and the data are three loads in a row).
+constexpr int kCopySlots = 4;
 __global__ void __launch_bounds__(256) evict_copy_kernel(PagedEvictParams p, int elem, int vecs) {
   const PagedCacheParams& c = p.c;
   const int s = blockIdx.z, h = blockIdx.y;
   const int size = min(max(paged_len(c, s), 0), p.budget);
   const int32_t* kept = p.kept + (static_cast<int64_t>(s) * c.h_kv + h) * p.budget;
-  const int64_t total = static_cast<int64_t>(size) * vecs;
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < total;
-       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int to = static_cast<int>(e / vecs), piece = static_cast<int>(e - static_cast<int64_t>(to) * vecs);
-    const int from = kept[to];
-    int page, row, npage, nrow;
-    page_of(c, from, page, row);
-    page_of(c, to, npage, nrow);
-    if (npage >= p.new_max_pages) {
-      paged_error(c, SSA_DEVICE_BAD_LENGTH);
-      continue;
+  const int per = 256 / vecs, lane_slot = threadIdx.x / vecs, piece = threadIdx.x - lane_slot * vecs;
+  if (lane_slot >= per) return;
+  const char* k = static_cast<const char*>(c.k);
+  const char* v = static_cast<const char*>(c.v);
+  for (int to0 = blockIdx.x * per * kCopySlots + lane_slot; to0 < size; to0 += gridDim.x * per * kCopySlots) {
+    int64_t src[kCopySlots], dst[kCopySlots];   // page, and row in the low bits
+    uint4 kx[kCopySlots], vx[kCopySlots];
+    float wx[kCopySlots];
+#pragma unroll
+    for (int e = 0; e < kCopySlots; ++e) {
+      const int to = to0 + e * per;
+      src[e] = dst[e] = -1;
+      if (to >= size) continue;
+      int page, row, npage, nrow;
+      page_of(c, kept[to], page, row);
+      page_of(c, to, npage, nrow);
+      if (npage >= p.new_max_pages) {
+        paged_error(c, SSA_DEVICE_BAD_LENGTH);
+        continue;
+      }
+      const int64_t pg = physical_page(c, c.table, c.table_stride, s, page);
+      const int64_t ng = physical_page(c, p.new_table, p.new_table_stride, s, npage);
+      if (pg >= 0 && ng >= 0) {
+        src[e] = pg << 10 | row;               // page_size <= 1024
+        dst[e] = ng << 10 | nrow;
+      }
     }
-    const int64_t pg = physical_page(c, c.table, c.table_stride, s, page);
-    const int64_t ng = physical_page(c, p.new_table, p.new_table_stride, s, npage);
-    if (pg < 0 || ng < 0) continue;
-    const char* k = static_cast<const char*>(c.k);
-    const char* v = static_cast<const char*>(c.v);
-    const uint4 kx = reinterpret_cast<const uint4*>(k + (pg * c.k_sp + row * c.k_sn + h * c.k_sh) * elem)[piece];
-    const uint4 vx = reinterpret_cast<const uint4*>(v + (pg * c.v_sp + row * c.v_sn + h * c.v_sh) * elem)[piece];
-    reinterpret_cast<uint4*>(const_cast<char*>(k) + (ng * c.k_sp + nrow * c.k_sn + h * c.k_sh) * elem)[piece] = kx;
-    reinterpret_cast<uint4*>(const_cast<char*>(v) + (ng * c.v_sp + nrow * c.v_sn + h * c.v_sh) * elem)[piece] = vx;
-    if (piece == 0)
-      c.w[ng * c.w_sp + nrow * c.w_sn + h * c.w_sh] = c.w[pg * c.w_sp + row * c.w_sn + h * c.w_sh];
+#pragma unroll
+    for (int e = 0; e < kCopySlots; ++e) {
+      if (src[e] < 0) continue;
+      const int64_t pg = src[e] >> 10, row = src[e] & 1023;
+      kx[e] = reinterpret_cast<const uint4*>(k + (pg * c.k_sp + row * c.k_sn + h * c.k_sh) * elem)[piece];
+      vx[e] = reinterpret_cast<const uint4*>(v + (pg * c.v_sp + row * c.v_sn + h * c.v_sh) * elem)[piece];
+      if (piece == 0) wx[e] = c.w[pg * c.w_sp + row * c.w_sn + h * c.w_sh];
+    }
+#pragma unroll
+    for (int e = 0; e < kCopySlots; ++e) {
+      if (src[e] < 0) continue;
+      const int64_t pg = dst[e] >> 10, row = dst[e] & 1023;
+      reinterpret_cast<uint4*>(const_cast<char*>(k) + (pg * c.k_sp + row * c.k_sn + h * c.k_sh) * elem)[piece] = kx[e];
+      reinterpret_cast<uint4*>(const_cast<char*>(v) + (pg * c.v_sp + row * c.v_sn + h * c.v_sh) * elem)[piece] = vx[e];
+      if (piece == 0) c.w[pg * c.w_sp + row * c.w_sn + h * c.w_sh] = wx[e];
+    }
   }
 }
 
@@ -186,10 +259,17 @@ cudaError_t launch_paged_append(const PagedAppendParams& p, ssa_dtype dt, cudaSt
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, ssa_dtype dt, cudaStream_t st) {
   const int elem = dt == SSA_F32 ? 4 : 2, vecs = p.c.d * elem / 16;
-  evict_select_kernel<<<dim3(p.c.h_kv, p.c.batch), kSelThreads, 0, st>>>(p);
-  cudaError_t e = cudaGetLastError();
+  // keys that can occur, up to what shared memory holds
+  const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
+  const int held = static_cast<int>(slots < kSelKeys ? slots : kSelKeys);
+  static SmemOptIn opt_in;
+  cudaError_t e = opt_in(reinterpret_cast<const void*>(evict_select_kernel), kSelKeys * 4);
   if (e != cudaSuccess) return e;
-  int64_t blocks = cdiv(static_cast<int64_t>(p.budget) * vecs, 256 * 4);
+  evict_select_kernel<<<dim3(p.c.h_kv, p.c.batch), kSelThreads, held * sizeof(uint32_t), st>>>(p, held);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int per = 256 / vecs * kCopySlots;
+  int64_t blocks = cdiv(p.budget, per);
   if (blocks > 1024) blocks = 1024;
   evict_copy_kernel<<<dim3(static_cast<unsigned>(blocks), p.c.h_kv, p.c.batch), 256, 0, st>>>(p, elem, vecs);
   return cudaGetLastError();

@@ -77,43 +77,54 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
-// The pages as a 4-D tensor of (d, slot and head by ascending stride, page),
-// boxes of 64 columns x one page (at most kt slots).  False: not such a tensor.
+// The pages as a 4-D tensor of (d, slot and head by ascending stride, page).
+// False: the strides are not such a tensor's.
+struct PageTensor {
+  int64_t s1, s2, sp, n1, n2;
+  int head_first;
+};
+inline bool page_tensor(const PagedCacheParams& c, int64_t sp, int64_t sn, int64_t sh, PageTensor* t) {
+  // strides of dimensions with one entry do not matter
+  if (c.h_kv == 1) sh = sn * c.page_size;
+  t->head_first = sh < sn;
+  t->s1 = t->head_first ? sh : sn;
+  t->s2 = t->head_first ? sn : sh;
+  t->n1 = t->head_first ? c.h_kv : c.page_size;
+  t->n2 = t->head_first ? c.page_size : c.h_kv;
+  t->sp = c.num_pages == 1 ? t->s2 * t->n2 : sp;
+  return t->s1 >= c.d && t->s2 >= t->s1 * t->n1 && t->sp >= t->s2 && t->sp * 2 < (1ll << 40);
+}
+
+// Its tensor map, boxes of 64 columns x one page (at most kt slots).
 inline bool page_map(const PagedCacheParams& c, const void* base, int64_t sp, int64_t sn, int64_t sh, ssa_dtype dt,
                      int kt, CUtensorMap* map, MapOrder* mo) {
   auto enc = tensor_map_encoder();
-  if (!enc) return false;
-  // strides of dimensions with one entry do not matter
-  if (c.h_kv == 1) sh = sn * c.page_size;
-  const bool head_first = sh < sn;
-  mo->head_first = head_first;
-  const int64_t s1 = head_first ? sh : sn, s2 = head_first ? sn : sh;
-  const cuuint64_t n1 = head_first ? c.h_kv : c.page_size, n2 = head_first ? c.page_size : c.h_kv;
-  if (s1 < c.d || s2 < s1 * static_cast<int64_t>(n1)) return false;
-  if (c.num_pages == 1) sp = s2 * static_cast<int64_t>(n2);
-  if (sp < s2 || sp * 2 >= (1ll << 40)) return false;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.d), n1, n2, static_cast<cuuint64_t>(c.num_pages)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(s1) * 2, static_cast<cuuint64_t>(s2) * 2,
-                                 static_cast<cuuint64_t>(sp) * 2};
+  PageTensor t;
+  if (!enc || !page_tensor(c, sp, sn, sh, &t)) return false;
+  mo->head_first = t.head_first;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.d), static_cast<cuuint64_t>(t.n1),
+                              static_cast<cuuint64_t>(t.n2), static_cast<cuuint64_t>(c.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(t.s1) * 2, static_cast<cuuint64_t>(t.s2) * 2,
+                                 static_cast<cuuint64_t>(t.sp) * 2};
   const cuuint32_t rows = c.page_size < kt ? c.page_size : kt;
-  const cuuint32_t box[4] = {64, head_first ? 1 : rows, head_first ? rows : 1, 1};
+  const cuuint32_t box[4] = {64, t.head_first ? 1 : rows, t.head_first ? rows : 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUtensorMapDataType t = dt == SSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return enc(map, t, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUtensorMapDataType type = dt == SSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(map, type, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // What the kernels on page tiles need of a cache: 16-bit rows of 64 or 128,
-// pages of a power of two of at least 8 slots, strides a tensor map takes.
+// pages of a power of two of at least 8 slots, strides a tensor map takes (K's
+// and V's in the same order).
 inline bool page_tiles_supported(const PagedAttnParams& p, ssa_dtype dt) {
   if (dt != SSA_BF16 && dt != SSA_F16) return false;
   if (p.c.d != 64 && p.c.d != 128) return false;
-  if (p.c.page_shift < 3 || p.c.num_pages < 1 || !(p.inv_scale > 0.f)) return false;
-  CUtensorMap m;
-  MapOrder a, b;
-  return page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, 64, &m, &a) &&
-         page_map(p.c, p.c.v, p.c.v_sp, p.c.v_sn, p.c.v_sh, dt, 64, &m, &b) && a.head_first == b.head_first;
+  if (p.c.page_shift < 3 || p.c.num_pages < 1 || !(p.inv_scale > 0.f) || !tensor_map_encoder()) return false;
+  PageTensor a, b;
+  return page_tensor(p.c, p.c.k_sp, p.c.k_sn, p.c.k_sh, &a) && page_tensor(p.c, p.c.v_sp, p.c.v_sn, p.c.v_sh, &b) &&
+         a.head_first == b.head_first;
 }
 
 }  // namespace ssa

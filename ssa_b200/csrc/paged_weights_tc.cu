@@ -364,8 +364,8 @@ cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, cudaStream_t st) {
   if (!page_map(p.c, p.c.k, p.c.k_sp, p.c.k_sn, p.c.k_sh, dt, kSlots, &km, &mo) || !query_map(p, dt, &qm, &qo))
     return cudaErrorInvalidValue;
   auto kern = weights_tc_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(Geo<D>::kSmem));
+  static SmemOptIn opt_in;
+  const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), Geo<D>::kSmem);
   if (e != cudaSuccess) return e;
   kern<<<148, kThreads, Geo<D>::kSmem, st>>>(km, qm, p, mo, qo);
   return cudaGetLastError();

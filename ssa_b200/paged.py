@@ -37,65 +37,77 @@ from .ops import _dtype_code, _last_contig, _require_cuda
 _APPEND, _ATTEND, _EVICT = range(3)
 
 
-def _index(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
+_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(i).cuda_stream, without the object
+_i32 = torch.int32
+
+
+def _index(t: torch.Tensor, name: str, dev, rows: int) -> torch.Tensor:
+    """An int32 vector of ``rows`` entries (any number: -1) on ``dev``."""
     if t.device != dev:
         raise RuntimeError(f"tensors on different devices: {dev} and {t.device} ({name})")
-    if t.dtype != torch.int32:
+    if t.dtype is not _i32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        want = ", ".join("*" if n is None else str(n) for n in shape)
-        raise ValueError(f"{name} must have shape [{want}], got {list(t.shape)}")
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    if t.dim() != 1 or (rows >= 0 and t.shape[0] != rows):
+        raise ValueError(f"{name} must have shape [{rows if rows >= 0 else '*'}], got {list(t.shape)}")
+    return t if t.stride(0) == 1 else t.contiguous()
+
+
+def _table(t: torch.Tensor, name: str, dev, rows: int) -> torch.Tensor:
+    """An int32 page table ``[rows, *]`` on ``dev``."""
+    if t.device != dev:
+        raise RuntimeError(f"tensors on different devices: {dev} and {t.device} ({name})")
+    if t.dtype is not _i32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise ValueError(f"{name} must have shape [{rows}, *], got {list(t.shape)}")
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
 def _cache_args(k_pages, v_pages, page_table, kv_lens, weights, op):
     """The filled :class:`SsaPagedCache` (with the op's error word) and the index
     tensors it points into."""
     dev = _require_cuda(k_pages, v_pages)
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must both be [num_pages, page_size, h_kv, d], got "
-                         f"{list(k_pages.shape)} and {list(v_pages.shape)}")
+                         f"{list(shape)} and {list(v_pages.shape)}")
     if k_pages.dtype != v_pages.dtype:
         raise TypeError(f"k_pages, v_pages dtypes differ: {k_pages.dtype}, {v_pages.dtype}")
+    kp, kn, kh, kd = k_pages.stride()
+    vp, vn, vh, vd = v_pages.stride()
     # the pages are written in place, so a copy would be of no use
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+    if kd != 1 or vd != 1:
         raise ValueError("the last dimension of k_pages and v_pages must be contiguous")
-    kv_lens = _index(kv_lens, "kv_lens", (None,), dev)
-    page_table = _index(page_table, "page_table", (kv_lens.shape[0], None), dev)
-    c = L.SsaPagedCache()
-    c.num_pages, c.page_size, c.h_kv, c.d = k_pages.shape
-    c.batch, c.max_pages = page_table.shape
-    c.dtype = _dtype_code(k_pages)
-    c.k_pages = k_pages.data_ptr()
-    c.k_stride_p, c.k_stride_n, c.k_stride_h, _ = k_pages.stride()
-    c.v_pages = v_pages.data_ptr()
-    c.v_stride_p, c.v_stride_n, c.v_stride_h, _ = v_pages.stride()
+    kv_lens = _index(kv_lens, "kv_lens", dev, -1)
+    batch = kv_lens.shape[0]
+    page_table = _table(page_table, "page_table", dev, batch)
+    w, wp, wn, wh = None, 0, 0, 0
     if weights is not None:
         if weights.device != dev:
             raise RuntimeError(f"tensors on different devices: {dev} and {weights.device} (weights)")
         if weights.dtype != torch.float32:
             raise TypeError(f"weights must be float32, got {weights.dtype}")
-        if weights.shape != k_pages.shape[:3]:
-            raise ValueError(f"weights must be [num_pages, page_size, h_kv] = {list(k_pages.shape[:3])}, got "
+        if weights.shape != shape[:3]:
+            raise ValueError(f"weights must be [num_pages, page_size, h_kv] = {list(shape[:3])}, got "
                              f"{list(weights.shape)}")
-        c.weights = weights.data_ptr()
-        c.w_stride_p, c.w_stride_n, c.w_stride_h = weights.stride()
-    c.page_table = page_table.data_ptr()
-    c.table_stride = page_table.stride(0)
-    c.kv_lens = kv_lens.data_ptr()
-    c.status = S.host_word(dev, op)
+        w, (wp, wn, wh) = weights.data_ptr(), weights.stride()
+    num_pages, page_size, h_kv, d = shape
+    c = L.SsaPagedCache(batch, page_table.shape[1], page_size, h_kv, d, _dtype_code(k_pages), num_pages,
+                        k_pages.data_ptr(), kp, kn, kh, v_pages.data_ptr(), vp, vn, vh, w, wp, wn, wh,
+                        page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), S.host_word(dev, op))
     return dev, c, (page_table, kv_lens)
 
 
 def _call(dev, fn, *args):
-    stream = torch.cuda.current_stream(dev).cuda_stream
     if torch.cuda.current_device() == dev.index:
-        code = fn(*args, stream)
+        code = fn(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            code = fn(*args, stream)
-    L.check(fn.__name__, code)
-    S.host_word_done(dev)
+            code = fn(*args, _raw_stream(dev.index))
+    if code:
+        L.check(fn.__name__, code)
+    if S.mode() == "sync":
+        S.host_word_done(dev)
 
 
 def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -114,20 +126,18 @@ def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
             those of the written slots become 0.
     """
     dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _APPEND)
-    _require_cuda(k_pages, k_new, v_new)
-    if k_new.shape != v_new.shape or k_new.dim() != 3 or k_new.shape[1:] != k_pages.shape[2:]:
-        raise ValueError(f"k_new and v_new must be [rows, {k_pages.shape[2]}, {k_pages.shape[3]}], got "
-                         f"{list(k_new.shape)} and {list(v_new.shape)}")
+    if k_new.device != dev or v_new.device != dev:
+        _require_cuda(k_pages, k_new, v_new)
+    shape = k_new.shape
+    if shape != v_new.shape or len(shape) != 3 or shape[1] != c.h_kv or shape[2] != c.d:
+        raise ValueError(f"k_new and v_new must be [rows, {c.h_kv}, {c.d}], got {list(shape)} and {list(v_new.shape)}")
     if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
         raise TypeError(f"k_new, v_new ({k_new.dtype}, {v_new.dtype}) must have the cache's dtype {k_pages.dtype}")
-    q_starts = _index(q_starts, "q_starts", (c.batch + 1,), dev)
+    q_starts = _index(q_starts, "q_starts", dev, c.batch + 1)
     k_new, v_new = _last_contig(k_new), _last_contig(v_new)
-    a = L.SsaPagedAppendArgs()
-    a.rows, a.q_starts = k_new.shape[0], q_starts.data_ptr()
-    a.k_new = k_new.data_ptr()
-    a.k_new_stride_n, a.k_new_stride_h, _ = k_new.stride()
-    a.v_new = v_new.data_ptr()
-    a.v_new_stride_n, a.v_new_stride_h, _ = v_new.stride()
+    kn, kh, _ = k_new.stride()
+    vn, vh, _ = v_new.stride()
+    a = L.SsaPagedAppendArgs(shape[0], q_starts.data_ptr(), k_new.data_ptr(), kn, kh, v_new.data_ptr(), vn, vh)
     _call(dev, L.lib().ssa_paged_append, ctypes.byref(c), ctypes.byref(a))
 
 
@@ -157,29 +167,27 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     written.
     """
     dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
-    _require_cuda(k_pages, q)
+    if q.device != dev:
+        _require_cuda(k_pages, q)
     if q.dim() != 3 or q.shape[2] != c.d:
         raise ValueError(f"q must be [rows, h_q, {c.d}], got {list(q.shape)}")
-    if q.shape[1] % c.h_kv:
+    rows, h_q, d = q.shape
+    if h_q % c.h_kv:
         raise ValueError("num_q_heads must be divisible by num_kv_heads")
     if q.dtype != k_pages.dtype:
         raise TypeError(f"q ({q.dtype}) must have the cache's dtype {k_pages.dtype}")
-    q_starts = _index(q_starts, "q_starts", (c.batch + 1,), dev)
+    q_starts = _index(q_starts, "q_starts", dev, c.batch + 1)
     q = _last_contig(q)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-    a = L.SsaPagedAttnArgs()
-    a.rows, a.q_starts, a.h_q, a.causal = q.shape[0], q_starts.data_ptr(), q.shape[1], 1 if is_causal else 0
-    a.scale = math.sqrt(c.d) if scale is None else float(scale)
-    a.q = q.data_ptr()
-    a.q_stride_n, a.q_stride_h, _ = q.stride()
-    a.out = out.data_ptr()
-    a.out_stride_n, a.out_stride_h, _ = out.stride()
-    if lse is not None:
-        a.lse = lse.data_ptr()
+    qn, qh, _ = q.stride()
+    out = q.new_empty((rows, h_q, d))
+    lse = q.new_empty((rows, h_q), dtype=torch.float32) if return_lse else None
+    a = L.SsaPagedAttnArgs(rows, q_starts.data_ptr(), h_q, 1 if is_causal else 0,
+                           math.sqrt(d) if scale is None else float(scale), q.data_ptr(), qn, qh, out.data_ptr(),
+                           h_q * d, d, lse.data_ptr() if return_lse else None)
     lib, rc, ra = L.lib(), ctypes.byref(c), ctypes.byref(a)
-    ws = torch.empty(max(int(lib.ssa_paged_attn_workspace_size(rc, ra)), 16), dtype=torch.uint8, device=dev)
-    _call(dev, lib.ssa_paged_attn, rc, ra, ws.data_ptr(), ws.numel())
+    nbytes = lib.ssa_paged_attn_workspace_size(rc, ra)
+    ws = q.new_empty((nbytes,), dtype=torch.uint8)
+    _call(dev, lib.ssa_paged_attn, rc, ra, ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -203,13 +211,11 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget {budget}, recent {recent}: need budget >= 1 and 0 <= recent <= budget")
-    new_table = _index(new_table, "new_table", (c.batch, None), dev)
+    new_table = _table(new_table, "new_table", dev, c.batch)
     kept = torch.empty((c.batch, c.h_kv, budget), dtype=torch.int32, device=dev)
     new_lens = torch.empty((c.batch,), dtype=torch.int32, device=dev)
-    a = L.SsaPagedEvictArgs()
-    a.budget, a.recent, a.new_max_pages = budget, recent, new_table.shape[1]
-    a.new_table, a.new_table_stride = new_table.data_ptr(), new_table.stride(0)
-    a.kept, a.new_lens = kept.data_ptr(), new_lens.data_ptr()
+    a = L.SsaPagedEvictArgs(budget, recent, new_table.shape[1], new_table.data_ptr(), new_table.stride(0),
+                            kept.data_ptr(), new_lens.data_ptr())
     _call(dev, L.lib().ssa_paged_evict, ctypes.byref(c), ctypes.byref(a))
     return kept, new_lens
 
