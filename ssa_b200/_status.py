@@ -42,7 +42,10 @@ _SLOTS = 256
 
 
 def mode() -> str:
-    v = os.environ.get("SSA_CHECKED", "1").strip().lower()
+    v = os.environ.get("SSA_CHECKED")
+    if v is None:
+        return "lazy"
+    v = v.strip().lower()
     if v in ("0", "off", "false", "no"):
         return "off"
     if v == "sync":
@@ -110,12 +113,13 @@ def _device_index(dev: torch.device) -> int:
     return dev.index if dev.index is not None else torch.cuda.current_device()
 
 
-def host_word(dev: torch.device, op: int) -> Optional[int]:
+def host_word(dev: torch.device, op: int):
     """Address of the error word of op number ``op`` (in ``_HostWords.OPS``), or
-    None with ``SSA_CHECKED=0``; raises for an error already found.  To be
-    followed by :func:`host_word_done` where :func:`mode` is ``sync``."""
-    if mode() == "off":
-        return None
+    None with ``SSA_CHECKED=0``, and whether :func:`host_word_done` is to follow
+    the launch; raises for an error already found."""
+    m = mode()
+    if m == "off":
+        return None, False
     key = _device_index(dev)
     w = _words.get(key)
     if w is None:
@@ -124,7 +128,7 @@ def host_word(dev: torch.device, op: int) -> Optional[int]:
     elif w.view[0] or w.view[1] or w.view[2]:
         _poll_words(dev)
     w.used = True
-    return w.base + 4 * op
+    return w.base + 4 * op, m == "sync"
 
 
 def host_word_done(dev: torch.device) -> None:

@@ -230,11 +230,10 @@ struct PagedWalk {
   int seq, head, tile, n, len, units;   // units: of the current item
 };
 
-// Total units, and the walk of CTA `cta` of `grid` (CTAs of less than
-// `min_units` each are not made: the rest stay idle).  Called by one full
-// warp; every lane gets the result.  False: no work.
-__device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int extra, int min_units, int64_t cta,
-                                      int64_t grid, PagedWalk& w) {
+// Total units, and the walk of CTA `cta` of `grid`.  Called by one full warp;
+// every lane gets the result.  False: no work.
+__device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int extra, int64_t cta, int64_t grid,
+                                      PagedWalk& w) {
   const int lane = threadIdx.x & 31;
   const int hk = p.c.h_kv;
   // the first 32 sequences stay in registers for the second look
@@ -253,7 +252,7 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
   int64_t total = mine;
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  int64_t ctas = total >= grid * min_units ? grid : mul_div(total + min_units - 1, 1, min_units);
+  const int64_t ctas = total < grid ? total : grid;
   w.total = total;
   w.ctas = ctas;
   if (cta >= ctas) return false;
@@ -321,6 +320,23 @@ __device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt,
   w.units = t.units(w.tile);
 }
 
+// The same for a whole CTA: warp 0 works it out, the others read it (after a
+// __syncthreads that the caller makes in any case).
+struct PagedStart {
+  PagedWalk w;
+  int any;
+};
+__device__ inline void paged_start(const PagedAttnParams& p, int tt, int kt, int extra, PagedStart* shared) {
+  if (threadIdx.x < 32) {
+    PagedWalk w{};
+    const bool any = paged_schedule(p, tt, kt, extra, blockIdx.x, gridDim.x, w);
+    if (threadIdx.x == 0) {
+      shared->w = w;
+      shared->any = any;
+    }
+  }
+}
+
 // The CTA that holds unit u: the last c with floor(c W / G) <= u.
 __device__ __forceinline__ int unit_cta(const PagedWalk& w, int64_t u) {
   const int64_t x = (u + 1) * w.ctas - 1;
@@ -373,6 +389,25 @@ class SmemOptIn {
  private:
   std::atomic<uint64_t> done_{0};
 };
+
+// Launch of a kernel that follows another of the same op: its CTAs may be set
+// up while the other drains, and wait (paged_after) before they read its results.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_after(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+// Everything the kernel launched before has written is visible after this.
+__device__ __forceinline__ void paged_after() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, ssa_dtype dt, cudaStream_t st);
 cudaError_t launch_paged_evict(const PagedEvictParams& p, ssa_dtype dt, cudaStream_t st);

@@ -156,9 +156,11 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
   int64_t* voff = koff + kKT;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int tt = tile_tokens(R, p.group), d = p.c.d;
-  PagedWalk w;
-  const bool any = paged_schedule(p, tt, kKT, kExtra, 1, blockIdx.x, gridDim.x, w);
-  if (!any) {
+  __shared__ PagedStart start;
+  paged_start(p, tt, kKT, kExtra, &start);
+  __syncthreads();
+  PagedWalk w = start.w;
+  if (!start.any) {
     if (tid == 0) p.split[blockIdx.x].valid = 0;
     return;
   }
@@ -312,6 +314,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) combine_kernel(PagedAttnParams p, int R) {
+  paged_after();
   const int b = blockIdx.x + 1;
   const PagedSplit it = p.split[b];
   const int64_t before = p.split[b - 1].item_first;
@@ -376,6 +379,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedAttnParams p, int R) 
 // ---------------------------------------------------------------------------
 template <typename T, int R, int DP>
 __global__ void __launch_bounds__(kThreads) weights_simt_kernel(PagedAttnParams p) {
+  paged_after();
   using G = SimtGeo<R, DP>;
   constexpr int RI = R / 16;
   extern __shared__ __align__(16) float smem[];
@@ -445,8 +449,7 @@ cudaError_t launch_simt(const PagedAttnParams& p, int grid, bool weights, cudaSt
   if (e != cudaSuccess) return e;
   const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
   if (slots == 0) return cudaSuccess;
-  kern<<<dim3(static_cast<unsigned>(cdiv(slots, kKT)), p.c.h_kv, p.c.batch), kThreads, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_after(kern, dim3(static_cast<unsigned>(cdiv(slots, kKT)), p.c.h_kv, p.c.batch), dim3(kThreads), smem, st, p);
 }
 
 template <typename T, int R>
@@ -513,11 +516,10 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
   // one wave of blocks: two warps' rows each for few rows, four for many
   const dim3 grid(a.grid - 1, a.rows == 256 ? 8 : a.rows / 8);
   switch (dt) {
-    case SSA_F32: combine_kernel<float><<<grid, 256, 0, st>>>(p, a.rows); break;
-    case SSA_BF16: combine_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, a.rows); break;
-    default: combine_kernel<__half><<<grid, 256, 0, st>>>(p, a.rows); break;
+    case SSA_F32: e = launch_after(combine_kernel<float>, grid, dim3(256), 0, st, p, a.rows); break;
+    case SSA_BF16: e = launch_after(combine_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, a.rows); break;
+    default: e = launch_after(combine_kernel<__half>, grid, dim3(256), 0, st, p, a.rows); break;
   }
-  e = cudaGetLastError();
   if (e != cudaSuccess || !p.c.w) return e;
   if (p.scores) return launch_paged_weights_dec(p, st);
   if (a.kernel == AttnKernel::kChunks && paged_weights_tc_supported(p, dt)) return launch_paged_weights_tc(p, dt, st);

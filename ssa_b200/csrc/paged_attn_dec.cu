@@ -45,7 +45,7 @@ struct Geo {
   static constexpr int kStages = D == 128 ? 6 : 12;
   static constexpr int kJoinRow = D + 4;                            // floats
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * 2 * kTileBytes +
-                                  kWarps * kRows * kJoinRow * 4 + 16 * kStages + 64;
+                                  kWarps * kRows * kJoinRow * 4 + 16 * kStages + 16 + sizeof(PagedStart);
 };
 
 template <typename T, int D>
@@ -73,11 +73,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  PagedWalk w;
-  const bool any = paged_schedule(p, tt, kKT, kExtra, 1, blockIdx.x, gridDim.x, w);
-  if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
+  PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 2 * G::kStages + 1);
+  paged_start(p, tt, kKT, kExtra, &start);
   __syncthreads();
-  if (!any) return;
+  PagedWalk w = start.w;
+  if (threadIdx.x == 0) p.split[blockIdx.x] = start.any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
+  if (!start.any) return;
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (!mbar_wait_or(bar, parity, abort_flag) && !*abort_flag) {
       *abort_flag = 1;
@@ -359,6 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
 // rows that see j of exp2(s_ij - lse2_i).  A thread takes four slots of one KV
 // head; the additions of a slot are in row order.
 __global__ void __launch_bounds__(256) weights_dec_kernel(PagedAttnParams p) {
+  paged_after();
   const int seq = blockIdx.z, head = blockIdx.y;
   const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, seq);
   const int j0 = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -417,8 +419,8 @@ cudaError_t launch_paged_attn_dec(const PagedAttnParams& p, ssa_dtype dt, int gr
 cudaError_t launch_paged_weights_dec(const PagedAttnParams& p, cudaStream_t st) {
   const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
   if (slots == 0) return cudaSuccess;
-  pdec::weights_dec_kernel<<<dim3(static_cast<unsigned>(cdiv(slots, 1024)), p.c.h_kv, p.c.batch), 256, 0, st>>>(p);
-  return cudaGetLastError();
+  return launch_after(pdec::weights_dec_kernel, dim3(static_cast<unsigned>(cdiv(slots, 1024)), p.c.h_kv, p.c.batch),
+                      dim3(256), 0, st, p);
 }
 
 }  // namespace ssa

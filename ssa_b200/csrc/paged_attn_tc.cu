@@ -176,12 +176,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  PagedWalk w;
-  const bool any = paged_schedule(p, tt, kKT, kExtra, 1, blockIdx.x, gridDim.x, w);
+  PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 2 * G::kStages + 16);
+  paged_start(p, tt, kKT, kExtra, &start);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
+  PagedWalk w = start.w;
+  const bool any = start.any;
   if (threadIdx.x == 0) p.split[blockIdx.x] = any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
   auto fail = [&]() {
     *abort_flag = 1;

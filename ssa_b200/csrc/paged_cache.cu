@@ -57,12 +57,13 @@ __device__ __forceinline__ uint32_t weight_key(float w) { return float_key(w != 
 
 constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
 constexpr int kSelBins = 2048;
+constexpr int kSelLoads = 16;      // weights in flight a thread
 constexpr int kSelKeys = 49152;    // keys held in shared memory (192 KB); longer sequences are read again
 
 // One CTA per (sequence, KV head).  The n_keep heaviest of the first `older`
 // slots are those whose key exceeds the n_keep-th largest, T, and the first
-// few that equal it.  The weights are read once into shared memory, eight
-// loads in flight a thread; T is found from its top bits down in three passes
+// few that equal it.  The weights are read once into shared memory,
+// sixteen loads in flight a thread; T is found from its top bits down in three passes
 // of 11, 11 and 10 bits, each counting the next digit of the keys that agree
 // with T so far and finding the digit by a sum from the top over the 2048
 // counts; then every warp counts and writes the kept slots of its own run of
@@ -90,37 +91,46 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(PagedEvictPar
     return pg < 0 ? 0u : weight_key(c.w[pg * c.w_sp + row * c.w_sn + h * c.w_sh]);
   };
   const bool hold = older <= held;
-  if (hold) {
-    for (int j0 = tid; j0 < older; j0 += 8 * kSelThreads) {
-      uint32_t k[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) k[e] = j0 + e * kSelThreads < older ? read_key(j0 + e * kSelThreads) : 0u;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (j0 + e * kSelThreads < older) sel_keys[j0 + e * kSelThreads] = k[e];
-    }
-  }
-  __syncthreads();
-  auto key_of = [&](int j) -> uint32_t { return hold ? sel_keys[j] : read_key(j); };
   uint32_t prefix = 0, known = 0;          // the bits of T found so far, and which
   int left = n_keep;                       // of the keys that agree with them, how many are kept
-  for (int pass = 0; pass < 3 && n_keep > 0; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
-    __syncthreads();
-    for (int j = tid; j - lane < older; j += kSelThreads) {
-      const uint32_t k = j < older ? key_of(j) : 0u;
-      const bool in = j < older && (k & known) == prefix;
-      const int bin = in ? static_cast<int>((k >> shift) & (bins - 1)) : -1;
-      // equal weights (a cache's first steps) would queue 32 deep on one counter
+  // counts a digit of each lane's key (bin -1: none).  Equal weights (a cache's
+  // first steps) would queue 32 deep on one counter.
+  auto count = [&](int bin) {
+    if (__all_sync(0xffffffffu, bin >= 0)) {
       int same;
       __match_all_sync(0xffffffffu, bin, &same);
       if (same) {
-        if (lane == 0 && bin >= 0) atomicAdd(&hist[bin], 32);
-      } else if (in) {
-        atomicAdd(&hist[bin], 1);
+        if (lane == 0) atomicAdd(&hist[bin], 32);
+        return;
       }
     }
+    if (bin >= 0) atomicAdd(&hist[bin], 1);
+  };
+  auto key_of = [&](int j) -> uint32_t { return hold ? sel_keys[j] : read_key(j); };
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
+    __syncthreads();
+    if (pass == 0) {
+      for (int j0 = tid; j0 - lane < older; j0 += kSelLoads * kSelThreads) {
+        uint32_t k[kSelLoads];
+#pragma unroll
+        for (int e = 0; e < kSelLoads; ++e) k[e] = j0 + e * kSelThreads < older ? read_key(j0 + e * kSelThreads) : 0u;
+#pragma unroll
+        for (int e = 0; e < kSelLoads; ++e) {
+          const int j = j0 + e * kSelThreads;
+          if (j < older && hold) sel_keys[j] = k[e];
+          if (j - lane < older) count(j < older ? static_cast<int>(k[e] >> 21) : -1);
+        }
+      }
+    } else {
+      for (int j = tid; j - lane < older; j += kSelThreads) {
+        const uint32_t k = j < older ? key_of(j) : 0u;
+        const bool in = j < older && (k & known) == prefix;
+        if (__any_sync(0xffffffffu, in)) count(in ? static_cast<int>((k >> shift) & (bins - 1)) : -1);
+      }
+    }
+    if (n_keep == 0) break;
     __syncthreads();
     // the largest digit b with (keys of digits >= b) >= left: a thread has two
     // digits, from the top
@@ -145,6 +155,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(PagedEvictPar
     known |= static_cast<uint32_t>(bins - 1) << shift;
     left = found[1];
   }
+  __syncthreads();
   if (n_keep == 0) prefix = 0xffffffffu;   // no key exceeds it, and none that equals it is kept
   // each warp's run of slots: kept if above T, if among the first `left` equal to T, or recent
   const int run = ((len + kSelWarps - 1) / kSelWarps + 31) / 32 * 32, lo = warp * run, hi = min(lo + run, len);
@@ -192,10 +203,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(PagedEvictPar
 }
 
 // Kept slots' keys, values and weights to the new pages.  A thread moves one
-// 16-byte piece of K and of V of four slots, all of their loads in flight
-// together (the slot, its page and the data are three loads in a row).
-constexpr int kCopySlots = 4;
+// 16-byte piece of K and of V of two slots, their loads in flight together
+// (the slot, its page and the data are three loads in a row; four slots a
+// thread cost more in resident threads than they gained).
+constexpr int kCopySlots = 2;
 __global__ void __launch_bounds__(256) evict_copy_kernel(PagedEvictParams p, int elem, int vecs) {
+  paged_after();                           // the kept slots
   const PagedCacheParams& c = p.c;
   const int s = blockIdx.z, h = blockIdx.y;
   const int size = min(max(paged_len(c, s), 0), p.budget);
@@ -271,8 +284,8 @@ cudaError_t launch_paged_evict(const PagedEvictParams& p, ssa_dtype dt, cudaStre
   const int per = 256 / vecs * kCopySlots;
   int64_t blocks = cdiv(p.budget, per);
   if (blocks > 1024) blocks = 1024;
-  evict_copy_kernel<<<dim3(static_cast<unsigned>(blocks), p.c.h_kv, p.c.batch), 256, 0, st>>>(p, elem, vecs);
-  return cudaGetLastError();
+  return launch_after(evict_copy_kernel, dim3(static_cast<unsigned>(blocks), p.c.h_kv, p.c.batch), dim3(256), 0, st, p,
+                      elem, vecs);
 }
 
 }  // namespace ssa

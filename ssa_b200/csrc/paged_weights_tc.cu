@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   fence_before();
   __syncthreads();
   fence_after();
+  paged_after();                                         // lse2
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (!mbar_wait_or(bar, parity, abort_flag) && !*abort_flag) {
@@ -367,8 +368,7 @@ cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, cudaStream_t st) {
   static SmemOptIn opt_in;
   const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), Geo<D>::kSmem);
   if (e != cudaSuccess) return e;
-  kern<<<148, kThreads, Geo<D>::kSmem, st>>>(km, qm, p, mo, qo);
-  return cudaGetLastError();
+  return launch_after(kern, dim3(148), dim3(kThreads), Geo<D>::kSmem, st, km, qm, p, mo, qo);
 }
 
 }  // namespace pwt

@@ -64,8 +64,8 @@ def _table(t: torch.Tensor, name: str, dev, rows: int) -> torch.Tensor:
 
 
 def _cache_args(k_pages, v_pages, page_table, kv_lens, weights, op):
-    """The filled :class:`SsaPagedCache` (with the op's error word) and the index
-    tensors it points into."""
+    """The device, the filled :class:`SsaPagedCache` (with the op's error word),
+    whether to wait for errors, and the index tensors the struct points into."""
     dev = _require_cuda(k_pages, v_pages)
     shape = k_pages.shape
     if len(shape) != 4 or shape != v_pages.shape:
@@ -92,13 +92,14 @@ def _cache_args(k_pages, v_pages, page_table, kv_lens, weights, op):
                              f"{list(weights.shape)}")
         w, (wp, wn, wh) = weights.data_ptr(), weights.stride()
     num_pages, page_size, h_kv, d = shape
+    word, sync = S.host_word(dev, op)
     c = L.SsaPagedCache(batch, page_table.shape[1], page_size, h_kv, d, _dtype_code(k_pages), num_pages,
                         k_pages.data_ptr(), kp, kn, kh, v_pages.data_ptr(), vp, vn, vh, w, wp, wn, wh,
-                        page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), S.host_word(dev, op))
-    return dev, c, (page_table, kv_lens)
+                        page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), word)
+    return dev, c, sync, (page_table, kv_lens)
 
 
-def _call(dev, fn, *args):
+def _call(dev, sync, fn, *args):
     if torch.cuda.current_device() == dev.index:
         code = fn(*args, _raw_stream(dev.index))
     else:
@@ -106,7 +107,7 @@ def _call(dev, fn, *args):
             code = fn(*args, _raw_stream(dev.index))
     if code:
         L.check(fn.__name__, code)
-    if S.mode() == "sync":
+    if sync:
         S.host_word_done(dev)
 
 
@@ -125,7 +126,7 @@ def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
         weights: optional ``[num_pages, page_size, h_kv]`` float32 slot weights;
             those of the written slots become 0.
     """
-    dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _APPEND)
+    dev, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _APPEND)
     if k_new.device != dev or v_new.device != dev:
         _require_cuda(k_pages, k_new, v_new)
     shape = k_new.shape
@@ -138,7 +139,7 @@ def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
     kn, kh, _ = k_new.stride()
     vn, vh, _ = v_new.stride()
     a = L.SsaPagedAppendArgs(shape[0], q_starts.data_ptr(), k_new.data_ptr(), kn, kh, v_new.data_ptr(), vn, vh)
-    _call(dev, L.lib().ssa_paged_append, ctypes.byref(c), ctypes.byref(a))
+    _call(dev, sync, L.lib().ssa_paged_append, ctypes.byref(c), ctypes.byref(a))
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -166,7 +167,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     sees no slot gets zeros (and ``-inf``).  Rows outside ``q_starts`` are not
     written.
     """
-    dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
+    dev, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
     if q.device != dev:
         _require_cuda(k_pages, q)
     if q.dim() != 3 or q.shape[2] != c.d:
@@ -187,7 +188,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lib, rc, ra = L.lib(), ctypes.byref(c), ctypes.byref(a)
     nbytes = lib.ssa_paged_attn_workspace_size(rc, ra)
     ws = q.new_empty((nbytes,), dtype=torch.uint8)
-    _call(dev, lib.ssa_paged_attn, rc, ra, ws.data_ptr(), nbytes)
+    _call(dev, sync, lib.ssa_paged_attn, rc, ra, ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -207,7 +208,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     """
     if weights is None:
         raise ValueError("weights is needed: eviction ranks slots by them")
-    dev, c, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
+    dev, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget {budget}, recent {recent}: need budget >= 1 and 0 <= recent <= budget")
@@ -216,7 +217,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     new_lens = torch.empty((c.batch,), dtype=torch.int32, device=dev)
     a = L.SsaPagedEvictArgs(budget, recent, new_table.shape[1], new_table.data_ptr(), new_table.stride(0),
                             kept.data_ptr(), new_lens.data_ptr())
-    _call(dev, L.lib().ssa_paged_evict, ctypes.byref(c), ctypes.byref(a))
+    _call(dev, sync, L.lib().ssa_paged_evict, ctypes.byref(c), ctypes.byref(a))
     return kept, new_lens
 
 
