@@ -3,12 +3,14 @@
 //
 // Bound by reading K and V once.  An item is 16 rows (the g heads of a KV
 // group at floor(16 / g) tokens); its key tiles of 64 slots come by TMA into
-// a deep ring (a producer warp, one lane per page box), which a CTA on every
-// SM keeps in flight across the items it walks.  Each of four warps takes 16
-// slots of every tile with its own running maximum, sum and output (mma.sync
-// m16n8k16, Q as A in registers, K and V by ldmatrix), so the warps meet only
-// where an item ends.  mma.sync suffices: 16 x 64 x d products a tile are a few
-// hundred clocks against about 1400 to fetch its 32 KB at d = 128.
+// a ring (a producer warp, one lane per page box), which a CTA on every SM
+// keeps in flight across the items it walks.  Two groups of four warps take the
+// tiles in turn, a warp 16 slots of each, with its own running maximum, sum and
+// output (mma.sync m16n8k16, Q as A in registers, K and V by ldmatrix), so the
+// warps meet only where an item ends.  mma.sync suffices: 16 x 64 x d products
+// a tile are a few hundred clocks against about 1400 to fetch its 32 KB at
+// d = 128.  (One group of four warps was 8% slower, bound by its own steps; a
+// ring of 96 KB is as fast as one of 192 KB.)
 //
 // P enters the product with V as two 16-bit terms (p = hi + lo, off by 2^-17),
 // sums and outputs are fp32.  Slots hidden from a row have p = 0; where the
@@ -33,8 +35,8 @@ using namespace tc;
 
 constexpr int kRows = 16;
 constexpr int kKT = 64;
-constexpr int kExtra = 2;          // units an item costs besides its tiles
-constexpr int kWarps = 4;          // consumers, 16 slots of a tile each
+constexpr int kExtra = 4;          // units an item costs besides its tiles
+constexpr int kWarps = 8;          // consumers: two groups of four, 16 slots of a tile each
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -42,7 +44,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 template <int D>
 struct Geo {
   static constexpr int kTileBytes = kKT * D * 2;                    // of K, and of V
-  static constexpr int kStages = D == 128 ? 6 : 12;
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  // a stage always serves the same group: its warps then see every phase of
+  // the stage's barrier, and a wait by parity means the phase it should
+  static_assert(kStages % 2 == 0, "stages alternate between the two groups");
   static constexpr int kJoinRow = D + 4;                            // floats
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * 2 * kTileBytes +
                                   kWarps * kRows * kJoinRow * 4 + 16 * kStages + 16 + sizeof(PagedStart);
@@ -66,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) {
       mbar_init(full + 8 * s, 1);
-      mbar_init(empty + 8 * s, kWarps);
+      mbar_init(empty + 8 * s, kWarps / 2);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -163,8 +168,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[t][e] = 0.f;
     for (int t = seg.first; t < seg.last; ++t, ++g) {
+      if ((g & 1) != (warp >> 2)) continue;
       const int st = static_cast<int>(g % G::kStages);
-      const int k0 = t * kKT + warp * 16;
+      const int k0 = t * kKT + (warp & 3) * 16;
       wait(full + 8 * st, static_cast<uint32_t>((g / G::kStages) & 1));
       __syncwarp();
       const uint32_t kb = ring + 2 * st * G::kTileBytes, vb = kb + G::kTileBytes;
@@ -174,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[t][e] = 0.f;
       {
-        const int key = warp * 16 + kk;
+        const int key = (warp & 3) * 16 + kk;
         const uint32_t row = kb + key * 128;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -233,17 +239,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
           split2<T>(s[t][2 * i], s[t][2 * i + 1], hi[2 * t + i], lo[2 * t + i]);
         }
       }
-      const int key = warp * 16 + vk;
+      const int key = (warp & 3) * 16 + vk;
       const uint32_t row = vb + key * 128;
-      uint32_t v[NT / 2][4];
+      auto v_at = [&](int t) { return row + (t / 4) * (kKT * 128) + ((((t % 4) * 2 + vp) ^ (key & 7)) << 4); };
       uint32_t odd = 0;
+      if (masked) {
 #pragma unroll
-      for (int t = 0; t < NT / 2; ++t) {
-        ldsm_x4_t(row + (t / 4) * (kKT * 128) + ((((t % 4) * 2 + vp) ^ (key & 7)) << 4), v[t][0], v[t][1], v[t][2],
-                  v[t][3]);
-        if (masked) odd |= odd_bits<T>(v[t][0]) | odd_bits<T>(v[t][1]) | odd_bits<T>(v[t][2]) | odd_bits<T>(v[t][3]);
+        for (int t = 0; t < NT / 2; ++t) {
+          uint32_t v[4];
+          ldsm_x4_t(v_at(t), v[0], v[1], v[2], v[3]);
+          odd |= odd_bits<T>(v[0]) | odd_bits<T>(v[1]) | odd_bits<T>(v[2]) | odd_bits<T>(v[3]);
+        }
       }
-      if (masked && __any_sync(0xffffffffu, odd != 0)) {
+      if (__any_sync(0xffffffffu, odd != 0)) {
         for (int j = 0; j < 16; ++j) {
           // p of rows gr, gr + 8 at slot j: fragment t = j / 8, lane column (j % 8) / 2
           const int src = (lane & 28) + ((j & 7) >> 1);
@@ -254,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
             const float y0 = __shfl_sync(0xffffffffu, s[1][2 * i], src), y1 = __shfl_sync(0xffffffffu, s[1][2 * i + 1], src);
             pj[i] = j < 8 ? ((j & 1) ? x1 : x0) : ((j & 1) ? y1 : y0);
           }
-          const int slot_row = warp * 16 + j;
+          const int slot_row = (warp & 3) * 16 + j;
           const unsigned char* vr = base + (2 * st + 1) * G::kTileBytes + slot_row * 128;
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -272,16 +280,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
       } else {
 #pragma unroll
         for (int t = 0; t < NT / 2; ++t) {
-          mma16816<T>(o[2 * t], hi, v[t][0], v[t][1]);
-          mma16816<T>(o[2 * t + 1], hi, v[t][2], v[t][3]);
-          mma16816<T>(o[2 * t], lo, v[t][0], v[t][1]);
-          mma16816<T>(o[2 * t + 1], lo, v[t][2], v[t][3]);
+          uint32_t v[4];
+          ldsm_x4_t(v_at(t), v[0], v[1], v[2], v[3]);
+          mma16816<T>(o[2 * t], hi, v[0], v[1]);
+          mma16816<T>(o[2 * t + 1], hi, v[2], v[3]);
+          mma16816<T>(o[2 * t], lo, v[0], v[1]);
+          mma16816<T>(o[2 * t + 1], lo, v[2], v[3]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + 8 * st);
     }
-    // ---- join the four warps ----
+    // ---- join the warps ----
     float* mine = join + warp * kRows * G::kJoinRow;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -296,8 +306,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
         dst[D + 1] = l[i];
       }
     }
-    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
-    const int r = threadIdx.x >> 3, x0 = (threadIdx.x & 7) * (D / 8);
+    asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+    const int r = threadIdx.x >> 4, x0 = (threadIdx.x & 15) * (D / 16);
     if (r < rows) {
       float mx = -INFINITY;
 #pragma unroll
@@ -316,31 +326,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
       T* out = static_cast<T*>(p.out) + (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh + x0;
       float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + r) * (D + 4);
 #pragma unroll
-      for (int x = 0; x < D / 8; x += 8) {
-        float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < D / 16; x += 4) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int y = 0; y < kWarps; ++y) {
-          const float4* src = reinterpret_cast<const float4*>(join + (y * kRows + r) * G::kJoinRow + x0 + x);
-          const float4 u = src[0], z = src[1];
-          a[0] = fmaf(fy[y], u.x, a[0]); a[1] = fmaf(fy[y], u.y, a[1]);
-          a[2] = fmaf(fy[y], u.z, a[2]); a[3] = fmaf(fy[y], u.w, a[3]);
-          a[4] = fmaf(fy[y], z.x, a[4]); a[5] = fmaf(fy[y], z.y, a[5]);
-          a[6] = fmaf(fy[y], z.z, a[6]); a[7] = fmaf(fy[y], z.w, a[7]);
+          const float4 u = *reinterpret_cast<const float4*>(join + (y * kRows + r) * G::kJoinRow + x0 + x);
+          a.x = fmaf(fy[y], u.x, a.x);
+          a.y = fmaf(fy[y], u.y, a.y);
+          a.z = fmaf(fy[y], u.z, a.z);
+          a.w = fmaf(fy[y], u.w, a.w);
         }
         if (whole) {
-          uint4 pk;
-          pk.x = pack2<T>(a[0] * inv, a[1] * inv);
-          pk.y = pack2<T>(a[2] * inv, a[3] * inv);
-          pk.z = pack2<T>(a[4] * inv, a[5] * inv);
-          pk.w = pack2<T>(a[6] * inv, a[7] * inv);
-          *reinterpret_cast<uint4*>(out + x) = pk;
+          uint2 pk;
+          pk.x = pack2<T>(a.x * inv, a.y * inv);
+          pk.y = pack2<T>(a.z * inv, a.w * inv);
+          *reinterpret_cast<uint2*>(out + x) = pk;
         } else {
-#pragma unroll
-          for (int e = 0; e < 8; e += 4)
-            *reinterpret_cast<float4*>(part + x0 + x + e) = make_float4(a[e], a[e + 1], a[e + 2], a[e + 3]);
+          *reinterpret_cast<float4*>(part + x0 + x) = a;
         }
       }
-      if ((threadIdx.x & 7) == 0) {
+      if ((threadIdx.x & 15) == 0) {
         if (whole) {
           const int64_t at = (w.q0 + tok) * (static_cast<int64_t>(p.c.h_kv) * p.group) + head;
           const float z = sum == 0.f ? -INFINITY : mx + log2f(sum);
@@ -352,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
         }
       }
     }
-    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");   // before the next item's partials overwrite these
+    asm volatile("barrier.cta.sync 1, 256;" ::: "memory");   // before the next item's partials overwrite these
   }
 }
 
