@@ -83,7 +83,7 @@ def poll(dev: torch.device) -> None:
     """Raise for the first finished op whose status word came back non-zero
     (does not wait for the GPU)."""
     if _words:
-        _poll_words(dev)
+        _poll_words(dev.index if dev.index is not None else torch.cuda.current_device())
     if not _rings:
         return
     with _lock:
@@ -95,51 +95,49 @@ def poll(dev: torch.device) -> None:
 
 
 class _HostWords:
-    """One word of mapped pinned memory per paged-cache op of one device."""
+    """A word of mapped pinned memory per paged-cache op of one device."""
 
     OPS = ("paged_append", "paged_attention", "paged_evict")
 
     def __init__(self):
-        self.host = torch.zeros(len(self.OPS), dtype=torch.int32).pin_memory()
-        self.base = self.host.data_ptr()
-        self.view = (ctypes.c_int32 * len(self.OPS)).from_address(self.base)
+        self.host = torch.zeros(4, dtype=torch.int32).pin_memory()
+        base = self.host.data_ptr()
+        self.view = (ctypes.c_int32 * 4).from_address(base)
+        self.low, self.high = (ctypes.c_int64.from_address(base + 8 * i) for i in range(2))   # all four, in two reads
+        self.address = [base + 4 * op for op in range(len(self.OPS))]
         self.used = False
 
 
 _words = {}
 
 
-def _device_index(dev: torch.device) -> int:
-    return dev.index if dev.index is not None else torch.cuda.current_device()
-
-
-def host_word(dev: torch.device, op: int):
-    """Address of the error word of op number ``op`` (in ``_HostWords.OPS``), or
-    None with ``SSA_CHECKED=0``, and whether :func:`host_word_done` is to follow
-    the launch; raises for an error already found."""
+def host_word(key: int, op: int):
+    """Address of the error word of op number ``op`` (in ``_HostWords.OPS``) on
+    device number ``key``, or None with ``SSA_CHECKED=0``, and whether
+    :func:`host_word_done` is to follow the launch; raises for an error already
+    found."""
     m = mode()
     if m == "off":
         return None, False
-    key = _device_index(dev)
     w = _words.get(key)
     if w is None:
         with _lock:
             w = _words.setdefault(key, _HostWords())
-    elif w.view[0] or w.view[1] or w.view[2]:
-        _poll_words(dev)
+    elif w.low.value or w.high.value:
+        _poll_words(key)
     w.used = True
-    return w.base + 4 * op, m == "sync"
+    return w.address[op], m == "sync"
 
 
 def host_word_done(dev: torch.device) -> None:
     """After the launch, with ``SSA_CHECKED=sync``: wait for it and raise now."""
     if not torch.cuda.is_current_stream_capturing():
         torch.cuda.current_stream(dev).synchronize()
-        _poll_words(dev)
+        _poll_words(dev.index)
 
 
-def _poll_words(dev: torch.device) -> None:
-    w = _words.get(_device_index(dev))
+def _poll_words(key: int) -> None:
+    w = _words.get(key)
     if w is None:
         return
     for i, op in enumerate(w.OPS):
@@ -204,11 +202,14 @@ def release(slot: Optional[Slot], op: str, decode: Callable[[str, int], Optional
 def check_errors(device=None) -> None:
     """Wait for every op launched so far on ``device`` (default: all devices
     with pending words) and raise for the first error a kernel reported."""
+    only = None if device is None else torch.device(device).index
+    if device is not None and only is None:
+        only = torch.cuda.current_device()
     for key, w in list(_words.items()):
-        if w.used and (device is None or key == _device_index(torch.device(device))):
+        if w.used and (only is None or key == only):
             torch.cuda.synchronize(key)
             w.used = False
-            _poll_words(torch.device("cuda", key))
+            _poll_words(key)
     with _lock:
         rings = list(_rings.values()) if device is None else [_ring(torch.device(device))]
         first = None

@@ -24,7 +24,6 @@ are found on the device and raised by a later op call or by
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import List, Optional, Sequence, Tuple, Union
 
@@ -38,77 +37,107 @@ _APPEND, _ATTEND, _EVICT = range(3)
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(i).cuda_stream, without the object
-_i32 = torch.int32
+_i32, _f32 = torch.int32, torch.float32
 
 
-def _index(t: torch.Tensor, name: str, dev, rows: int) -> torch.Tensor:
-    """An int32 vector of ``rows`` entries (any number: -1) on ``dev``."""
-    if t.device != dev:
-        raise RuntimeError(f"tensors on different devices: {dev} and {t.device} ({name})")
+def _index(t: torch.Tensor, name: str, key: int, rows: int) -> torch.Tensor:
+    """An int32 vector of ``rows`` entries (any number: -1) on device ``key``."""
+    if t.dtype is _i32 and t.dim() == 1 and t.get_device() == key and (rows < 0 or t.shape[0] == rows):
+        return t if t.stride(0) == 1 else t.contiguous()
+    return _refuse_index(t, name, key, 1, rows)
+
+
+def _table(t: torch.Tensor, name: str, key: int, rows: int) -> torch.Tensor:
+    """An int32 page table ``[rows, *]`` on device ``key``."""
+    if t.dtype is _i32 and t.dim() == 2 and t.get_device() == key and t.shape[0] == rows:
+        return t if t.stride(1) == 1 else t.contiguous()
+    return _refuse_index(t, name, key, 2, rows)
+
+
+def _refuse_index(t, name, key, dims, rows):
+    if t.get_device() != key:
+        raise RuntimeError(f"tensors on different devices: cuda:{key} and {t.device} ({name})")
     if t.dtype is not _i32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.dim() != 1 or (rows >= 0 and t.shape[0] != rows):
-        raise ValueError(f"{name} must have shape [{rows if rows >= 0 else '*'}], got {list(t.shape)}")
-    return t if t.stride(0) == 1 else t.contiguous()
+    want = ", ".join([str(rows) if rows >= 0 else "*"] + ["*"] * (dims - 1))
+    raise ValueError(f"{name} must have shape [{want}], got {list(t.shape)}")
 
 
-def _table(t: torch.Tensor, name: str, dev, rows: int) -> torch.Tensor:
-    """An int32 page table ``[rows, *]`` on ``dev``."""
-    if t.device != dev:
-        raise RuntimeError(f"tensors on different devices: {dev} and {t.device} ({name})")
-    if t.dtype is not _i32:
-        raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != rows:
-        raise ValueError(f"{name} must have shape [{rows}, *], got {list(t.shape)}")
-    return t if t.stride(1) == 1 else t.contiguous()
+def _check_rows(t, name, key, dtype, shape):
+    """``[rows, heads, d]`` of the cache's device and type, last dimension contiguous."""
+    if t.get_device() != key:
+        _require_cuda(t)
+        raise RuntimeError(f"tensors on different devices: cuda:{key} and {t.device} ({name})")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} ({t.dtype}) must have the cache's dtype {dtype}")
+    return _last_contig(t)
 
 
 def _cache_args(k_pages, v_pages, page_table, kv_lens, weights, op):
-    """The device, the filled :class:`SsaPagedCache` (with the op's error word),
-    whether to wait for errors, and the index tensors the struct points into."""
-    dev = _require_cuda(k_pages, v_pages)
+    """The device's number, the filled :class:`SsaPagedCache` (with the op's error
+    word), whether to wait for errors, and the index tensors the struct points into."""
+    key = k_pages.get_device()
+    if not k_pages.is_cuda or v_pages.get_device() != key:
+        _require_cuda(k_pages, v_pages)
     shape = k_pages.shape
     if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must both be [num_pages, page_size, h_kv, d], got "
                          f"{list(shape)} and {list(v_pages.shape)}")
-    if k_pages.dtype != v_pages.dtype:
+    if k_pages.dtype is not v_pages.dtype:
         raise TypeError(f"k_pages, v_pages dtypes differ: {k_pages.dtype}, {v_pages.dtype}")
     kp, kn, kh, kd = k_pages.stride()
     vp, vn, vh, vd = v_pages.stride()
     # the pages are written in place, so a copy would be of no use
     if kd != 1 or vd != 1:
         raise ValueError("the last dimension of k_pages and v_pages must be contiguous")
-    kv_lens = _index(kv_lens, "kv_lens", dev, -1)
+    kv_lens = _index(kv_lens, "kv_lens", key, -1)
     batch = kv_lens.shape[0]
-    page_table = _table(page_table, "page_table", dev, batch)
+    page_table = _table(page_table, "page_table", key, batch)
     w, wp, wn, wh = None, 0, 0, 0
     if weights is not None:
-        if weights.device != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {weights.device} (weights)")
-        if weights.dtype != torch.float32:
+        if weights.get_device() != key:
+            raise RuntimeError(f"tensors on different devices: cuda:{key} and {weights.device} (weights)")
+        if weights.dtype is not _f32:
             raise TypeError(f"weights must be float32, got {weights.dtype}")
         if weights.shape != shape[:3]:
             raise ValueError(f"weights must be [num_pages, page_size, h_kv] = {list(shape[:3])}, got "
                              f"{list(weights.shape)}")
         w, (wp, wn, wh) = weights.data_ptr(), weights.stride()
     num_pages, page_size, h_kv, d = shape
-    word, sync = S.host_word(dev, op)
+    word, sync = S.host_word(key, op)
     c = L.SsaPagedCache(batch, page_table.shape[1], page_size, h_kv, d, _dtype_code(k_pages), num_pages,
                         k_pages.data_ptr(), kp, kn, kh, v_pages.data_ptr(), vp, vn, vh, w, wp, wn, wh,
                         page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), word)
-    return dev, c, sync, (page_table, kv_lens)
+    return key, c, sync, (page_table, kv_lens)
 
 
-def _call(dev, sync, fn, *args):
-    if torch.cuda.current_device() == dev.index:
-        code = fn(*args, _raw_stream(dev.index))
+def _call(key, sync, fn, *args):
+    if torch.cuda.current_device() == key:
+        code = fn(*args, _raw_stream(key))
     else:
-        with torch.cuda.device(dev):
-            code = fn(*args, _raw_stream(dev.index))
+        with torch.cuda.device(key):
+            code = fn(*args, _raw_stream(key))
     if code:
         L.check(fn.__name__, code)
     if sync:
-        S.host_word_done(dev)
+        S.host_word_done(torch.device("cuda", key))
+
+
+# One workspace per (device, stream), kept: calls on a stream follow one another.
+# A capture takes its own (its graph owns that memory), and so do rare large ones.
+_KEPT = 96 << 20
+_workspaces = {}
+
+
+def _workspace(key: int, nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    if nbytes > _KEPT or torch.cuda.is_current_stream_capturing():
+        return like.new_empty((nbytes,), dtype=torch.uint8)
+    at = key, _raw_stream(key)
+    ws = _workspaces.get(at)
+    if ws is None or ws.numel() < nbytes:
+        with torch.cuda.device(key):
+            ws = _workspaces[at] = like.new_empty((nbytes,), dtype=torch.uint8)
+    return ws
 
 
 def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -126,20 +155,17 @@ def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
         weights: optional ``[num_pages, page_size, h_kv]`` float32 slot weights;
             those of the written slots become 0.
     """
-    dev, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _APPEND)
-    if k_new.device != dev or v_new.device != dev:
-        _require_cuda(k_pages, k_new, v_new)
-    shape = k_new.shape
+    key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _APPEND)
+    dtype, shape = k_pages.dtype, k_new.shape
+    k_new = _check_rows(k_new, "k_new", key, dtype, shape)
+    v_new = _check_rows(v_new, "v_new", key, dtype, shape)
     if shape != v_new.shape or len(shape) != 3 or shape[1] != c.h_kv or shape[2] != c.d:
         raise ValueError(f"k_new and v_new must be [rows, {c.h_kv}, {c.d}], got {list(shape)} and {list(v_new.shape)}")
-    if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
-        raise TypeError(f"k_new, v_new ({k_new.dtype}, {v_new.dtype}) must have the cache's dtype {k_pages.dtype}")
-    q_starts = _index(q_starts, "q_starts", dev, c.batch + 1)
-    k_new, v_new = _last_contig(k_new), _last_contig(v_new)
+    q_starts = _index(q_starts, "q_starts", key, c.batch + 1)
     kn, kh, _ = k_new.stride()
     vn, vh, _ = v_new.stride()
     a = L.SsaPagedAppendArgs(shape[0], q_starts.data_ptr(), k_new.data_ptr(), kn, kh, v_new.data_ptr(), vn, vh)
-    _call(dev, sync, L.lib().ssa_paged_append, ctypes.byref(c), ctypes.byref(a))
+    _call(key, sync, L.lib().ssa_paged_append, c, a)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -167,28 +193,25 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     sees no slot gets zeros (and ``-inf``).  Rows outside ``q_starts`` are not
     written.
     """
-    dev, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
-    if q.device != dev:
-        _require_cuda(k_pages, q)
-    if q.dim() != 3 or q.shape[2] != c.d:
-        raise ValueError(f"q must be [rows, h_q, {c.d}], got {list(q.shape)}")
-    rows, h_q, d = q.shape
+    key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
+    shape = q.shape
+    q = _check_rows(q, "q", key, k_pages.dtype, shape)
+    if len(shape) != 3 or shape[2] != c.d:
+        raise ValueError(f"q must be [rows, h_q, {c.d}], got {list(shape)}")
+    rows, h_q, d = shape
     if h_q % c.h_kv:
         raise ValueError("num_q_heads must be divisible by num_kv_heads")
-    if q.dtype != k_pages.dtype:
-        raise TypeError(f"q ({q.dtype}) must have the cache's dtype {k_pages.dtype}")
-    q_starts = _index(q_starts, "q_starts", dev, c.batch + 1)
-    q = _last_contig(q)
+    q_starts = _index(q_starts, "q_starts", key, c.batch + 1)
     qn, qh, _ = q.stride()
-    out = q.new_empty((rows, h_q, d))
-    lse = q.new_empty((rows, h_q), dtype=torch.float32) if return_lse else None
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((rows, h_q), dtype=_f32) if return_lse else None
     a = L.SsaPagedAttnArgs(rows, q_starts.data_ptr(), h_q, 1 if is_causal else 0,
                            math.sqrt(d) if scale is None else float(scale), q.data_ptr(), qn, qh, out.data_ptr(),
                            h_q * d, d, lse.data_ptr() if return_lse else None)
-    lib, rc, ra = L.lib(), ctypes.byref(c), ctypes.byref(a)
-    nbytes = lib.ssa_paged_attn_workspace_size(rc, ra)
-    ws = q.new_empty((nbytes,), dtype=torch.uint8)
-    _call(dev, sync, lib.ssa_paged_attn, rc, ra, ws.data_ptr(), nbytes)
+    lib = L.lib()
+    nbytes = lib.ssa_paged_attn_workspace_size(c, a)
+    ws = _workspace(key, nbytes, q)
+    _call(key, sync, lib.ssa_paged_attn, c, a, ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -208,16 +231,16 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     """
     if weights is None:
         raise ValueError("weights is needed: eviction ranks slots by them")
-    dev, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
+    key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget {budget}, recent {recent}: need budget >= 1 and 0 <= recent <= budget")
-    new_table = _table(new_table, "new_table", dev, c.batch)
-    kept = torch.empty((c.batch, c.h_kv, budget), dtype=torch.int32, device=dev)
-    new_lens = torch.empty((c.batch,), dtype=torch.int32, device=dev)
+    new_table = _table(new_table, "new_table", key, c.batch)
+    kept = kv_lens.new_empty((c.batch, c.h_kv, budget))
+    new_lens = kv_lens.new_empty((c.batch,))
     a = L.SsaPagedEvictArgs(budget, recent, new_table.shape[1], new_table.data_ptr(), new_table.stride(0),
                             kept.data_ptr(), new_lens.data_ptr())
-    _call(dev, sync, L.lib().ssa_paged_evict, ctypes.byref(c), ctypes.byref(a))
+    _call(key, sync, L.lib().ssa_paged_evict, c, a)
     return kept, new_lens
 
 
