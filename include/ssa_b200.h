@@ -369,6 +369,10 @@ typedef struct {
   float* lse;                 /* optional [rows, h_q]: log of the row's sum of exponentials */
 } SsaPagedAttnArgs;
 
+/* Bytes of workspace the call needs.  Its first SSA_PAGED_ZEROED bytes must be zero before the first call that uses it;
+ * every call leaves them zero.  Calls that may overlap on the GPU need a
+ * workspace each. */
+#define SSA_PAGED_ZEROED 16384
 size_t ssa_paged_attn_workspace_size(const SsaPagedCache* cache, const SsaPagedAttnArgs* args);
 
 /* Softmax attention of the new rows over what their sequences have cached.

@@ -109,6 +109,9 @@ class _HostWords:
 
 
 _words = {}
+# Workspaces the paged ops keep, by (device, stream).  Their heads are zero between
+# calls, except after a kernel that gave up.
+workspaces = {}
 
 
 def host_word(key: int, op: int):
@@ -251,5 +254,6 @@ def paged_error(op: str, bits: int) -> Exception:
     if bits & L.SSA_DEVICE_BAD_LENGTH:
         return ValueError(f"{op}: q_starts or a length does not fit the rows and the page table")
     if bits & L.SSA_DEVICE_TIMEOUT:
+        workspaces.clear()
         return RuntimeError(f"{op}: a device pipeline wait timed out; results are undefined")
     return RuntimeError(f"{op}: device status 0x{bits:x}")

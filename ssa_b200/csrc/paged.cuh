@@ -12,8 +12,8 @@
 // [c W / G, (c + 1) W / G) of the W there are, whatever the lengths of the
 // batch: ragged batches and long contexts of few rows spread evenly, with no
 // plan made on the host.  An item cut by a CTA boundary leaves partial results
-// (running maximum, sum, unnormalised rows) that combine_kernel joins in CTA
-// order, so results do not depend on timing.
+// (running maximum, sum, unnormalised rows) that are joined in CTA order, so
+// results do not depend on timing (paged_join.cuh).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -62,6 +62,7 @@ struct PagedAttnParams {
   float* lse2;                     // [rows, h_q] row log2-sum-exp2 for the weights pass, or NULL
   float* part;                     // [grid][2][tile rows][d + 4]: unnormalised row, maximum (log2), sum, -
   PagedSplit* split;               // [grid]
+  int32_t* counters;               // [grid], zero before and after a launch
   float* scores;                   // [rows, h_q, slots of a table row] scaled logits (base 2), or NULL
   int64_t rows;
   int group, causal;

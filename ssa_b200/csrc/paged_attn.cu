@@ -13,8 +13,8 @@
 #include <cmath>
 
 #include "common.cuh"
-#include "mma_utils.cuh"
 #include "paged.cuh"
+#include "paged_join.cuh"
 #include "paged_tma.cuh"
 
 namespace ssa {
@@ -23,8 +23,6 @@ namespace {
 constexpr int kKT = 64;            // slots per key tile
 constexpr int kThreads = 256;
 constexpr int kExtra = 1;          // units an item costs besides its tiles
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // Rows of the item's tile: row r is token tile * tt + r / g, head h * g + r % g.
 struct TileRows {
@@ -39,26 +37,6 @@ __device__ __forceinline__ TileRows tile_rows(const PagedWalk& w, int tt, int gr
 // Slots the row of token `tok` sees.
 __device__ __forceinline__ int seen_slots(const PagedAttnParams& p, int n, int len, int tok) {
   return p.causal ? max(len - n + tok + 1, 0) : len;
-}
-
-// lse of a row from its maximum (base 2) and sum; -inf for a row that saw nothing.
-__device__ __forceinline__ void store_lse(const PagedAttnParams& p, int64_t tok, int head, float m, float l) {
-  const int64_t at = tok * (static_cast<int64_t>(p.c.h_kv) * p.group) + head;
-  const float z = l == 0.f ? -INFINITY : m + log2f(l);
-  if (p.lse) p.lse[at] = z * kLn2;
-  if (p.lse2) p.lse2[at] = z;
-}
-
-template <typename T>
-__device__ __forceinline__ void store4(T* dst, const float4& v, float f) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(dst) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-  } else {
-    uint2 u;
-    u.x = pack2<T>(v.x * f, v.y * f);
-    u.y = pack2<T>(v.z * f, v.w * f);
-    *reinterpret_cast<uint2*>(dst) = u;
-  }
 }
 
 template <typename T>
@@ -320,55 +298,14 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedAttnParams p, int R) 
   const int64_t before = p.split[b - 1].item_first;
   // the item starts before this CTA, and in the CTA before it
   if (!it.valid || it.cta_first != b - 1) return;
-  const int d = p.c.d, pd = d + 4, parts = it.cta_last - b + 2;     // CTAs b - 1 .. cta_last
+  const int pd = p.c.d + 4, parts = it.cta_last - b + 2;            // CTAs b - 1 .. cta_last
   const int slot0 = before == it.item_first ? 0 : 1;                // CTA b - 1: is it also that CTA's first item
-  const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
-  const int64_t step = static_cast<int64_t>(2) * R * pd;
-  const int x0 = 4 * lane, x1 = x0 + 128;                           // this lane's columns
-  for (int r = blockIdx.y * (blockDim.x / kWarp) + warp; r < it.rows; r += gridDim.y * (blockDim.x / kWarp)) {
-    const float* src = p.part + (static_cast<int64_t>(b - 1) * 2 * R + r) * pd;
-    float m = -INFINITY, l = 0.f;
-    float4 o0 = make_float4(0.f, 0.f, 0.f, 0.f), o1 = o0;
-    for (int i0 = 0; i0 < parts; i0 += 4) {
-      float2 ml[4];
-      float4 a0[4], a1[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ml[i] = make_float2(-INFINITY, 0.f);
-        a0[i] = a1[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i0 + i < parts) {
-          const float* s = src + (i0 + i) * step + (i0 + i == 0 && slot0 ? static_cast<int64_t>(R) * pd : 0);
-          ml[i] = *reinterpret_cast<const float2*>(s + d);
-          if (x0 < d) a0[i] = *reinterpret_cast<const float4*>(s + x0);
-          if (x1 < d) a1[i] = *reinterpret_cast<const float4*>(s + x1);
-        }
-      }
-      float mn = m;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mn = fmaxf(mn, ml[i].x);
-      const float base = mn == -INFINITY ? 0.f : mn, f = exp2f(m - base);
-      m = mn;
-      l *= f;
-      o0.x *= f; o0.y *= f; o0.z *= f; o0.w *= f;
-      o1.x *= f; o1.y *= f; o1.z *= f; o1.w *= f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float g = exp2f(ml[i].x - base);
-        l = fmaf(g, ml[i].y, l);
-        o0.x = fmaf(g, a0[i].x, o0.x); o0.y = fmaf(g, a0[i].y, o0.y);
-        o0.z = fmaf(g, a0[i].z, o0.z); o0.w = fmaf(g, a0[i].w, o0.w);
-        o1.x = fmaf(g, a1[i].x, o1.x); o1.y = fmaf(g, a1[i].y, o1.y);
-        o1.z = fmaf(g, a1[i].z, o1.z); o1.w = fmaf(g, a1[i].w, o1.w);
-      }
-    }
-    const int64_t tok = it.tok0 + r / p.group;
-    const int head = it.head * p.group + r % p.group;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* dst = static_cast<T*>(p.out) + tok * p.o_sn + head * p.o_sh;
-    if (x0 < d) store4(dst + x0, o0, inv);
-    if (x1 < d) store4(dst + x1, o1, inv);
-    if (lane == 0) store_lse(p, tok, head, m, l);
-  }
+  const int64_t one = static_cast<int64_t>(R) * pd;
+  const float* first = p.part + static_cast<int64_t>(b - 1) * 2 * one;
+  const int warps = blockDim.x / kWarp;
+  for (int r = blockIdx.y * warps + threadIdx.x / kWarp; r < it.rows; r += gridDim.y * warps)
+    write_joined<T, 4>(p, [&](int i) { return first + (2 * i + (i == 0 ? slot0 : 0)) * one + r * pd; }, parts, it.tok0,
+                       it.head, r);
 }
 
 // ---------------------------------------------------------------------------
@@ -473,7 +410,7 @@ enum class AttnKernel { kSimt, kTokens, kChunks };
 struct AttnPlan {
   AttnKernel kernel;
   int rows, grid;
-  size_t split, lse2, scores, total;
+  size_t part, split, lse2, scores, total;
 };
 
 // More than 16 rows (new tokens x heads of a group) per sequence on average
@@ -486,7 +423,8 @@ AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   a.grid = a.kernel == AttnKernel::kSimt ? 2 * 148 : 148;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t lines = static_cast<size_t>(p.rows) * p.c.h_kv * p.group;
-  a.split = up(static_cast<size_t>(a.grid) * 2 * a.rows * (p.c.d + 4) * 4);
+  a.part = SSA_PAGED_ZEROED;                 // after the counters, whose place never changes
+  a.split = a.part + up(static_cast<size_t>(a.grid) * 2 * a.rows * (p.c.d + 4) * 4);
   a.lse2 = a.split + up(a.grid * sizeof(PagedSplit));
   a.scores = a.lse2 + (p.c.w ? up(lines * 4) : 0);
   a.total = a.scores;
@@ -501,7 +439,8 @@ size_t paged_attn_workspace(const PagedAttnParams& p, ssa_dtype dt) { return att
 cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStream_t st) {
   const AttnPlan a = attn_plan(p, dt);
   char* at = static_cast<char*>(ws);
-  p.part = reinterpret_cast<float*>(at);
+  p.counters = reinterpret_cast<int32_t*>(at);
+  p.part = reinterpret_cast<float*>(at + a.part);
   p.split = reinterpret_cast<PagedSplit*>(at + a.split);
   p.lse2 = p.c.w ? reinterpret_cast<float*>(at + a.lse2) : nullptr;
   p.scores = a.total > a.scores ? reinterpret_cast<float*>(at + a.scores) : nullptr;
@@ -513,12 +452,14 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
       e = a.rows == 64 ? launch_simt_t<64>(p, dt, a.grid, false, st) : launch_simt_t<16>(p, dt, a.grid, false, st);
   }
   if (e != cudaSuccess) return e;
-  // one wave of blocks: two warps' rows each for few rows, four for many
-  const dim3 grid(a.grid - 1, a.rows == 256 ? 8 : a.rows / 8);
-  switch (dt) {
-    case SSA_F32: e = launch_after(combine_kernel<float>, grid, dim3(256), 0, st, p, a.rows); break;
-    case SSA_BF16: e = launch_after(combine_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, a.rows); break;
-    default: e = launch_after(combine_kernel<__half>, grid, dim3(256), 0, st, p, a.rows); break;
+  if (a.kernel != AttnKernel::kTokens) {
+    // one wave of blocks: two warps' rows each for few rows, four for many
+    const dim3 grid(a.grid - 1, a.rows == 256 ? 8 : a.rows / 8);
+    switch (dt) {
+      case SSA_F32: e = launch_after(combine_kernel<float>, grid, dim3(256), 0, st, p, a.rows); break;
+      case SSA_BF16: e = launch_after(combine_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, a.rows); break;
+      default: e = launch_after(combine_kernel<__half>, grid, dim3(256), 0, st, p, a.rows); break;
+    }
   }
   if (e != cudaSuccess || !p.c.w) return e;
   if (p.scores) return launch_paged_weights_dec(p, st);

@@ -25,6 +25,7 @@
 #include "common.cuh"
 #include "mma_utils.cuh"
 #include "paged.cuh"
+#include "paged_join.cuh"
 #include "paged_tma.cuh"
 #include "tc_utils.cuh"
 
@@ -38,8 +39,6 @@ constexpr int kKT = 64;
 constexpr int kExtra = 4;          // units an item costs besides its tiles
 constexpr int kWarps = 8;          // consumers: two groups of four, 16 slots of a tile each
 constexpr int kThreads = 32 * (kWarps + 1);
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 template <int D>
 struct Geo {
@@ -59,6 +58,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
                                                                PagedAttnParams p, MapOrder mo) {
   using G = Geo<D>;
   constexpr int KS = D / 16, NT = D / 8;
+  constexpr int64_t kPartFloats = kRows * (D + 4);
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
   uint64_t* bars = reinterpret_cast<uint64_t*>(join + kWarps * kRows * G::kJoinRow);
   const uint32_t ring = smem_u32(base), full = smem_u32(bars), empty = full + 8 * G::kStages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * G::kStages);
+  volatile int* last = abort_flag + 1;
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int tt = tile_tokens(kRows, p.group);
   if (threadIdx.x == 0) {
@@ -82,7 +83,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
   paged_start(p, tt, kKT, kExtra, &start);
   __syncthreads();
   PagedWalk w = start.w;
-  if (threadIdx.x == 0) p.split[blockIdx.x] = start.any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
   if (!start.any) return;
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (!mbar_wait_or(bar, parity, abort_flag) && !*abort_flag) {
@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
     }
     asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
     const int r = threadIdx.x >> 4, x0 = (threadIdx.x & 15) * (D / 16);
+    const bool whole = seg.whole;
     if (r < rows) {
       float mx = -INFINITY;
 #pragma unroll
@@ -320,11 +321,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
         fy[y] = ex2_approx(src[D] - off);
         sum = fmaf(fy[y], src[D + 1], sum);
       }
-      const bool whole = seg.whole;
       const int tok = tok0 + r / p.group, head = w.head * p.group + r % p.group;
       const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
       T* out = static_cast<T*>(p.out) + (w.q0 + tok) * p.o_sn + static_cast<int64_t>(head) * p.o_sh + x0;
-      float* part = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * kRows + r) * (D + 4);
+      float* part = p.part + (blockIdx.x * 2 + slot) * kPartFloats + r * (D + 4);
 #pragma unroll
       for (int x = 0; x < D / 16; x += 4) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -347,17 +347,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
       }
       if ((threadIdx.x & 15) == 0) {
         if (whole) {
-          const int64_t at = (w.q0 + tok) * (static_cast<int64_t>(p.c.h_kv) * p.group) + head;
-          const float z = sum == 0.f ? -INFINITY : mx + log2f(sum);
-          if (p.lse) p.lse[at] = z * kLn2;
-          if (p.lse2) p.lse2[at] = z;
+          store_lse(p, w.q0 + tok, head, mx, sum);
         } else {
           part[D] = mx;
           part[D + 1] = sum;
         }
       }
     }
-    asm volatile("barrier.cta.sync 1, 256;" ::: "memory");   // before the next item's partials overwrite these
+    if (!whole) __threadfence();                         // the part, before this CTA counts itself in
+    asm volatile("barrier.cta.sync 1, 256;" ::: "memory");   // also: before the next item's partials overwrite these
+    if (!whole) {
+      // the last of the item's CTAs joins it, a warp per row
+      const int a = unit_cta(w, w.item_first + kExtra), parts = unit_cta(w, w.item_first + w.units - 1) - a + 1;
+      if (threadIdx.x == 0) {
+        const bool is = atomicAdd(p.counters + a, 1) == parts - 1;
+        if (is) p.counters[a] = 0;
+        *last = is;
+      }
+      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+      if (*last) {
+        __threadfence();
+        // the item is the second of CTA a's two parts if a's share starts before it
+        const int second = mul_div(a, w.total, w.ctas) < w.item_first ? 1 : 0;
+        const float* first = p.part + 2 * static_cast<int64_t>(a) * kPartFloats;
+        for (int r = warp; r < rows; r += kWarps)
+          write_joined<T, 8>(p, [&](int i) { return first + (2 * i + (i == 0 ? second : 0)) * kPartFloats + r * (D + 4); },
+                             parts, w.q0 + tok0, w.head, r);
+      }
+    }
   }
 }
 

@@ -39,6 +39,7 @@
 #include "common.cuh"
 #include "mma_utils.cuh"
 #include "paged.cuh"
+#include "paged_join.cuh"
 #include "paged_tma.cuh"
 #include "tc_utils.cuh"
 
@@ -51,8 +52,6 @@ constexpr int kRows = 256;         // rows of an item
 constexpr int kKT = 128;           // slots per key tile
 constexpr int kExtra = 4;          // units an item costs besides its tiles
 constexpr int kThreads = 320;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 8.f;      // how far (log2) a tile may exceed the running maximum
 
 template <int D>
@@ -564,10 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       }
       if (live) {
         if (whole) {
-          const int64_t at = (w.q0 + tok) * (static_cast<int64_t>(p.c.h_kv) * p.group) + head;
-          const float z = l == 0.f ? -INFINITY : m - kShift + log2f(l);
-          if (p.lse) p.lse[at] = z * kLn2;
-          if (p.lse2) p.lse2[at] = z;
+          store_lse(p, w.q0 + tok, head, m - kShift, l);
         } else {
           part[D] = m - kShift;
           part[D + 1] = l;

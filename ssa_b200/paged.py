@@ -124,19 +124,22 @@ def _call(key, sync, fn, *args):
 
 
 # One workspace per (device, stream), kept: calls on a stream follow one another.
-# A capture takes its own (its graph owns that memory), and so do rare large ones.
+# A capture takes its own (its graph owns that memory), and so do rare large
+# ones.  The head of a workspace is zero before a call and after it.
 _KEPT = 96 << 20
-_workspaces = {}
 
 
 def _workspace(key: int, nbytes: int, like: torch.Tensor) -> torch.Tensor:
     if nbytes > _KEPT or torch.cuda.is_current_stream_capturing():
-        return like.new_empty((nbytes,), dtype=torch.uint8)
+        ws = like.new_empty((nbytes,), dtype=torch.uint8)
+        ws[:L.SSA_PAGED_ZEROED].zero_()
+        return ws
     at = key, _raw_stream(key)
-    ws = _workspaces.get(at)
+    ws = S.workspaces.get(at)
     if ws is None or ws.numel() < nbytes:
         with torch.cuda.device(key):
-            ws = _workspaces[at] = like.new_empty((nbytes,), dtype=torch.uint8)
+            ws = S.workspaces[at] = like.new_empty((nbytes,), dtype=torch.uint8)
+            ws[:L.SSA_PAGED_ZEROED].zero_()
     return ws
 
 
