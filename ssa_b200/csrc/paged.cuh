@@ -92,6 +92,12 @@ __device__ __forceinline__ void page_of(const PagedCacheParams& c, int slot, int
   }
 }
 
+// Elements from row to row of the kept scores: the slots a table row holds, in
+// whole 16-byte vectors.
+__host__ __device__ inline int64_t score_stride(const PagedCacheParams& c) {
+  return (static_cast<int64_t>(c.max_pages) * c.page_size + 3) / 4 * 4;
+}
+
 // Page of a slot below the sequence's length; -1 where the table is wrong.
 __device__ __forceinline__ int64_t physical_page(const PagedCacheParams& c, const int32_t* table, int64_t stride,
                                                  int seq, int page) {

@@ -9,8 +9,7 @@
 // query rows (the g heads of a KV group at R / g consecutive tokens) and walks
 // key tiles of 64 slots: 256 threads form a 16 x 16 grid, a thread owns R / 16
 // rows and every 16th key (scores) or column quad (output).
-#include <algorithm>
-#include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -52,41 +51,8 @@ __device__ __forceinline__ void load_rows(const PagedAttnParams& p, int64_t q0, 
                      static_cast<int64_t>(head * p.group + r % p.group) * p.q_sh + x;
       load8<T>(src, f);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) qs[r * stride + x + i] = f[i] * c;
-  }
-}
-
-// 64 slots' element offsets in the pages (-1: past `lim`, or a bad page).
-__device__ __forceinline__ void tile_offsets(const PagedCacheParams& c, int seq, int head, int k0, int lim,
-                                             int64_t* koff, int64_t* voff) {
-  if (threadIdx.x < kKT) {
-    const int j = k0 + threadIdx.x;
-    int64_t ko = -1, vo = -1;
-    if (j < lim) {
-      int page, row;
-      page_of(c, j, page, row);
-      const int64_t pg = physical_page(c, c.table, c.table_stride, seq, page);
-      if (pg >= 0) {
-        ko = pg * c.k_sp + row * c.k_sn + static_cast<int64_t>(head) * c.k_sh;
-        vo = pg * c.v_sp + row * c.v_sn + static_cast<int64_t>(head) * c.v_sh;
-      }
-    }
-    koff[threadIdx.x] = ko;
-    voff[threadIdx.x] = vo;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void load_tile(const void* base, const int64_t* off, int d, int dpad, int stride,
-                                          float* dst) {
-  const int vecs = dpad / 8;
-  for (int e = threadIdx.x; e < kKT * vecs; e += kThreads) {
-    const int r = e / vecs, x = (e - r * vecs) * 8;
-    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (off[r] >= 0 && x < d) load8<T>(static_cast<const T*>(base) + off[r] + x, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) dst[r * stride + x + i] = f[i];
+    *reinterpret_cast<float4*>(qs + r * stride + x) = make_float4(f[0] * c, f[1] * c, f[2] * c, f[3] * c);
+    *reinterpret_cast<float4*>(qs + r * stride + x + 4) = make_float4(f[4] * c, f[5] * c, f[6] * c, f[7] * c);
   }
 }
 
@@ -119,8 +85,49 @@ __device__ __forceinline__ void scores(const float* qs, const float* ks, int d, 
 template <int R, int DP>
 struct SimtGeo {
   static constexpr int QS = DP + 4, PS = kKT + 4;          // row strides: 16-byte rows on shifted banks
-  static constexpr size_t kSmem = sizeof(float) * (R * QS + kKT * QS + R * PS) + 2 * sizeof(int64_t) * kKT;
+  // Q, a key tile, a value tile, P
+  static constexpr size_t kSmem = sizeof(float) * (R * QS + 2 * kKT * QS + R * PS);
 };
+
+// This thread's row of a key tile (four threads a row): its element offsets in
+// the pages, -1 past `lim` or where the page is bad.
+struct RowOffsets {
+  int64_t k, v;
+};
+__device__ __forceinline__ RowOffsets row_offsets(const PagedCacheParams& c, int seq, int head, int j, int lim) {
+  RowOffsets o{-1, -1};
+  if (j < lim) {
+    int page, row;
+    page_of(c, j, page, row);
+    const int64_t pg = physical_page(c, c.table, c.table_stride, seq, page);
+    if (pg >= 0) {
+      o.k = pg * c.k_sp + row * c.k_sn + static_cast<int64_t>(head) * c.k_sh;
+      o.v = pg * c.v_sp + row * c.v_sn + static_cast<int64_t>(head) * c.v_sh;
+    }
+  }
+  return o;
+}
+// Its quarter of the row on the way to shared memory as fp32 (asynchronously
+// where the cache is fp32); columns d .. dpad and rows without a slot are zero.
+template <typename T>
+__device__ __forceinline__ void bring_row(const void* base, int64_t off, int d, int dpad, float* dst) {
+  for (int x = (threadIdx.x & 3) * 8; x < dpad; x += 32) {
+    if (off < 0 || x >= d) {
+      *reinterpret_cast<float4*>(dst + x) = make_float4(0.f, 0.f, 0.f, 0.f);
+      *reinterpret_cast<float4*>(dst + x + 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else if constexpr (sizeof(T) == 4) {
+      const T* src = static_cast<const T*>(base) + off + x;
+      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(dst + x));
+      cp_async16(to, src);
+      cp_async16(to + 16, src + 4);
+    } else {
+      float f[8];
+      load8<T>(static_cast<const T*>(base) + off + x, f);
+      *reinterpret_cast<float4*>(dst + x) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(dst + x + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    }
+  }
+}
 
 template <typename T, int R, int DP>
 __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) {
@@ -129,46 +136,58 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
   extern __shared__ __align__(16) float smem[];
   float* qs = smem;
   float* ks = qs + R * G::QS;
-  float* ps = ks + kKT * G::QS;
-  int64_t* koff = reinterpret_cast<int64_t*>(ps + R * G::PS);
-  int64_t* voff = koff + kKT;
+  float* vs = ks + kKT * G::QS;
+  float* ps = vs + kKT * G::QS;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int tt = tile_tokens(R, p.group), d = p.c.d;
+  const int64_t cap = score_stride(p.c);
   __shared__ PagedStart start;
+  __shared__ bool last_part;
   paged_start(p, tt, kKT, kExtra, &start);
   __syncthreads();
   PagedWalk w = start.w;
-  if (!start.any) {
-    if (tid == 0) p.split[blockIdx.x].valid = 0;
-    return;
-  }
-  if (tid == 0) p.split[blockIdx.x] = paged_split(p, w, tt, kExtra);
+  if (tid == 0) p.split[blockIdx.x] = start.any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
+  if (!start.any) return;
+  float* const krow = ks + (tid >> 2) * G::QS;
+  float* const vrow = vs + (tid >> 2) * G::QS;
   bool going = true;
   for (int slot = 0; going; slot = 1, going = paged_advance(p, tt, kKT, kExtra, w)) {
     const PagedSegment seg = paged_segment(w, kExtra);
     if (seg.first == seg.last) continue;
     const TileRows t = tile_rows(w, tt, p.group);
+    const int tile_min = seen_slots(p, w.n, w.len, t.tok0);                              // every row sees these
+    const int tile_max = seen_slots(p, w.n, w.len, t.tok0 + t.rows / p.group - 1);       // some row sees these
     __syncthreads();
+    RowOffsets off = row_offsets(p.c, w.seq, w.head, seg.first * kKT + (tid >> 2), tile_max);
+    bring_row<T>(p.c.k, off.k, d, d, krow);
+    cp_commit();
+    bring_row<T>(p.c.v, off.v, d, DP, vrow);
+    cp_commit();
     load_rows<T>(p, w.q0, w.head, t, R, G::QS, qs);
     float m[RI], l[RI], o[RI][CI][4];
     int lim[RI];
+    float* sc[RI];
 #pragma unroll
     for (int i = 0; i < RI; ++i) {
+      const int r = ty + 16 * i;
       m[i] = -INFINITY;
       l[i] = 0.f;
-      lim[i] = seen_slots(p, w.n, w.len, t.tok0 + min((ty + 16 * i) / p.group, tt - 1));
+      lim[i] = seen_slots(p, w.n, w.len, t.tok0 + min(r / p.group, tt - 1));
+      sc[i] = p.scores && r < t.rows
+                  ? p.scores + ((w.q0 + t.tok0 + r / p.group) * (static_cast<int64_t>(p.c.h_kv) * p.group) +
+                                w.head * p.group + r % p.group) * cap : nullptr;
 #pragma unroll
       for (int c = 0; c < CI; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][c][e] = 0.f;
     }
-    const int tile_min = seen_slots(p, w.n, w.len, t.tok0);                              // every row sees these
-    const int tile_max = seen_slots(p, w.n, w.len, t.tok0 + t.rows / p.group - 1);       // some row sees these
     for (int kt = seg.first; kt < seg.last; ++kt) {
       const int k0 = kt * kKT;
-      tile_offsets(p.c, w.seq, w.head, k0, tile_max, koff, voff);
-      __syncthreads();
-      load_tile<T>(p.c.k, koff, d, d, G::QS, ks);
+      const bool more = kt + 1 < seg.last;
+      // the next tile's page is looked up now, its keys come during this tile's
+      // product and its values during the next tile's scores
+      if (more) off = row_offsets(p.c, w.seq, w.head, k0 + kKT + (tid >> 2), tile_max);
+      cp_wait<1>();                                          // the keys
       __syncthreads();
       float s[RI][4];
       scores<RI>(qs, ks, d, G::QS, tx, ty, s);
@@ -177,11 +196,13 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (k0 + tx + 16 * j >= lim[i]) s[i][j] = -INFINITY;
+          const int at = k0 + tx + 16 * j;
+          if (sc[i] && at < cap) sc[i][at] = s[i][j];
+          if (at >= lim[i]) s[i][j] = -INFINITY;
           mx = fmaxf(mx, s[i][j]);
         }
 #pragma unroll
-        for (int off = 8; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        for (int x = 8; x; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
         const float mn = fmaxf(m[i], mx);
         const float base = mn == -INFINITY ? 0.f : mn;       // a row that has seen nothing: p = 0, no NaN
         const float r = exp2f(m[i] - base);
@@ -199,10 +220,20 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][c][e] *= r;
       }
+      cp_wait<0>();                                          // the values
       __syncthreads();
-      load_tile<T>(p.c.v, voff, d, DP, G::QS, ks);
-      __syncthreads();
-      if (k0 + kKT <= tile_min) {
+      if (more) bring_row<T>(p.c.k, off.k, d, d, krow);
+      cp_commit();
+      // a tile that some row does not see whole: if it holds a non-finite value,
+      // hidden slots are left out one by one (0 * inf would be NaN)
+      bool odd = false;
+      if (k0 + kKT > tile_min) {
+        for (int x = (tid & 3) * 8; x < d; x += 32)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) odd |= !isfinite(vrow[x + e]);
+        odd = __syncthreads_or(odd);
+      }
+      if (!odd) {
 #pragma unroll 2
         for (int j = 0; j < kKT; j += 4) {
           float4 pr[RI];
@@ -212,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
           for (int jj = 0; jj < 4; ++jj)
 #pragma unroll
             for (int c = 0; c < CI; ++c) {
-              const float4 v = *reinterpret_cast<const float4*>(ks + (j + jj) * G::QS + 64 * c + 4 * tx);
+              const float4 v = *reinterpret_cast<const float4*>(vs + (j + jj) * G::QS + 64 * c + 4 * tx);
 #pragma unroll
               for (int i = 0; i < RI; ++i) {
                 const float e = jj == 0 ? pr[i].x : jj == 1 ? pr[i].y : jj == 2 ? pr[i].z : pr[i].w;
@@ -224,12 +255,10 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
             }
         }
       } else {
-        // some row does not see the whole tile: a hidden slot's value is not
-        // multiplied at all (0 * inf would be NaN)
         for (int j = 0; j < kKT; ++j)
 #pragma unroll
           for (int c = 0; c < CI; ++c) {
-            const float4 v = *reinterpret_cast<const float4*>(ks + j * G::QS + 64 * c + 4 * tx);
+            const float4 v = *reinterpret_cast<const float4*>(vs + j * G::QS + 64 * c + 4 * tx);
 #pragma unroll
             for (int i = 0; i < RI; ++i) {
               const float e = ps[(ty + 16 * i) * G::PS + j];
@@ -243,40 +272,57 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
           }
       }
       __syncthreads();
+      if (more) bring_row<T>(p.c.v, off.v, d, DP, vrow);
+      cp_commit();
     }
-    const bool whole = seg.whole;
+    const int64_t one = static_cast<int64_t>(R) * (d + 4);
 #pragma unroll
     for (int i = 0; i < RI; ++i) {
 #pragma unroll
-      for (int off = 8; off; off >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+      for (int x = 8; x; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
       const int r = ty + 16 * i;
       if (r >= t.rows) continue;
-      if (whole) {
+      if (seg.whole) {
         const int64_t tok = w.q0 + t.tok0 + r / p.group;
         const int head = w.head * p.group + r % p.group;
         const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-        T* dst = static_cast<T*>(p.out) + tok * p.o_sn + head * p.o_sh;
+        T* dst = static_cast<T*>(p.out) + tok * p.o_sn + static_cast<int64_t>(head) * p.o_sh;
 #pragma unroll
         for (int c = 0; c < CI; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int x = 64 * c + 4 * tx + e;
-            if (x < d) dst[x] = Elem<T>::from_f(o[i][c][e] * inv);
-          }
+          if (64 * c + 4 * tx < d)
+            store4(dst + 64 * c + 4 * tx, make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]), inv);
         if (tx == 0) store_lse(p, tok, head, m[i], l[i]);
       } else {
-        float* dst = p.part + (static_cast<int64_t>(blockIdx.x * 2 + slot) * R + r) * (d + 4);
+        float* dst = p.part + (blockIdx.x * 2 + slot) * one + r * (d + 4);
 #pragma unroll
         for (int c = 0; c < CI; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int x = 64 * c + 4 * tx + e;
-            if (x < d) dst[x] = o[i][c][e];
-          }
+          if (64 * c + 4 * tx < d)
+            *reinterpret_cast<float4*>(dst + 64 * c + 4 * tx) =
+                make_float4(o[i][c][0], o[i][c][1], o[i][c][2], o[i][c][3]);
         if (tx == 0) {
           dst[d] = m[i];
           dst[d + 1] = l[i];
         }
+      }
+    }
+    if (R == 16 && !seg.whole) {
+      // few rows: the last of the item's CTAs joins it, a warp per row
+      const int a = unit_cta(w, w.item_first + kExtra), parts = unit_cta(w, w.item_first + w.units - 1) - a + 1;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        last_part = atomicAdd(p.counters + a, 1) == parts - 1;
+        if (last_part) p.counters[a] = 0;
+      }
+      __syncthreads();
+      if (last_part) {
+        __threadfence();
+        // the item is the second of CTA a's two parts if a's share starts before it
+        const int second = mul_div(a, w.total, w.ctas) < w.item_first ? 1 : 0;
+        const float* first = p.part + 2 * static_cast<int64_t>(a) * one;
+        for (int r = tid / kWarp; r < t.rows; r += kThreads / kWarp)
+          write_joined<T, 8>(p, [&](int i) { return first + (2 * i + (i == 0 ? second : 0)) * one + r * (d + 4); },
+                             parts, w.q0 + t.tok0, w.head, r);
       }
     }
   }
@@ -322,17 +368,15 @@ __global__ void __launch_bounds__(kThreads) weights_simt_kernel(PagedAttnParams 
   extern __shared__ __align__(16) float smem[];
   float* qs = smem;
   float* ks = qs + R * G::QS;
-  float* ps = ks + kKT * G::QS;
-  int64_t* koff = reinterpret_cast<int64_t*>(ps + R * G::PS);
-  int64_t* voff = koff + kKT;
+  float* ps = ks + 2 * kKT * G::QS;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int seq = blockIdx.z, head = blockIdx.y, k0 = blockIdx.x * kKT;
   const int tt = tile_tokens(R, p.group), d = p.c.d;
   const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, seq);
   if (q.n == 0 || k0 >= q.len) return;
-  tile_offsets(p.c, seq, head, k0, q.len, koff, voff);
-  __syncthreads();
-  load_tile<T>(p.c.k, koff, d, d, G::QS, ks);
+  bring_row<T>(p.c.k, row_offsets(p.c, seq, head, k0 + (tid >> 2), q.len).k, d, d, ks + (tid >> 2) * G::QS);
+  cp_commit();
+  cp_wait<0>();
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   for (int t0 = 0; t0 < q.n; t0 += tt) {
     const TileRows t{t0, min(tt, q.n - t0) * p.group};
@@ -369,40 +413,46 @@ __global__ void __launch_bounds__(kThreads) weights_simt_kernel(PagedAttnParams 
   }
 }
 
-template <typename T, int R, int DP>
-cudaError_t launch_simt(const PagedAttnParams& p, int grid, bool weights, cudaStream_t st) {
-  const int smem = static_cast<int>(SimtGeo<R, DP>::kSmem);
-  if (!weights) {
-    auto kern = attn_simt_kernel<T, R, DP>;
-    static SmemOptIn opt_in;
-    const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), smem);
-    if (e != cudaSuccess) return e;
-    kern<<<grid, kThreads, smem, st>>>(p);
-    return cudaGetLastError();
-  }
-  auto kern = weights_simt_kernel<T, R, DP>;
-  static SmemOptIn opt_in;
-  const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), smem);
-  if (e != cudaSuccess) return e;
-  const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
-  if (slots == 0) return cudaSuccess;
-  return launch_after(kern, dim3(static_cast<unsigned>(cdiv(slots, kKT)), p.c.h_kv, p.c.batch), dim3(kThreads), smem, st, p);
-}
-
-template <typename T, int R>
-cudaError_t launch_simt_d(const PagedAttnParams& p, int grid, bool weights, cudaStream_t st) {
-  if (p.c.d <= 64) return launch_simt<T, R, 64>(p, grid, weights, st);
-  if (p.c.d <= 128) return launch_simt<T, R, 128>(p, grid, weights, st);
-  return launch_simt<T, R, 256>(p, grid, weights, st);
+// Runs f(type tag, head size class) for the call's type and head size.
+template <typename F>
+cudaError_t by_type_and_size(const PagedAttnParams& p, ssa_dtype dt, F&& f) {
+  auto sized = [&](auto zero) {
+    if (p.c.d <= 64) return f(zero, std::integral_constant<int, 64>{});
+    if (p.c.d <= 128) return f(zero, std::integral_constant<int, 128>{});
+    return f(zero, std::integral_constant<int, 256>{});
+  };
+  if (dt == SSA_F32) return sized(float{});
+  if (dt == SSA_BF16) return sized(__nv_bfloat16{});
+  return sized(__half{});
 }
 
 template <int R>
-cudaError_t launch_simt_t(const PagedAttnParams& p, ssa_dtype dt, int grid, bool weights, cudaStream_t st) {
-  switch (dt) {
-    case SSA_F32: return launch_simt_d<float, R>(p, grid, weights, st);
-    case SSA_BF16: return launch_simt_d<__nv_bfloat16, R>(p, grid, weights, st);
-    default: return launch_simt_d<__half, R>(p, grid, weights, st);
-  }
+cudaError_t launch_simt(const PagedAttnParams& p, ssa_dtype dt, int grid, cudaStream_t st) {
+  return by_type_and_size(p, dt, [&](auto zero, auto size) {
+    using T = decltype(zero);
+    constexpr int DP = decltype(size)::value;
+    auto kern = attn_simt_kernel<T, R, DP>;
+    static SmemOptIn opt_in;
+    const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), SimtGeo<R, DP>::kSmem);
+    if (e != cudaSuccess) return e;
+    kern<<<grid, kThreads, SimtGeo<R, DP>::kSmem, st>>>(p);
+    return cudaGetLastError();
+  });
+}
+
+cudaError_t launch_weights_simt(const PagedAttnParams& p, ssa_dtype dt, cudaStream_t st) {
+  const int64_t slots = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
+  if (slots == 0) return cudaSuccess;
+  const dim3 grid(static_cast<unsigned>(cdiv(slots, kKT)), p.c.h_kv, p.c.batch);
+  return by_type_and_size(p, dt, [&](auto zero, auto size) {
+    using T = decltype(zero);
+    constexpr int DP = decltype(size)::value;
+    auto kern = weights_simt_kernel<T, 64, DP>;
+    static SmemOptIn opt_in;
+    const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), SimtGeo<64, DP>::kSmem);
+    if (e != cudaSuccess) return e;
+    return launch_after(kern, grid, dim3(kThreads), SimtGeo<64, DP>::kSmem, st, p);
+  });
 }
 
 // The kernel that serves a call, its tile rows and grid, and the workspace.
@@ -415,11 +465,12 @@ struct AttnPlan {
 
 // More than 16 rows (new tokens x heads of a group) per sequence on average
 // take tiles of many rows; 16-bit caches that page tiles fit, the tensor cores.
+// (On the CUDA cores a tile costs its rows whether they are used or not.)
 AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   AttnPlan a{};
   const bool chunks = p.rows * p.group > 16ll * p.c.batch;
   a.kernel = !page_tiles_supported(p, dt) ? AttnKernel::kSimt : chunks ? AttnKernel::kChunks : AttnKernel::kTokens;
-  a.rows = !chunks ? 16 : a.kernel == AttnKernel::kChunks ? 256 : 64;
+  a.rows = !chunks ? 16 : a.kernel == AttnKernel::kChunks ? 256 : p.rows * p.group > 32ll * p.c.batch ? 64 : 32;
   a.grid = a.kernel == AttnKernel::kSimt ? 2 * 148 : 148;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t lines = static_cast<size_t>(p.rows) * p.c.h_kv * p.group;
@@ -428,7 +479,7 @@ AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   a.lse2 = a.split + up(a.grid * sizeof(PagedSplit));
   a.scores = a.lse2 + (p.c.w ? up(lines * 4) : 0);
   a.total = a.scores;
-  if (p.c.w && a.kernel == AttnKernel::kTokens) a.total += up(lines * p.c.max_pages * p.c.page_size * 4);
+  if (p.c.w && a.rows == 16) a.total += up(lines * score_stride(p.c) * 4);
   return a;
 }
 
@@ -449,12 +500,14 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
     case AttnKernel::kChunks: e = launch_paged_attn_tc(p, dt, a.grid, st); break;
     case AttnKernel::kTokens: e = launch_paged_attn_dec(p, dt, a.grid, st); break;
     default:
-      e = a.rows == 64 ? launch_simt_t<64>(p, dt, a.grid, false, st) : launch_simt_t<16>(p, dt, a.grid, false, st);
+      e = a.rows == 64   ? launch_simt<64>(p, dt, a.grid, st)
+          : a.rows == 32 ? launch_simt<32>(p, dt, a.grid, st)
+                         : launch_simt<16>(p, dt, a.grid, st);
   }
   if (e != cudaSuccess) return e;
-  if (a.kernel != AttnKernel::kTokens) {
-    // one wave of blocks: two warps' rows each for few rows, four for many
-    const dim3 grid(a.grid - 1, a.rows == 256 ? 8 : a.rows / 8);
+  if (a.rows > 16) {
+    // one wave of blocks, a row or four for every warp
+    const dim3 grid(a.grid - 1, 8);
     switch (dt) {
       case SSA_F32: e = launch_after(combine_kernel<float>, grid, dim3(256), 0, st, p, a.rows); break;
       case SSA_BF16: e = launch_after(combine_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, a.rows); break;
@@ -464,7 +517,7 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
   if (e != cudaSuccess || !p.c.w) return e;
   if (p.scores) return launch_paged_weights_dec(p, st);
   if (a.kernel == AttnKernel::kChunks && paged_weights_tc_supported(p, dt)) return launch_paged_weights_tc(p, dt, st);
-  return a.rows >= 64 ? launch_simt_t<64>(p, dt, 0, true, st) : launch_simt_t<16>(p, dt, 0, true, st);
+  return launch_weights_simt(p, dt, st);
 }
 
 }  // namespace ssa

@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
   // ---------------- consumers ----------------
   const int gr = lane >> 2, gc = lane & 3;               // rows gr, gr + 8; column pairs 2 gc of a fragment
   const float c = p.inv_scale * kLog2e;
-  const int64_t cap = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
+  const int64_t cap = score_stride(p.c);
   // ldmatrix rows of this lane: K (slots x 16 columns), V transposed (16 slots x columns)
   const int kk = (lane >> 4) * 8 + (lane & 7), kp = (lane >> 3) & 1;
   const int vk = ((lane >> 3) & 1) * 8 + (lane & 7), vp = lane >> 4;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(256) weights_dec_kernel(PagedAttnParams p) {
   const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, seq);
   const int j0 = (blockIdx.x * 256 + threadIdx.x) * 4;
   if (q.n == 0 || j0 >= q.len) return;
-  const int64_t cap = static_cast<int64_t>(p.c.max_pages) * p.c.page_size;
+  const int64_t cap = score_stride(p.c);
   const int h_q = p.c.h_kv * p.group;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < q.n; ++i) {
