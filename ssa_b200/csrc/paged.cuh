@@ -237,9 +237,10 @@ struct PagedWalk {
   int seq, head, tile, n, len, units;   // units: of the current item
 };
 
-// Total units, and the walk of CTA `cta` of `grid`.  Called by one full warp;
-// every lane gets the result.  False: no work.
-__device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int extra, int64_t cta, int64_t grid,
+// Total units, and the walk of CTA `cta` of `grid`; little work is shared by
+// fewer CTAs, of `least` units each.  Called by one full warp; every lane gets
+// the result.  False: no work.
+__device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int extra, int least, int64_t cta, int64_t grid,
                                       PagedWalk& w) {
   const int lane = threadIdx.x & 31;
   const int hk = p.c.h_kv;
@@ -259,7 +260,7 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
   int64_t total = mine;
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const int64_t ctas = total < grid ? total : grid;
+  const int64_t ctas = total >= grid * least ? grid : mul_div(total + least - 1, 1, least);
   w.total = total;
   w.ctas = ctas;
   if (cta >= ctas) return false;
@@ -333,10 +334,10 @@ struct PagedStart {
   PagedWalk w;
   int any;
 };
-__device__ inline void paged_start(const PagedAttnParams& p, int tt, int kt, int extra, PagedStart* shared) {
+__device__ inline void paged_start(const PagedAttnParams& p, int tt, int kt, int extra, int least, PagedStart* shared) {
   if (threadIdx.x < 32) {
     PagedWalk w{};
-    const bool any = paged_schedule(p, tt, kt, extra, blockIdx.x, gridDim.x, w);
+    const bool any = paged_schedule(p, tt, kt, extra, least, blockIdx.x, gridDim.x, w);
     if (threadIdx.x == 0) {
       shared->w = w;
       shared->any = any;

@@ -22,6 +22,7 @@ namespace {
 constexpr int kKT = 64;            // slots per key tile
 constexpr int kThreads = 256;
 constexpr int kExtra = 1;          // units an item costs besides its tiles
+constexpr int kLeast = 1;          // units a CTA takes at least
 
 // Rows of the item's tile: row r is token tile * tt + r / g, head h * g + r % g.
 struct TileRows {
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
   const int64_t cap = score_stride(p.c);
   __shared__ PagedStart start;
   __shared__ bool last_part;
-  paged_start(p, tt, kKT, kExtra, &start);
+  paged_start(p, tt, kKT, kExtra, kLeast, &start);
   __syncthreads();
   PagedWalk w = start.w;
   if (tid == 0) p.split[blockIdx.x] = start.any ? paged_split(p, w, tt, kExtra) : PagedSplit{};
@@ -465,12 +466,15 @@ struct AttnPlan {
 
 // More than 16 rows (new tokens x heads of a group) per sequence on average
 // take tiles of many rows; 16-bit caches that page tiles fit, the tensor cores.
-// (On the CUDA cores a tile costs its rows whether they are used or not.)
+// On the CUDA cores a tile costs its rows whether they are used or not, and a
+// row of a 32-row tile about 5/4 of one of a 64-row tile.
 AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   AttnPlan a{};
   const bool chunks = p.rows * p.group > 16ll * p.c.batch;
   a.kernel = !page_tiles_supported(p, dt) ? AttnKernel::kSimt : chunks ? AttnKernel::kChunks : AttnKernel::kTokens;
-  a.rows = !chunks ? 16 : a.kernel == AttnKernel::kChunks ? 256 : p.rows * p.group > 32ll * p.c.batch ? 64 : 32;
+  const int64_t mean = (p.rows * p.group + p.c.batch - 1) / p.c.batch, padded64 = (mean + 63) / 64 * 64,
+                padded32 = (mean + 31) / 32 * 32;
+  a.rows = !chunks ? 16 : a.kernel == AttnKernel::kChunks ? 256 : 4 * padded64 <= 5 * padded32 ? 64 : 32;
   a.grid = a.kernel == AttnKernel::kSimt ? 2 * 148 : 148;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t lines = static_cast<size_t>(p.rows) * p.c.h_kv * p.group;

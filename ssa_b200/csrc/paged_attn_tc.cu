@@ -51,6 +51,7 @@ using namespace tc;
 constexpr int kRows = 256;         // rows of an item
 constexpr int kKT = 128;           // slots per key tile
 constexpr int kExtra = 4;          // units an item costs besides its tiles
+constexpr int kLeast = 1;          // units a CTA takes at least
 constexpr int kThreads = 320;
 constexpr float kSlack = 8.f;      // how far (log2) a tile may exceed the running maximum
 
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 2 * G::kStages + 16);
-  paged_start(p, tt, kKT, kExtra, &start);
+  paged_start(p, tt, kKT, kExtra, kLeast, &start);
   fence_before();
   __syncthreads();
   fence_after();

@@ -96,15 +96,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(PagedEvictPar
   // counts a digit of each lane's key (bin -1: none).  Equal weights (a cache's
   // first steps) would queue 32 deep on one counter.
   auto count = [&](int bin) {
-    if (__all_sync(0xffffffffu, bin >= 0)) {
-      int same;
-      __match_all_sync(0xffffffffu, bin, &same);
-      if (same) {
-        if (lane == 0) atomicAdd(&hist[bin], 32);
-        return;
-      }
+    const int one = __shfl_sync(0xffffffffu, bin, 0);
+    if (one >= 0 && __all_sync(0xffffffffu, bin == one)) {
+      if (lane == 0) atomicAdd(&hist[bin], 32);
+    } else if (bin >= 0) {
+      atomicAdd(&hist[bin], 1);
     }
-    if (bin >= 0) atomicAdd(&hist[bin], 1);
   };
   auto key_of = [&](int j) -> uint32_t { return hold ? sel_keys[j] : read_key(j); };
   for (int pass = 0; pass < 3; ++pass) {
@@ -174,9 +171,11 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(PagedEvictPar
   for (int j = lo + lane; j - lane < hi; j += 32) {
     bool gt, eq;
     kind(j, gt, eq);
-    ng += __popc(__ballot_sync(0xffffffffu, gt));
-    ne += __popc(__ballot_sync(0xffffffffu, eq));
+    ng += gt;
+    ne += eq;
   }
+  ng = __reduce_add_sync(0xffffffffu, ng);
+  ne = __reduce_add_sync(0xffffffffu, ne);
   __syncthreads();
   if (lane == 0) {
     wsum[warp][0] = ng;
