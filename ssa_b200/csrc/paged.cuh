@@ -109,6 +109,16 @@ __device__ __forceinline__ int64_t physical_page(const PagedCacheParams& c, cons
   return pg;
 }
 
+// The same without a branch, for loops that keep many loads in flight: page 0
+// and `bad` where the table is wrong (paged_len lets no slot of an empty cache by).
+__device__ __forceinline__ int64_t page_or_zero(const PagedCacheParams& c, const int32_t* table, int64_t stride,
+                                                int seq, int page, bool& bad) {
+  const int32_t pg = table[static_cast<int64_t>(seq) * stride + page];
+  const bool ok = pg >= 0 && pg < c.num_pages;
+  bad |= !ok;
+  return ok ? pg : 0;
+}
+
 // New rows [q0, q0 + n) and length of a sequence; n = 0 where they are wrong.
 struct PagedSeq {
   int64_t q0;
@@ -118,6 +128,10 @@ __device__ __forceinline__ int paged_len(const PagedCacheParams& c, int s) {
   const int len = c.kv_lens[s];
   if (len < 0 || len > static_cast<int64_t>(c.max_pages) * c.page_size) {
     paged_error(c, SSA_DEVICE_BAD_LENGTH);
+    return -1;
+  }
+  if (len > 0 && c.num_pages == 0) {
+    paged_error(c, SSA_DEVICE_BAD_PAGE);
     return -1;
   }
   return len;
