@@ -370,7 +370,8 @@ typedef struct {
 } SsaPagedAttnArgs;
 
 /* Bytes of workspace the call needs.  Its first SSA_PAGED_ZEROED bytes must be zero before the first call that uses it;
- * every call leaves them zero.  Calls that may overlap on the GPU need a
+ * every call leaves them zero (but one that reports SSA_DEVICE_TIMEOUT: zero
+ * them again).  Calls that may overlap on the GPU need a
  * workspace each. */
 #define SSA_PAGED_ZEROED 16384
 size_t ssa_paged_attn_workspace_size(const SsaPagedCache* cache, const SsaPagedAttnArgs* args);

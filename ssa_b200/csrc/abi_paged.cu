@@ -29,8 +29,8 @@ ssa_status check_cache(const SsaPagedCache* c, ssa::PagedCacheParams& o) {
   if (c->d < 8 || c->d > 256 || c->d % 8 != 0)
     return fail(SSA_ERR_UNSUPPORTED, "head_dim %d: need a multiple of 8 in [8, 256]", c->d);
   if (!valid_dtype(c->dtype)) return fail(SSA_ERR_INVALID_ARG, "bad dtype");
-  if (static_cast<int64_t>(c->max_pages) * c->page_size >= (1ll << 31) - 4096 || c->num_pages >= (1ll << 31))
-    return fail(SSA_ERR_UNSUPPORTED, "max_pages * page_size and num_pages must be < 2^31");
+  if (static_cast<int64_t>(c->max_pages) * c->page_size >= (1ll << 31) - (1ll << 17) || c->num_pages >= (1ll << 31))
+    return fail(SSA_ERR_UNSUPPORTED, "max_pages * page_size must be < 2^31 - 2^17, num_pages < 2^31");
   if (c->batch > 0 && (!c->kv_lens || (c->max_pages > 0 && !c->page_table)))
     return fail(SSA_ERR_INVALID_ARG, "page_table / kv_lens is NULL");
   if (c->num_pages > 0 && (!c->k_pages || !c->v_pages)) return fail(SSA_ERR_INVALID_ARG, "k_pages / v_pages is NULL");
@@ -73,8 +73,8 @@ ssa_status attn_params(const SsaPagedCache* c, const SsaPagedAttnArgs* a, ssa::P
     return fail(SSA_ERR_INVALID_ARG, "num_q_heads (%d) must be a multiple of num_kv_heads (%d)", a->h_q, c->h_kv);
   if (a->h_q / c->h_kv > 16)
     return fail(SSA_ERR_UNSUPPORTED, "%d query heads per KV head: at most 16", a->h_q / c->h_kv);
-  if (!(std::isfinite(a->scale) && a->scale != 0.f))
-    return fail(SSA_ERR_INVALID_ARG, "scale must be finite and not 0");
+  if (!(std::isfinite(a->scale) && a->scale != 0.f && std::isfinite(1.f / a->scale)))
+    return fail(SSA_ERR_INVALID_ARG, "scale must be finite and not 0, and so must its reciprocal");
   if (a->rows > 0 && (!a->q || !a->out)) return fail(SSA_ERR_INVALID_ARG, "q / out is NULL");
   if (!aligned_rows(a->q, a->q_stride_n, a->q_stride_h, c->dtype) ||
       !aligned_rows(a->out, a->out_stride_n, a->out_stride_h, c->dtype))

@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
               unpair(fma_pair(pair(__uint_as_float(v[q4 & 1][4 * j + 2]), __uint_as_float(v[q4 & 1][4 * j + 3])), c2,
                               pair(-z.z, -z.w)), e2, e3);
               if (j % 2 == 0) {                            // a quarter of the exponentials off the MUFU
-                exp2_pair<5>(e0, e1);
+                exp2_pair(e0, e1);
               } else {
                 e0 = ex2_approx(e0);
                 e1 = ex2_approx(e1);

@@ -170,36 +170,37 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// The larger of two floats, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // 2^x of two values <= 127 on the FMA and ALU pipes, to take some of the load
-// off the MUFU: 2^n by the exponent bits, 2^f for f = x - n in [-1/2, 1/2] by a
-// minimax polynomial (Remez exchange on the relative error).  Degree 4: relative
-// error 2.7e-6; degree 5: 2.4e-7.  Below 2^-126 the result is 2^-126; no NaN or
-// infinity comes out as such.
-template <int DEG>
+// off the MUFU: 2^n by the exponent bits times 2^f, f = x - n in [-1/2, 1/2], by
+// a minimax polynomial of degree 5 (Remez exchange on the relative error; 2.4e-7
+// in fp32).  Below 2^-126 the result is 2^-126; NaN stays NaN.
 __device__ __forceinline__ void exp2_pair(float& a, float& b) {
-  const uint64_t x = pair(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t x = pair(max_nan(a, -126.f), max_nan(b, -126.f));
   const uint64_t t = add_pair(x, pair(12582912.f, 12582912.f));            // 1.5 * 2^23: n in the low bits
   const uint64_t n = add_pair(t, pair(-12582912.f, -12582912.f));
   const uint64_t f = fma_pair(n, pair(-1.f, -1.f), x);
-  uint64_t r;
-  if constexpr (DEG == 4) {
-    r = fma_pair(pair(0.009570102207362652f, 0.009570102207362652f), f, pair(0.05591785907745361f, 0.05591785907745361f));
-    r = fma_pair(r, f, pair(0.240247443318367f, 0.240247443318367f));
-    r = fma_pair(r, f, pair(0.6931217908859253f, 0.6931217908859253f));
-    r = fma_pair(r, f, pair(0.9999992847442627f, 0.9999992847442627f));
-  } else {
-    r = fma_pair(pair(0.0013276472454890609f, 0.0013276472454890609f), f,
-                 pair(0.009675540961325169f, 0.009675540961325169f));
-    r = fma_pair(r, f, pair(0.05550713092088699f, 0.05550713092088699f));
-    r = fma_pair(r, f, pair(0.24022120237350464f, 0.24022120237350464f));
-    r = fma_pair(r, f, pair(0.6931469440460205f, 0.6931469440460205f));
-    r = fma_pair(r, f, pair(1.0000001192092896f, 1.0000001192092896f));
-  }
-  float ra, rb, ta, tb;
-  unpair(r, ra, rb);
+  uint64_t r = fma_pair(pair(0.0013276472454890609f, 0.0013276472454890609f), f,
+                        pair(0.009675540961325169f, 0.009675540961325169f));
+  r = fma_pair(r, f, pair(0.05550713092088699f, 0.05550713092088699f));
+  r = fma_pair(r, f, pair(0.24022120237350464f, 0.24022120237350464f));
+  r = fma_pair(r, f, pair(0.6931469440460205f, 0.6931469440460205f));
+  r = fma_pair(r, f, pair(1.0000001192092896f, 1.0000001192092896f));
+  float ta, tb;
   unpair(t, ta, tb);
-  a = __int_as_float(__float_as_int(ra) + (__float_as_int(ta) << 23));
-  b = __int_as_float(__float_as_int(rb) + (__float_as_int(tb) << 23));
+  r = mul_pair(r, pair(__int_as_float((__float_as_int(ta) << 23) + 0x3f800000),
+                       __int_as_float((__float_as_int(tb) << 23) + 0x3f800000)));
+  unpair(r, a, b);
 }
 __device__ __forceinline__ void tmem_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 

@@ -267,6 +267,18 @@ def test_slot_weights_match_formula(lens, q_lens, h_q, h_kv, d, page, layout, ca
     assert torch.equal(c["w"][add == 0].double(), w0[add == 0])
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("q_len", [1, 200])
+def test_nan_in_a_key_reaches_every_weight_of_the_rows_that_see_it(dtype, d, q_len):
+    c = make([300], [q_len], 8, 2, d, 32, dtype, seed=13, weights=True)
+    pg, sl = slots(c, 0, 300)
+    c["k"][pg[250], sl[250], 0, 7] = math.nan          # the last row sees it, and all 300 slots
+    w0 = c["w"].clone()
+    ssa.paged_attention(c["q"], c["k"], c["v"], c["page_table"], c["q_starts"], c["kv_lens"], weights=c["w"])
+    assert torch.isnan(c["w"][pg, sl, 0]).all()
+    assert torch.isfinite(c["w"][pg, sl, 1]).all() and (c["w"][pg, sl, 1] >= w0[pg, sl, 1]).all()
+
+
 def test_a_page_shared_by_two_sequences_collects_both():
     c = make([64, 64], [1, 1], 8, 2, 64, 32, torch.bfloat16, seed=8, weights=True)
     c["table"][1] = c["table"][0]

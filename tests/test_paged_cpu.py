@@ -72,7 +72,7 @@ def test_cache_argument_errors(lib, over, code):
 
 @pytest.mark.parametrize("over,code", [
     (dict(rows=-1), 1), (dict(rows=1 << 31), 1), (dict(q_starts=None), 1), (dict(h_q=7), 1), (dict(h_q=0), 1),
-    (dict(h_q=34), 2), (dict(scale=0.0), 1), (dict(scale=math.inf), 1), (dict(scale=math.nan), 1),
+    (dict(h_q=34), 2), (dict(scale=0.0), 1), (dict(scale=math.inf), 1), (dict(scale=math.nan), 1), (dict(scale=1e-45), 1),
     (dict(q=None), 1), (dict(out=None), 1), (dict(q=0x6004), 4), (dict(out_stride_h=68), 4),
 ])
 def test_attention_argument_errors(lib, over, code):
