@@ -14,12 +14,9 @@
 // 128 x 128 exponentials, which bound it (1024 clocks against 512 at d = 128);
 // a quarter of them is made on the FMA pipe instead (4% faster; a half, no more).
 //
-//   warps 0-7, 8-15 streams: two threads share a slot (its TMEM lane), 64 rows of a
-//                   tile each, and add to its weight one after the other; scores
-//                   from TMEM, two buffers a stream.  (One thread a slot left the
-//                   pipes waiting: 3000 clocks a tile pair against 2048 of MUFU.)
-//   warp 16         TMEM allocation; MMA issue (the warp decides, one lane issues)
-//   warp 17         TMA producer: K (two items deep), Q rows and their lse2 (ring of 3)
+//   warps 0-3, 4-7  streams: a slot per thread; scores from TMEM, two buffers each
+//   warp 8          TMEM allocation, single-thread MMA issue
+//   warp 9          TMA producer: K (two items deep), Q rows and their lse2 (ring of 3)
 //
 // Every wait is bounded (about one second); on expiry the CTA records
 // SSA_DEVICE_TIMEOUT and runs to its end without further waits or copies.
@@ -38,14 +35,14 @@ using namespace tc;
 
 constexpr int kSlots = 128;        // of a stream
 constexpr int kRows = 128;         // of a Q tile
-constexpr int kThreads = 576;
+constexpr int kThreads = 320;
 constexpr int kQStages = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
 struct Geo {
   static constexpr int kTileBytes = 128 * D * 2;
-  static constexpr size_t kSmem = 1024 + (4 + kQStages) * static_cast<size_t>(kTileBytes) + kQStages * kRows * 4 + kRows + 352;
+  static constexpr size_t kSmem = 1024 + (4 + kQStages) * static_cast<size_t>(kTileBytes) + kQStages * kRows * 4 + kRows * 2 + 192;
 };
 
 struct QueryMap {
@@ -92,15 +89,11 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   unsigned char* q_ring = base + 4 * G::kTileBytes;      // base: K [2 items][2 streams]
   float* z_ring = reinterpret_cast<float*>(q_ring + kQStages * G::kTileBytes);
-  unsigned char* row_token = reinterpret_cast<unsigned char*>(z_ring + kQStages * kRows);   // token of a row in its tile
+  short* row_token = reinterpret_cast<short*>(z_ring + kQStages * kRows);   // token of a row in its tile
   uint64_t* bars = reinterpret_cast<uint64_t*>(row_token + kRows);
   const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, q_full = k_empty + 16, q_empty = q_full + 8 * kQStages;
   const uint32_t s_full = q_empty + 8 * kQStages, s_empty = s_full + 32;     // [stream][buffer]
-  // [item mod 3][stream][quarter]: the first half's weights are in.  A half can be
-  // two tiles, so with short items two items, ahead of the other (the two score
-  // buffers); three barriers keep the phase a wait means unambiguous.
-  const uint32_t added = s_empty + 32;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 2 * kQStages + 32);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 2 * kQStages + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int g = p.group, tt = qm.tokens;
@@ -110,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     reinterpret_cast<uint4*>(q_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
   if (threadIdx.x < kRows) {
     const int row = threadIdx.x, a = qm.head_first ? row / g : row % tt, h = qm.head_first ? row % g : row / tt;
-    row_token[row] = static_cast<unsigned char>(h < g && a < tt ? a : kRows);       // kRows: no row
+    row_token[row] = static_cast<short>(h < g && a < tt ? a : kRows);       // kRows: no row
   }
   fence_proxy_async();
   if (threadIdx.x == 0) {
@@ -120,19 +113,18 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     }
     for (int s = 0; s < kQStages; ++s) {
       mbar_init(q_full + 8 * s, 1 + 32);                 // the copies' bytes, and the lse2 of 32 lanes
-      mbar_init(q_empty + 8 * s, 1 + 16);                // the MMAs, and the streams' warps
+      mbar_init(q_empty + 8 * s, 1 + 8);                 // the MMAs, and the streams' warps
     }
     for (int b = 0; b < 4; ++b) {
       mbar_init(s_full + 8 * b, 1);
-      mbar_init(s_empty + 8 * b, 8);
+      mbar_init(s_empty + 8 * b, 4);
     }
-    for (int b = 0; b < 24; ++b) mbar_init(added + 8 * b, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&qmap);
   }
-  if (warp == 16) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -150,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   Items it{0, -1, {0, 0, 0}};
   int64_t t = 0, n = 0;                                  // Q tiles and items so far
 
-  if (warp == 17) {
+  if (warp == 9) {
     // ---------------- producer ----------------
     const int piece_rows = min(p.c.page_size, kSlots), pieces = kSlots / piece_rows, boxes = pieces * (D / 64);
     const int piece = lane & (pieces - 1), half = lane / pieces;
@@ -192,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         const int tokens = min(tt, it.q.n - tile * tt);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          z[e] = row_tok[e] < tokens ? -__ldg(p.lse2 + (tok + row_tok[e]) * h_q + head * g + row_head[e]) : -INFINITY;
+          z[e] = row_tok[e] < tokens ? __ldg(p.lse2 + (tok + row_tok[e]) * h_q + head * g + row_head[e]) : INFINITY;
       };
       if (r * tt < it.q.n) fetch(r);
       for (; r * tt < it.q.n; ++r, ++t) {
@@ -208,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
                       qm.head_first ? y : zc, qm.head_first ? zc : y, q_full + 8 * s);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z_ring[s * kRows + lane + 32 * e] = z[e];   // negated; exp2(s - inf) = 0 where there is no row
+        for (int e = 0; e < 4; ++e) z_ring[s * kRows + lane + 32 * e] = z[e];   // exp2(s - inf) = 0 where there is no row
         mbar_arrive(q_full + 8 * s);
         if ((r + 1) * tt < it.q.n) fetch(r + 1);
       }
@@ -218,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       if (r < n || stop) mbar_wait(k_full + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
     for (int64_t r = t - 1; lane == 0 && r >= 0 && r >= t - kQStages; --r)
       mbar_wait(q_full + 8 * static_cast<int>(r % kQStages), static_cast<uint32_t>((r / kQStages) & 1));
-  } else if (warp == 16) {
+  } else if (warp == 8) {
     // ---------------- MMA issuer: the warp decides, one lane issues ----------------
     constexpr uint32_t kTileDesc = G::kTileBytes >> 4, kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
     const uint32_t k_lo = smem_u32(base) >> 4, q_lo = smem_u32(q_ring) >> 4;
@@ -263,8 +255,8 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     for (int64_t r = n - 1; r >= 0 && r >= n - 2; --r)
       mbar_wait(k_empty + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
   } else {
-    // ---------------- stream x: half `hf` of the rows of a slot per thread ----------------
-    const int x = warp >> 3, hf = (warp >> 2) & 1, r0 = (warp & 3) * 32 + lane;
+    // ---------------- stream x: a slot per thread ----------------
+    const int x = warp >> 2, r0 = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float c = p.inv_scale * kLog2e;
     const uint64_t c2 = pair(c, c);
@@ -280,46 +272,47 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         fence_after();
         const int64_t lim0 = p.causal ? static_cast<int64_t>(it.q.len) - it.q.n + r * tt + 1 : it.q.len;
         const bool masked = lim0 < k0 + (x + 1) * kSlots || it.q.n - r * tt < tt;
-        const float4* zs = reinterpret_cast<const float4*>(z_ring + s * kRows + hf * 64);
-        const uint32_t ta = tmem + lane_base + (2 * x + sb) * 128 + hf * 64;
+        const float4* zs = reinterpret_cast<const float4*>(z_ring + s * kRows);
+        const uint32_t ta = tmem + lane_base + (2 * x + sb) * 128;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint64_t sums[2] = {0, 0};
         uint32_t v[2][32];
         tmem_ld32_async(ta, v[0]);
 #pragma unroll
-        for (int q4 = 0; q4 < 2; ++q4) {
+        for (int q4 = 0; q4 < 4; ++q4) {
           tmem_wait();
-          if (q4 == 0) tmem_ld32_async(ta + 32, v[1]);
+          if (q4 < 3) tmem_ld32_async(ta + 32 * (q4 + 1), v[(q4 + 1) & 1]);
           if (!masked) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float4 z = zs[q4 * 8 + j];
               float e0, e1, e2, e3;
               unpair(fma_pair(pair(__uint_as_float(v[q4 & 1][4 * j]), __uint_as_float(v[q4 & 1][4 * j + 1])), c2,
-                              pair(z.x, z.y)), e0, e1);
+                              pair(-z.x, -z.y)), e0, e1);
               unpair(fma_pair(pair(__uint_as_float(v[q4 & 1][4 * j + 2]), __uint_as_float(v[q4 & 1][4 * j + 3])), c2,
-                              pair(z.z, z.w)), e2, e3);
+                              pair(-z.z, -z.w)), e2, e3);
               if (j % 2 == 0) {                            // a quarter of the exponentials off the MUFU
                 exp2_pair(e0, e1);
               } else {
                 e0 = ex2_approx(e0);
                 e1 = ex2_approx(e1);
               }
-              sums[0] = add_pair(sums[0], pair(e0, e1));
-              sums[1] = add_pair(sums[1], pair(ex2_approx(e2), ex2_approx(e3)));
+              sum[0] += e0;
+              sum[1] += e1;
+              sum[2] += ex2_approx(e2);
+              sum[3] += ex2_approx(e3);
             }
           } else {
             // a row of token a sees the slot from token `from` on
-            const uchar4* ts = reinterpret_cast<const uchar4*>(row_token + hf * 64);
+            const short4* ts = reinterpret_cast<const short4*>(row_token);
             const int from = p.causal ? slot - (it.q.len - it.q.n) - r * tt : -1, tokens = min(tt, it.q.n - r * tt);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float4 z = zs[q4 * 8 + j];
-              const uchar4 a = ts[q4 * 8 + j];
-              const float e0 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j]), c, z.x));
-              const float e1 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 1]), c, z.y));
-              const float e2 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 2]), c, z.z));
-              const float e3 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 3]), c, z.w));
+              const short4 a = ts[q4 * 8 + j];
+              const float e0 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j]), c, -z.x));
+              const float e1 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 1]), c, -z.y));
+              const float e2 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 2]), c, -z.z));
+              const float e3 = ex2_approx(fmaf(__uint_as_float(v[q4 & 1][4 * j + 3]), c, -z.w));
               sum[0] += a.x >= from && a.x < tokens ? e0 : 0.f;
               sum[1] += a.y >= from && a.y < tokens ? e1 : 0.f;
               sum[2] += a.z >= from && a.z < tokens ? e2 : 0.f;
@@ -327,11 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
             }
           }
         }
-        {
-          float a, b;
-          unpair(add_pair(sums[0], sums[1]), a, b);
-          total += (a + b) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-        }
+        total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -340,26 +329,17 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         }
         __syncwarp();
       }
-      // one half after the other, so that the order of the additions is fixed
-      const uint32_t turn = added + 8 * (static_cast<int>(n % 3) * 8 + x * 4 + (warp & 3));
-      if (hf) wait(turn, static_cast<uint32_t>((n / 3) & 1));
-      __syncwarp();
       if (slot < it.q.len) {
         int page, row;
         page_of(p.c, slot, page, row);
         const int64_t pg = physical_page(p.c, p.c.table, p.c.table_stride, it.seq, page);
         if (pg >= 0) atomicAdd(&p.c.w[pg * p.c.w_sp + row * p.c.w_sn + head * p.c.w_sh], total);
       }
-      if (!hf) {
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(turn);
-      }
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 8) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
