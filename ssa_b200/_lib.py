@@ -195,3 +195,23 @@ def check(fn: str, code: int) -> None:
     if code != 0:
         detail = lib().ssa_last_error().decode(errors="replace")
         raise SSAError(fn, code, detail)
+
+
+_call = None
+
+
+def paged_call():
+    """The extension module of the paged ops' argument path, bound to the library
+    (raises if it is absent, as :func:`lib` does)."""
+    global _call
+    if _call is None:
+        handle = lib()
+        path = os.path.join(HERE, "_paged_call.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `python -m ssa_b200.build`")
+        from . import _paged_call as module
+
+        module.bind(*(ctypes.cast(getattr(handle, f), _vp).value for f in (
+            "ssa_paged_append", "ssa_paged_attn_workspace_size", "ssa_paged_attn", "ssa_paged_evict")))
+        _call = module
+    return _call

@@ -111,16 +111,20 @@ def _cache_args(k_pages, v_pages, page_table, kv_lens, weights, op):
     return key, c, sync, (page_table, kv_lens)
 
 
+def _finish(key, sync, name, code):
+    if code:
+        L.check(name, code)
+    if sync:
+        S.host_word_done(torch.device("cuda", key))
+
+
 def _call(key, sync, fn, *args):
     if torch.cuda.current_device() == key:
         code = fn(*args, _raw_stream(key))
     else:
         with torch.cuda.device(key):
             code = fn(*args, _raw_stream(key))
-    if code:
-        L.check(fn.__name__, code)
-    if sync:
-        S.host_word_done(torch.device("cuda", key))
+    _finish(key, sync, fn.__name__, code)
 
 
 # One workspace per (device, stream), kept: calls on a stream follow one another.
@@ -158,6 +162,13 @@ def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
         weights: optional ``[num_pages, page_size, h_kv]`` float32 slot weights;
             those of the written slots become 0.
     """
+    if k_pages.is_cuda:
+        # the plain case in one step; whatever it does not take is looked at below
+        key = k_pages.get_device()
+        word, sync = S.host_word(key, _APPEND)
+        code = L.paged_call().append(k_new, v_new, k_pages, v_pages, page_table, q_starts, kv_lens, weights, word)
+        if code is not None:
+            return _finish(key, sync, "ssa_paged_append", code)
     key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _APPEND)
     dtype, shape = k_pages.dtype, k_new.shape
     k_new = _check_rows(k_new, "k_new", key, dtype, shape)
@@ -196,6 +207,17 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     sees no slot gets zeros (and ``-inf``).  Rows outside ``q_starts`` are not
     written.
     """
+    if k_pages.is_cuda:
+        key = k_pages.get_device()
+        ws = S.workspaces.get((key, _raw_stream(key)))
+        if ws is not None and not torch.cuda.is_current_stream_capturing():
+            word, sync = S.host_word(key, _ATTEND)
+            done = L.paged_call().attend(q, k_pages, v_pages, page_table, q_starts, kv_lens, scale, is_causal, weights,
+                                         return_lse, word, ws)
+            if done is not None:
+                code, out, lse = done
+                _finish(key, sync, "ssa_paged_attn", code)
+                return (out, lse) if return_lse else out
     key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
     shape = q.shape
     q = _check_rows(q, "q", key, k_pages.dtype, shape)
@@ -234,8 +256,16 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     """
     if weights is None:
         raise ValueError("weights is needed: eviction ranks slots by them")
-    key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
     budget, recent = int(budget), int(recent)
+    if k_pages.is_cuda:
+        key = k_pages.get_device()
+        word, sync = S.host_word(key, _EVICT)
+        done = L.paged_call().evict(k_pages, v_pages, weights, page_table, kv_lens, new_table, budget, recent, word)
+        if done is not None:
+            code, kept, new_lens = done
+            _finish(key, sync, "ssa_paged_evict", code)
+            return kept, new_lens
+    key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
     if budget < 1 or not 0 <= recent <= budget:
         raise ValueError(f"budget {budget}, recent {recent}: need budget >= 1 and 0 <= recent <= budget")
     new_table = _table(new_table, "new_table", key, c.batch)
