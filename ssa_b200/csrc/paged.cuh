@@ -224,23 +224,52 @@ struct TileCosts {
     const uint32_t y = a * m + b;
     return sum + (a && y >= k ? floor_sum(y / k, a, k, y % k) : 0);
   }
-  // The tile that unit u (of the sequence's units of one head) lies in, and the
-  // units before it: a 32-way search by a full warp.
-  __device__ int find(int64_t u, int64_t& first) const {
-    const int lane = threadIdx.x & 31;
-    int lo = 0, width = tiles;                 // the tile is in [lo, lo + width)
-    first = 0;
-    while (width > 1) {
-      const int step = (width + 31) / 32, t = lo + lane * step;
-      const int64_t b = lane * step < width ? before(t) : u + 1;
-      const int hit = 31 - __clz(__ballot_sync(0xffffffffu, b <= u));
-      first = __shfl_sync(0xffffffffu, b, hit);
-      width = min(step, lo + width - (lo + hit * step));
-      lo += hit * step;
-    }
-    return lo;
+};
+
+// The same with the parts exchanged, for the slot weights: a tile is `kt` slots,
+// its units the row tiles (of `tt` tokens) that hold a row that sees one of them.
+struct SlotCosts {
+  int n, len, tt, kt, more, causal, row_tiles, tiles;
+  __host__ __device__ SlotCosts(int n_, int len_, int tt_, int kt_, int extra, int causal_)
+      : n(n_), len(len_), tt(tt_), kt(kt_), more(extra), causal(causal_),
+        row_tiles(static_cast<int>((static_cast<uint32_t>(n_) + tt_ - 1) / static_cast<uint32_t>(tt_))),
+        tiles(n_ > 0 ? static_cast<int>((static_cast<uint32_t>(len_) + kt_ - 1) / static_cast<uint32_t>(kt_)) : 0) {}
+  // first token that sees the tile (below n: the tile begins below len)
+  __host__ __device__ int first_token(int i) const {
+    const int64_t t = static_cast<int64_t>(i) * kt - (static_cast<int64_t>(len) - n);
+    return causal && t > 0 ? static_cast<int>(t) : 0;
+  }
+  __host__ __device__ int first_row_tile(int i) const {
+    return static_cast<int>(static_cast<uint32_t>(first_token(i)) / static_cast<uint32_t>(tt));
+  }
+  __host__ __device__ int units(int i) const { return row_tiles - first_row_tile(i) + more; }
+  // units of tiles 0 .. i-1
+  __host__ __device__ int64_t before(int i) const {
+    const int64_t all = static_cast<int64_t>(i) * (row_tiles + more), old = static_cast<int64_t>(len) - n;
+    if (!causal) return all;
+    // tiles from `from` on miss floor((their first slot - old) / tt) row tiles
+    const int from = old > 0 ? static_cast<int>((old + kt - 1) / kt) : 0;
+    return i > from ? all - floor_sum(i - from, tt, kt, static_cast<uint32_t>(static_cast<int64_t>(from) * kt - old)) : all;
   }
 };
+
+// The tile that unit u (of a sequence's units of one head) lies in, and the
+// units before it: a 32-way search by a full warp.
+template <typename Costs>
+__device__ inline int find_tile(const Costs& t, int64_t u, int64_t& first) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, width = t.tiles;                 // the tile is in [lo, lo + width)
+  first = 0;
+  while (width > 1) {
+    const int step = (width + 31) / 32;
+    const int64_t b = lane * step < width ? t.before(lo + lane * step) : u + 1;
+    const int hit = 31 - __clz(__ballot_sync(0xffffffffu, b <= u));
+    first = __shfl_sync(0xffffffffu, b, hit);
+    width = min(step, lo + width - (lo + hit * step));
+    lo += hit * step;
+  }
+  return lo;
+}
 
 // A CTA's walk over its units: the current item, and the unit in it.
 struct PagedWalk {
@@ -254,6 +283,7 @@ struct PagedWalk {
 // Total units, and the walk of CTA `cta` of `grid`; little work is shared by
 // fewer CTAs, of `least` units each.  Called by one full warp; every lane gets
 // the result.  False: no work.
+template <typename Costs = TileCosts>
 __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, int extra, int least, int64_t cta, int64_t grid,
                                       PagedWalk& w) {
   const int lane = threadIdx.x & 31;
@@ -263,7 +293,7 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
   int64_t mine = 0, cost_first = 0;
   for (int s = lane; s < p.c.batch; s += 32) {
     const PagedSeq q = paged_seq(p.c, p.q_starts, p.rows, s);
-    const TileCosts t(q.n, q.len, tt, kt, extra, p.causal);
+    const Costs t(q.n, q.len, tt, kt, extra, p.causal);
     const int64_t cost = t.before(t.tiles) * hk;
     if (s < 32) {
       q_first = q;
@@ -288,7 +318,7 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
     PagedSeq q = q_first;
     if (s0 > 0 && s < p.c.batch) {
       q = paged_seq(p.c, p.q_starts, p.rows, s);
-      const TileCosts t(q.n, q.len, tt, kt, extra, p.causal);
+      const Costs t(q.n, q.len, tt, kt, extra, p.causal);
       cost = t.before(t.tiles) * hk;
     }
     int64_t incl = cost;
@@ -306,11 +336,11 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
       w.n = __shfl_sync(0xffffffffu, q.n, src);
       w.len = __shfl_sync(0xffffffffu, q.len, src);
       w.q0 = __shfl_sync(0xffffffffu, q.q0, src);
-      const TileCosts t(w.n, w.len, tt, kt, extra, p.causal);
+      const Costs t(w.n, w.len, tt, kt, extra, p.causal);
       const int64_t per = t.before(t.tiles), off = w.u - first;
       w.head = static_cast<int>(mul_div(off, 1, per));
       int64_t in_tiles;
-      w.tile = t.find(off - w.head * per, in_tiles);
+      w.tile = find_tile(t, off - w.head * per, in_tiles);
       w.item_first = first + w.head * per + in_tiles;
       w.units = t.units(w.tile);
       return true;
@@ -322,9 +352,10 @@ __device__ inline bool paged_schedule(const PagedAttnParams& p, int tt, int kt, 
 
 // The item after the current one (w.u is its first unit).  Every lane of a
 // warp, or a single thread, may call it: no exchange between lanes.
+template <typename Costs = TileCosts>
 __device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt, int extra, PagedWalk& w) {
   w.item_first += w.units;
-  TileCosts t(w.n, w.len, tt, kt, extra, p.causal);
+  Costs t(w.n, w.len, tt, kt, extra, p.causal);
   if (++w.tile >= t.tiles) {
     w.tile = 0;
     if (++w.head >= p.c.h_kv) {
@@ -335,8 +366,8 @@ __device__ inline void paged_next_item(const PagedAttnParams& p, int tt, int kt,
         w.n = q.n;
         w.len = q.len;
         w.q0 = q.q0;
-      } while (w.n == 0);
-      t = TileCosts(w.n, w.len, tt, kt, extra, p.causal);
+        t = Costs(w.n, w.len, tt, kt, extra, p.causal);
+      } while (t.tiles == 0);
     }
   }
   w.units = t.units(w.tile);
@@ -348,10 +379,11 @@ struct PagedStart {
   PagedWalk w;
   int any;
 };
+template <typename Costs = TileCosts>
 __device__ inline void paged_start(const PagedAttnParams& p, int tt, int kt, int extra, int least, PagedStart* shared) {
   if (threadIdx.x < 32) {
     PagedWalk w{};
-    const bool any = paged_schedule(p, tt, kt, extra, least, blockIdx.x, gridDim.x, w);
+    const bool any = paged_schedule<Costs>(p, tt, kt, extra, least, blockIdx.x, gridDim.x, w);
     if (threadIdx.x == 0) {
       shared->w = w;
       shared->any = any;
@@ -385,10 +417,11 @@ __device__ __forceinline__ PagedSegment paged_segment(const PagedWalk& w, int ex
   return s;
 }
 // To the first unit past the current item; false if that is not this CTA's.
+template <typename Costs = TileCosts>
 __device__ __forceinline__ bool paged_advance(const PagedAttnParams& p, int tt, int kt, int extra, PagedWalk& w) {
   w.u = w.item_first + w.units;
   if (w.u >= w.end) return false;
-  paged_next_item(p, tt, kt, extra, w);
+  paged_next_item<Costs>(p, tt, kt, extra, w);
   return true;
 }
 

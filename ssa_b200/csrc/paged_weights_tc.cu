@@ -5,17 +5,19 @@
 //
 // with lse2_i from the attention kernel.  The scores are made again, transposed:
 // S^T = K Q^T puts a slot in every TMEM lane and the rows in its columns, so
-// the sum over rows is a thread's own, with no exchange between lanes and no
-// atomics between CTAs: one CTA has all rows of its slots, in one order.
+// the sum over rows is a thread's own, with no exchange between lanes.
 //
 // An item is 256 slots of one (sequence, KV head): two streams of 128 slots
 // share every tile of Q rows (the g heads of a group at floor(128 / g) tokens).
+// The row tiles of all items are shared out evenly (SlotCosts, paged.cuh); the
+// slot sums of an item that is cut are joined by the last of its CTAs, in CTA order.
 // Per row tile and stream the tensor cores do 128 x 128 x d products, the MUFU
 // 128 x 128 exponentials, which bound it (1024 clocks against 512 at d = 128);
 // a quarter of them is made on the FMA pipe instead (4% faster; a half, no more).
-// 2 x 1024 tokens x 32 heads over 8192 slots, bf16: 235 us, 550 TFLOP/s; the last
-// of that call's 512 items leave SMs idle for a fifth of it.  Two threads a slot
-// (16 warps) took the same time.
+// 2 x 1024 tokens x 32 heads over 8192 slots, bf16: 214 us, 600 TFLOP/s (whole
+// items in turn: 235; 4 x 1618 tokens x 8 heads of 64 over 3529: 12% of the call
+// gained; items of two row tiles lose 5% by the join).  Two threads a slot (16
+// warps) took the same time.
 //
 //   warps 0-3, 4-7  streams: a slot per thread; scores from TMEM, two buffers each
 //   warp 8          TMEM allocation, single-thread MMA issue
@@ -39,47 +41,23 @@ using namespace tc;
 constexpr int kSlots = 128;        // of a stream
 constexpr int kRows = 128;         // of a Q tile
 constexpr int kThreads = 320;
+constexpr int kGrid = 148;
+constexpr int kExtra = 2;          // units an item costs besides its row tiles
+constexpr int kLeast = 1;          // units a CTA takes at least
+static_assert(kGrid * 8 * 4 <= SSA_PAGED_ZEROED, "a counter for every warp of the streams of a CTA");
 constexpr int kQStages = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
 struct Geo {
   static constexpr int kTileBytes = 128 * D * 2;
-  static constexpr size_t kSmem = 1024 + (4 + kQStages) * static_cast<size_t>(kTileBytes) + kQStages * kRows * 4 + kRows * 2 + 192;
+  static constexpr size_t kSmem = 1024 + (4 + kQStages) * static_cast<size_t>(kTileBytes) + kQStages * kRows * 4 + kRows * 2 + 160 + sizeof(PagedStart);
 };
 
 struct QueryMap {
   int tokens;                      // per Q tile
   int head_first;                  // row r of a tile: token r / g, head r % g; else token r % tokens, head r / tokens
 };
-
-// Item i of the call: 256 slots of a (sequence, KV head).  Items of a sequence
-// run tile by tile, heads inside, later tiles (seen by fewer rows) last.
-struct Items {
-  int64_t base;                    // items of the sequences before `seq`
-  int seq;
-  PagedSeq q;
-};
-__device__ __forceinline__ int64_t items_of(const PagedAttnParams& p, const PagedSeq& q) {
-  return q.n > 0 ? static_cast<int64_t>((q.len + 2 * kSlots - 1) / (2 * kSlots)) * p.c.h_kv : 0;
-}
-__device__ __forceinline__ bool seek(const PagedAttnParams& p, Items& it, int64_t i) {
-  while (it.seq < p.c.batch) {
-    if (it.seq >= 0) {
-      const int64_t n = items_of(p, it.q);
-      if (i < it.base + n) return true;
-      it.base += n;
-    }
-    if (++it.seq < p.c.batch) it.q = paged_seq(p.c, p.q_starts, p.rows, it.seq);
-  }
-  return false;
-}
-// First token of the sequence that sees slot k0 (q.n if none does).
-__device__ __forceinline__ int first_token(const PagedAttnParams& p, const PagedSeq& q, int k0) {
-  if (!p.causal) return 0;
-  const int64_t t = static_cast<int64_t>(k0) - (static_cast<int64_t>(q.len) - q.n);
-  return t < 0 ? 0 : t > q.n ? q.n : static_cast<int>(t);
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -98,6 +76,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
   const uint32_t s_full = q_empty + 8 * kQStages, s_empty = s_full + 32;     // [stream][buffer]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 2 * kQStages + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 4 + 2 * kQStages + 10);
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int g = p.group, tt = qm.tokens;
 
@@ -131,6 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  paged_start<SlotCosts>(p, tt, 2 * kSlots, kExtra, kLeast, &start);
   fence_before();
   __syncthreads();
   fence_after();
@@ -142,10 +122,20 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       paged_error(p.c, SSA_DEVICE_TIMEOUT);
     }
   };
-  Items it{0, -1, {0, 0, 0}};
+  PagedWalk w = start.w;
+  const bool any = start.any;
+  auto advance = [&]() { return paged_advance<SlotCosts>(p, tt, 2 * kSlots, kExtra, w); };
+  // the current item's part of this CTA: row tiles [first, last)
+  auto row_tiles = [&]() {
+    PagedSegment s = paged_segment(w, kExtra);
+    const int r0 = SlotCosts(w.n, w.len, tt, 2 * kSlots, kExtra, p.causal).first_row_tile(w.tile);
+    s.first += r0;
+    s.last += r0;
+    return s;
+  };
   int64_t t = 0, n = 0;                                  // Q tiles and items so far
 
-  if (warp == 9) {
+  if (any && warp == 9) {
     // ---------------- producer ----------------
     const int piece_rows = min(p.c.page_size, kSlots), pieces = kSlots / piece_rows, boxes = pieces * (D / 64);
     const int piece = lane & (pieces - 1), half = lane / pieces;
@@ -161,9 +151,10 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     }
     const uint32_t q_bytes = static_cast<uint32_t>(tt * g) * 128 * (D / 64);
     bool stop = false;
-    for (int64_t i = blockIdx.x; !stop && seek(p, it, i); i += gridDim.x, ++n) {
-      const int head = static_cast<int>((i - it.base) % p.c.h_kv);
-      const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots;
+    for (bool going = true; going && !stop; going = !stop && advance()) {
+      const PagedSegment seg = row_tiles();
+      if (seg.first == seg.last) continue;
+      const int head = w.head, k0 = w.tile * 2 * kSlots;
       const int b = static_cast<int>(n & 1);
       wait(k_empty + 8 * b, static_cast<uint32_t>((n >> 1) & 1) ^ 1u);
       stop = __any_sync(0xffffffffu, *abort_flag);
@@ -173,24 +164,23 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
 #pragma unroll
       for (int x = 0; x < 2; ++x)
         if (lane < boxes) {
-          const PageSpot at = page_spot(p.c, it.seq, k0 + x * kSlots + piece * piece_rows, it.q.len);
+          const PageSpot at = page_spot(p.c, w.seq, k0 + x * kSlots + piece * piece_rows, w.len);
           tma_load_4d(smem_u32(base) + (2 * b + x) * G::kTileBytes + half * (kSlots * 128) + piece * piece_rows * 128,
                       &kmap, half * 64, mo.head_first ? head : at.row, mo.head_first ? at.row : head, at.page,
                       k_full + 8 * b);
         }
       // lse2 of the next tile's rows is on its way while this tile's ring entry
       // is waited for
-      int r = first_token(p, it.q, k0) / tt;
       float z[4];
       auto fetch = [&](int tile) {
-        const int64_t tok = it.q.q0 + static_cast<int64_t>(tile) * tt;
-        const int tokens = min(tt, it.q.n - tile * tt);
+        const int64_t tok = w.q0 + static_cast<int64_t>(tile) * tt;
+        const int tokens = min(tt, w.n - tile * tt);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           z[e] = row_tok[e] < tokens ? __ldg(p.lse2 + (tok + row_tok[e]) * h_q + head * g + row_head[e]) : INFINITY;
       };
-      if (r * tt < it.q.n) fetch(r);
-      for (; r * tt < it.q.n; ++r, ++t) {
+      fetch(seg.first);
+      for (int r = seg.first; r < seg.last; ++r, ++t) {
         const int s = static_cast<int>(t % kQStages);
         wait(q_empty + 8 * s, static_cast<uint32_t>((t / kQStages) & 1) ^ 1u);
         stop = __any_sync(0xffffffffu, *abort_flag);
@@ -198,32 +188,32 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         if (lane == 0) mbar_expect_tx(q_full + 8 * s, q_bytes);
         __syncwarp();
         if (lane < D / 64) {
-          const int y = head * g, zc = static_cast<int>(it.q.q0) + r * tt;
+          const int y = head * g, zc = static_cast<int>(w.q0) + r * tt;
           tma_load_3d(smem_u32(q_ring + s * G::kTileBytes) + lane * (kRows * 128), &qmap, lane * 64,
                       qm.head_first ? y : zc, qm.head_first ? zc : y, q_full + 8 * s);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) z_ring[s * kRows + lane + 32 * e] = z[e];   // exp2(s - inf) = 0 where there is no row
         mbar_arrive(q_full + 8 * s);
-        if ((r + 1) * tt < it.q.n) fetch(r + 1);
+        if (r + 1 < seg.last) fetch(r + 1);
       }
+      ++n;
     }
     // every issued copy lands before the CTA exits
-    for (int64_t r = n - (stop ? 0 : 1); lane == 0 && r >= 0 && r >= n - 2; --r)
-      if (r < n || stop) mbar_wait(k_full + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
+    for (int64_t r = n - 1; lane == 0 && r >= 0 && r >= n - 2; --r) mbar_wait(k_full + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
     for (int64_t r = t - 1; lane == 0 && r >= 0 && r >= t - kQStages; --r)
       mbar_wait(q_full + 8 * static_cast<int>(r % kQStages), static_cast<uint32_t>((r / kQStages) & 1));
-  } else if (warp == 8) {
+  } else if (any && warp == 8) {
     // ---------------- MMA issuer: the warp decides, one lane issues ----------------
     constexpr uint32_t kTileDesc = G::kTileBytes >> 4, kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
     const uint32_t k_lo = smem_u32(base) >> 4, q_lo = smem_u32(q_ring) >> 4;
     auto desc = [](uint32_t lo) { return (static_cast<uint64_t>(kDescHi) << 32) | (lo & 0x3fffu); };
     int s = 0;
     uint32_t qpar = 0;
-    for (int64_t i = blockIdx.x; !__any_sync(0xffffffffu, *abort_flag) && seek(p, it, i); i += gridDim.x, ++n) {
-      const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots;
-      const int b = static_cast<int>(n & 1), r0 = first_token(p, it.q, k0) / tt;
-      const int tiles = __shfl_sync(0xffffffffu, max((it.q.n + tt - 1) / tt - r0, 0), 0);
+    for (bool going = true; going && !__any_sync(0xffffffffu, *abort_flag); going = advance()) {
+      const PagedSegment seg = row_tiles();
+      const int b = static_cast<int>(n & 1), tiles = __shfl_sync(0xffffffffu, seg.last - seg.first, 0);
+      if (tiles == 0) continue;
       wait(k_full + 8 * b, static_cast<uint32_t>((n >> 1) & 1));
       for (int j = 0; j < tiles; ++j, ++t) {
         const int sb = static_cast<int>(t & 1);
@@ -252,29 +242,32 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
       }
       if (elect_one()) mma_commit(k_empty + 8 * b);
       __syncwarp();
+      ++n;
     }
     // the last commits arrive once every MMA is done; both buffers of K are
     // then free (an item's k_empty is its n-th phase)
     for (int64_t r = n - 1; r >= 0 && r >= n - 2; --r)
       mbar_wait(k_empty + 8 * static_cast<int>(r & 1), static_cast<uint32_t>((r >> 1) & 1));
-  } else {
+  } else if (any) {
     // ---------------- stream x: a slot per thread ----------------
     const int x = warp >> 2, r0 = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float c = p.inv_scale * kLog2e;
     const uint64_t c2 = pair(c, c);
-    for (int64_t i = blockIdx.x; !__any_sync(0xffffffffu, *abort_flag) && seek(p, it, i); i += gridDim.x, ++n) {
-      const int head = static_cast<int>((i - it.base) % p.c.h_kv);
-      const int k0 = static_cast<int>((i - it.base) / p.c.h_kv) * 2 * kSlots, slot = k0 + x * kSlots + r0;
+    bool going = true;
+    for (int second = 0; going && !__any_sync(0xffffffffu, *abort_flag); second = 1, going = advance()) {
+      const PagedSegment seg = row_tiles();
+      if (seg.first == seg.last) continue;
+      const int k0 = w.tile * 2 * kSlots, slot = k0 + x * kSlots + r0;
       float total = 0.f;
-      for (int r = first_token(p, it.q, k0) / tt; r * tt < it.q.n; ++r, ++t) {
+      for (int r = seg.first; r < seg.last; ++r, ++t) {
         const int s = static_cast<int>(t % kQStages), sb = static_cast<int>(t & 1);
         wait(q_full + 8 * s, static_cast<uint32_t>((t / kQStages) & 1));   // lse2 of the rows
         wait(s_full + 8 * (2 * x + sb), static_cast<uint32_t>((t >> 1) & 1));
         __syncwarp();
         fence_after();
-        const int64_t lim0 = p.causal ? static_cast<int64_t>(it.q.len) - it.q.n + r * tt + 1 : it.q.len;
-        const bool masked = lim0 < k0 + (x + 1) * kSlots || it.q.n - r * tt < tt;
+        const int64_t lim0 = p.causal ? static_cast<int64_t>(w.len) - w.n + r * tt + 1 : w.len;
+        const bool masked = lim0 < k0 + (x + 1) * kSlots || w.n - r * tt < tt;
         const float4* zs = reinterpret_cast<const float4*>(z_ring + s * kRows);
         const uint32_t ta = tmem + lane_base + (2 * x + sb) * 128;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -307,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
           } else {
             // a row of token a sees the slot from token `from` on
             const short4* ts = reinterpret_cast<const short4*>(row_token);
-            const int from = p.causal ? slot - (it.q.len - it.q.n) - r * tt : -1, tokens = min(tt, it.q.n - r * tt);
+            const int from = p.causal ? slot - (w.len - w.n) - r * tt : -1, tokens = min(tt, w.n - r * tt);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float4 z = zs[q4 * 8 + j];
@@ -332,11 +325,35 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         }
         __syncwarp();
       }
-      if (slot < it.q.len) {
+      bool mine = true;
+      if (!seg.whole) {
+        // a warp's slots are joined by the last of the item's CTAs, in CTA order
+        // (the counter is zero before the launch and after it)
+        const int a = unit_cta(w, w.item_first + kExtra), parts = unit_cta(w, w.item_first + w.units - 1) - a + 1;
+        const int at = x * kSlots + r0;
+        p.part[(2 * blockIdx.x + second) * 2 * kSlots + at] = total;
+        __threadfence();
+        __syncwarp();
+        int counted = 0;
+        if (lane == 0) {
+          counted = atomicAdd(p.counters + a * 8 + warp, 1);
+          if (counted == parts - 1) p.counters[a * 8 + warp] = 0;
+        }
+        mine = __shfl_sync(0xffffffffu, counted, 0) == parts - 1;
+        if (mine) {
+          __threadfence();
+          // the item is the second of CTA a's two parts if a's share starts before it
+          const int in_a = mul_div(a, w.total, w.ctas) < w.item_first ? 1 : 0;
+          total = 0.f;
+          for (int i = 0; i < parts; ++i)
+            total += __ldcg(p.part + (2 * (a + i) + (i == 0 ? in_a : 0)) * 2 * kSlots + at);
+        }
+      }
+      if (mine && slot < w.len) {
         int page, row;
         page_of(p.c, slot, page, row);
-        const int64_t pg = physical_page(p.c, p.c.table, p.c.table_stride, it.seq, page);
-        if (pg >= 0) atomicAdd(&p.c.w[pg * p.c.w_sp + row * p.c.w_sn + head * p.c.w_sh], total);
+        const int64_t pg = physical_page(p.c, p.c.table, p.c.table_stride, w.seq, page);
+        if (pg >= 0) atomicAdd(&p.c.w[pg * p.c.w_sp + row * p.c.w_sn + w.head * p.c.w_sh], total);
       }
     }
   }
@@ -384,7 +401,7 @@ cudaError_t launch_t(const PagedAttnParams& p, ssa_dtype dt, cudaStream_t st) {
   static SmemOptIn opt_in;
   const cudaError_t e = opt_in(reinterpret_cast<const void*>(kern), Geo<D>::kSmem);
   if (e != cudaSuccess) return e;
-  return launch_after(kern, dim3(148), dim3(kThreads), Geo<D>::kSmem, st, km, qm, p, mo, qo);
+  return launch_after(kern, dim3(kGrid), dim3(kThreads), Geo<D>::kSmem, st, km, qm, p, mo, qo);
 }
 
 }  // namespace pwt
