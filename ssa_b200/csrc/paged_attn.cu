@@ -8,7 +8,10 @@
 // (s * log2 e is folded into q when it is loaded).  One CTA holds a tile of R
 // query rows (the g heads of a KV group at R / g consecutive tokens) and walks
 // key tiles of 64 slots: 256 threads form a 16 x 16 grid, a thread owns R / 16
-// rows and every 16th key (scores) or column quad (output).  Bound by shared-memory
+// rows and every 16th key (scores) or column quad (output).  A warp none of whose
+// rows exists only loads: it would take its share of shared memory's bandwidth
+// (16 tokens x 32 heads of 128 over 4000 slots, fp32: 325 us with it, 145 without,
+// 3.6 TB/s).  Bound by shared-memory
 // loads and FMAs, 4 R 64 d flops a tile; small calls by latency.  fp32, 3 chunks of
 // up to 129 tokens x 8 heads of 64 over up to 1500 slots: 29 us and 6 us for the join.
 #include <type_traits>
@@ -158,6 +161,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
     const PagedSegment seg = paged_segment(w, kExtra);
     if (seg.first == seg.last) continue;
     const TileRows t = tile_rows(w, tt, p.group);
+    const bool live = tid / kWarp * 2 < t.rows;                // the warp has a row (its first is row 2 * warp)
     const int tile_min = seen_slots(p, w.n, w.len, t.tok0);                              // every row sees these
     const int tile_max = seen_slots(p, w.n, w.len, t.tok0 + t.rows / p.group - 1);       // some row sees these
     __syncthreads();
@@ -193,9 +197,9 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
       cp_wait<1>();                                          // the keys
       __syncthreads();
       float s[RI][4];
-      scores<RI>(qs, ks, d, G::QS, tx, ty, s);
+      if (live) scores<RI>(qs, ks, d, G::QS, tx, ty, s);
 #pragma unroll
-      for (int i = 0; i < RI; ++i) {
+      for (int i = 0; live && i < RI; ++i) {
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -236,7 +240,9 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
           for (int e = 0; e < 8; ++e) odd |= !isfinite(vrow[x + e]);
         odd = __syncthreads_or(odd);
       }
-      if (!odd) {
+      if (!live) {
+        // nothing to add
+      } else if (!odd) {
 #pragma unroll 2
         for (int j = 0; j < kKT; j += 4) {
           float4 pr[RI];
