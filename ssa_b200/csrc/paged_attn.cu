@@ -11,9 +11,13 @@
 // rows and every 16th key (scores) or column quad (output).  A warp none of whose
 // rows exists only loads: it would take its share of shared memory's bandwidth
 // (16 tokens x 32 heads of 128 over 4000 slots, fp32: 325 us with it, 145 without,
-// 3.6 TB/s).  Bound by shared-memory
-// loads and FMAs, 4 R 64 d flops a tile; small calls by latency.  fp32, 3 chunks of
-// up to 129 tokens x 8 heads of 64 over up to 1500 slots: 29 us and 6 us for the join.
+// 3.6 TB/s).
+//
+// Tiles of 64 rows are bound by what shared memory returns: a step of four columns
+// is 64 FMAs a thread, 16 clocks of the SM for every warp, and eight 16-byte loads, 32
+// clocks.  fp32, 6 x 191 tokens x 28 heads of 128 over 4430 slots: 2.36 ms, 30
+// TFLOP/s.  Small calls are bound by latency: 3 chunks of up to 129 tokens x 8 heads of
+// 64 over up to 1500 slots take 29 us and 6 us for the join.
 #include <type_traits>
 
 #include "common.cuh"
@@ -70,6 +74,7 @@ __device__ __forceinline__ void scores(const float* qs, const float* ks, int d, 
   for (int i = 0; i < RI; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 2
   for (int x = 0; x < d; x += 4) {
     float4 a[RI], b[4];
 #pragma unroll
@@ -243,7 +248,7 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(PagedAttnParams p) 
       if (!live) {
         // nothing to add
       } else if (!odd) {
-#pragma unroll 2
+#pragma unroll 4
         for (int j = 0; j < kKT; j += 4) {
           float4 pr[RI];
 #pragma unroll
@@ -465,6 +470,18 @@ cudaError_t launch_weights_simt(const PagedAttnParams& p, ssa_dtype dt, cudaStre
   });
 }
 
+// CTAs of the CUDA-core kernel that an SM's shared memory holds, two at most (a
+// share of the work for more than are resident cost 3% to 6%).
+int simt_resident(int rows, int d) {
+  auto bytes = [&](auto size) {
+    constexpr int DP = decltype(size)::value;
+    return rows == 64 ? SimtGeo<64, DP>::kSmem : rows == 32 ? SimtGeo<32, DP>::kSmem : SimtGeo<16, DP>::kSmem;
+  };
+  const size_t one = d <= 64 ? bytes(std::integral_constant<int, 64>{})
+                     : d <= 128 ? bytes(std::integral_constant<int, 128>{}) : bytes(std::integral_constant<int, 256>{});
+  return 2 * (one + 2048) <= 228 * 1024 ? 2 : 1;       // with what a CTA takes besides
+}
+
 // The kernel that serves a call, its tile rows and grid, and the workspace.
 enum class AttnKernel { kSimt, kTokens, kChunks };
 struct AttnPlan {
@@ -474,7 +491,9 @@ struct AttnPlan {
 };
 
 // More than 16 rows (new tokens x heads of a group) per sequence on average
-// take tiles of many rows; 16-bit caches that page tiles fit, the tensor cores.
+// take tiles of many rows; 16-bit caches that page tiles fit, the tensor cores
+// (24 x 5 tokens over 8000 slots, four heads a group: 167 us, and 249 with tiles of
+// 16 rows; one such sequence over 2000: 18.0 and 15.8).
 // On the CUDA cores a tile costs its rows whether they are used or not, and a
 // row of a 32-row tile about 5/4 of one of a 64-row tile.
 AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
@@ -484,7 +503,7 @@ AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   const int64_t mean = (p.rows * p.group + p.c.batch - 1) / p.c.batch, padded64 = (mean + 63) / 64 * 64,
                 padded32 = (mean + 31) / 32 * 32;
   a.rows = !chunks ? 16 : a.kernel == AttnKernel::kChunks ? 256 : 4 * padded64 <= 5 * padded32 ? 64 : 32;
-  a.grid = a.kernel == AttnKernel::kSimt ? 2 * 148 : 148;
+  a.grid = a.kernel == AttnKernel::kSimt ? 148 * simt_resident(a.rows, p.c.d) : 148;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t lines = static_cast<size_t>(p.rows) * p.c.h_kv * p.group;
   a.part = SSA_PAGED_ZEROED;                 // after the counters, whose place never changes

@@ -224,7 +224,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if len(shape) != 3 or shape[2] != c.d:
         raise ValueError(f"q must be [rows, h_q, {c.d}], got {list(shape)}")
     rows, h_q, d = shape
-    if h_q % c.h_kv:
+    if c.h_kv < 1 or h_q % c.h_kv:
         raise ValueError("num_q_heads must be divisible by num_kv_heads")
     q_starts = _index(q_starts, "q_starts", key, c.batch + 1)
     qn, qh, _ = q.stride()

@@ -115,3 +115,10 @@ def test_what_the_module_refuses_is_named_by_python(name, change):
     for k in ("k", "v", "w"):
         if k != name:
             assert torch.equal(t[k], before[k])
+
+
+@pytest.mark.gpu
+def test_a_cache_without_heads_is_refused():
+    t = _tensors("cuda")
+    with pytest.raises(ValueError):
+        ssa.paged_attention(t["q"], t["k"][:, :, :0], t["v"][:, :, :0], t["table"], t["starts"], t["lens"])
