@@ -498,6 +498,10 @@ struct AttnPlan {
 // row of a 32-row tile about 5/4 of one of a 64-row tile.
 AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   AttnPlan a{};
+  if (p.rows == 0 || p.c.batch == 0) {       // nothing is launched: the zeroed head alone
+    a.total = SSA_PAGED_ZEROED;
+    return a;
+  }
   const bool chunks = p.rows * p.group > 16ll * p.c.batch;
   a.kernel = !page_tiles_supported(p, dt) ? AttnKernel::kSimt : chunks ? AttnKernel::kChunks : AttnKernel::kTokens;
   const int64_t mean = (p.rows * p.group + p.c.batch - 1) / p.c.batch, padded64 = (mean + 63) / 64 * 64,

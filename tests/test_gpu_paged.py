@@ -598,3 +598,14 @@ def test_cache_refusals():
     tracked.extend([t], [60])
     with pytest.raises(RuntimeError, match="free pages"):
         tracked.evict([t], 32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_without_sequences(dtype):
+    """A padded q and an empty batch: nothing to do, and nothing is done."""
+    c = make([20], [5], 4, 2, 64, 16, dtype, weights=True)
+    none, start = torch.empty((0, 2), dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    before = c["w"].clone()
+    out, lse = ssa.paged_attention(c["q"], c["k"], c["v"], none, start, none[:, 0], weights=c["w"], return_lse=True)
+    assert out.shape == (5, 4, 64) and lse.shape == (5, 4) and torch.equal(c["w"], before)
+    ssa.check_errors()

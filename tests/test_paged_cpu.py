@@ -3,6 +3,9 @@ ABI before any launch, and the refusals of the Python ops."""
 
 import ctypes
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -119,3 +122,23 @@ def test_cpu_tensors_raise_no_fallback():
                  lambda: ssa.paged_evict(k, k, k[..., 0], i[None, :1], i[:1], i[None, :1], 4)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_workspace_of_a_call_without_work(lib):
+    """No sequence or no row: a size all the same, and a call that does nothing.
+    In a process of its own: a fault there would take this one along."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = f"""
+import ctypes, sys
+sys.path[:0] = [{root!r}, {os.path.join(root, 'tests')!r}]
+from test_paged_cpu import L, _attn, _cache
+lib = L.lib()
+for dtype in (L.SSA_F32, L.SSA_BF16, L.SSA_F16):
+    for batch, rows in ((0, 0), (0, 5), (2, 0)):
+        c, a = _cache(batch=batch, dtype=dtype), _attn(rows=rows)
+        need = lib.ssa_paged_attn_workspace_size(ctypes.byref(c), ctypes.byref(a))
+        assert need == L.SSA_PAGED_ZEROED, (dtype, batch, rows, need)
+        assert lib.ssa_paged_attn(ctypes.byref(c), ctypes.byref(a), None, 0, None) == 0
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stderr)
