@@ -372,7 +372,8 @@ typedef struct {
 /* Bytes of workspace the call needs.  Its first SSA_PAGED_ZEROED bytes must be zero before the first call that uses it;
  * every call leaves them zero (but one that reports SSA_DEVICE_TIMEOUT: zero
  * them again).  Calls that may overlap on the GPU need a
- * workspace each. */
+ * workspace each, and so do host threads that call at the same time, on one stream
+ * too: a call is several launches, which must not mix with another's. */
 #define SSA_PAGED_ZEROED 16384
 size_t ssa_paged_attn_workspace_size(const SsaPagedCache* cache, const SsaPagedAttnArgs* args);
 

@@ -109,6 +109,19 @@ class _HostWords:
 
 
 _words = {}
+
+
+class Workspace:
+    """A buffer that :func:`ssa_b200.paged_attention` keeps, and the lock that is held over
+    the launches of a call: they hand partial results through the buffer, and
+    nothing but the order of the launches keeps two threads' calls apart."""
+
+    __slots__ = ("buffer", "launching")
+
+    def __init__(self, buffer):
+        self.buffer, self.launching = buffer, threading.Lock()
+
+
 # Workspaces the paged ops keep, by (device, stream).  Their heads are zero between
 # calls, except after a kernel that gave up.
 workspaces = {}

@@ -118,32 +118,39 @@ def _finish(key, sync, name, code):
         S.host_word_done(torch.device("cuda", key))
 
 
-def _call(key, sync, fn, *args):
+def _launch(key, fn, *args):
     if torch.cuda.current_device() == key:
-        code = fn(*args, _raw_stream(key))
-    else:
-        with torch.cuda.device(key):
-            code = fn(*args, _raw_stream(key))
-    _finish(key, sync, fn.__name__, code)
+        return fn(*args, _raw_stream(key))
+    with torch.cuda.device(key):
+        return fn(*args, _raw_stream(key))
 
 
-# One workspace per (device, stream), kept: calls on a stream follow one another.
+def _call(key, sync, fn, *args):
+    _finish(key, sync, fn.__name__, _launch(key, fn, *args))
+
+
+# One workspace per (device, stream), kept: calls on a stream follow one another,
+# also those of several threads, which take turns to launch (S.Workspace).
 # A capture takes its own (its graph owns that memory), and so do rare large
 # ones.  The head of a workspace is zero before a call and after it.
 _KEPT = 96 << 20
 
 
-def _workspace(key: int, nbytes: int, like: torch.Tensor) -> torch.Tensor:
+def _new_workspace(nbytes: int, like: torch.Tensor) -> S.Workspace:
+    ws = like.new_empty((nbytes,), dtype=torch.uint8)
+    ws[:L.SSA_PAGED_ZEROED].zero_()
+    return S.Workspace(ws)
+
+
+def _workspace(key: int, nbytes: int, like: torch.Tensor) -> S.Workspace:
     if nbytes > _KEPT or torch.cuda.is_current_stream_capturing():
-        ws = like.new_empty((nbytes,), dtype=torch.uint8)
-        ws[:L.SSA_PAGED_ZEROED].zero_()
-        return ws
+        return _new_workspace(nbytes, like)
     at = key, _raw_stream(key)
     ws = S.workspaces.get(at)
-    if ws is None or ws.numel() < nbytes:
+    if ws is None or ws.buffer.numel() < nbytes:
         with torch.cuda.device(key):
-            ws = S.workspaces[at] = like.new_empty((nbytes,), dtype=torch.uint8)
-            ws[:L.SSA_PAGED_ZEROED].zero_()
+            ws = _new_workspace(nbytes, like)
+        S.workspaces[at] = ws            # only now: another thread may take it at once
     return ws
 
 
@@ -212,8 +219,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         ws = S.workspaces.get((key, _raw_stream(key)))
         if ws is not None and not torch.cuda.is_current_stream_capturing():
             word, sync = S.host_word(key, _ATTEND)
-            done = L.paged_call().attend(q, k_pages, v_pages, page_table, q_starts, kv_lens, scale, is_causal, weights,
-                                         return_lse, word, ws)
+            with ws.launching:
+                done = L.paged_call().attend(q, k_pages, v_pages, page_table, q_starts, kv_lens, scale, is_causal,
+                                             weights, return_lse, word, ws.buffer)
             if done is not None:
                 code, out, lse = done
                 _finish(key, sync, "ssa_paged_attn", code)
@@ -236,7 +244,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     lib = L.lib()
     nbytes = lib.ssa_paged_attn_workspace_size(c, a)
     ws = _workspace(key, nbytes, q)
-    _call(key, sync, lib.ssa_paged_attn, c, a, ws.data_ptr(), nbytes)
+    with ws.launching:
+        code = _launch(key, lib.ssa_paged_attn, c, a, ws.buffer.data_ptr(), nbytes)
+    _finish(key, sync, "ssa_paged_attn", code)
     return (out, lse) if return_lse else out
 
 
