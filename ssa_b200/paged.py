@@ -250,6 +250,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return (out, lse) if return_lse else out
 
 
+def _check_budget(budget: int, recent: int) -> None:
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"budget {budget}, recent {recent}: need budget >= 1 and 0 <= recent <= budget")
+
+
 def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Tensor, page_table: torch.Tensor,
                 kv_lens: torch.Tensor, new_table: torch.Tensor, budget: int, recent: int = 0
                 ) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -276,8 +281,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
             _finish(key, sync, "ssa_paged_evict", code)
             return kept, new_lens
     key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _EVICT)
-    if budget < 1 or not 0 <= recent <= budget:
-        raise ValueError(f"budget {budget}, recent {recent}: need budget >= 1 and 0 <= recent <= budget")
+    _check_budget(budget, recent)
     new_table = _table(new_table, "new_table", key, c.batch)
     kept = kv_lens.new_empty((c.batch, c.h_kv, budget))
     new_lens = kv_lens.new_empty((c.batch,))
@@ -400,12 +404,14 @@ class PagedCache:
         """Cuts the sequences longer than ``budget`` back to it in every layer
         (:func:`paged_evict`); returns their ids.  The copies go to free pages,
         so at least one sequence's budget of them must be free; as many
-        sequences as fit are cut at a time."""
+        sequences as fit are cut at a time.  Where a call fails, the sequences
+        not yet cut in every layer keep their pages and lengths."""
         if self.weights is None:
             raise ValueError("the cache keeps no weights: make it with track_weights=True")
-        ids = list(ids)
+        ids, budget, recent = list(ids), int(budget), int(recent)
         if len(set(ids)) != len(ids):
             raise ValueError("ids must be distinct")
+        _check_budget(budget, recent)
         todo = [s for s in ids if self._len[s] > budget]
         done, need = list(todo), self._pages_for(budget)
         if todo and len(self._free) < need:
@@ -415,11 +421,16 @@ class PagedCache:
             todo = todo[len(now):]
             old = [self._pages[s] for s in now]
             new = [[self._free.pop() for _ in range(need)] for _ in now]
-            table, lens = self._upload(old, [self._len[s] for s in now])
-            new_table, = self._upload(new)
-            for layer in range(self.num_layers):
-                paged_evict(self.k_pages[layer], self.v_pages[layer], self.weights[layer], table, lens, new_table,
-                            budget, recent)
+            try:
+                table, lens = self._upload(old, [self._len[s] for s in now])
+                new_table, = self._upload(new)
+                for layer in range(self.num_layers):
+                    paged_evict(self.k_pages[layer], self.v_pages[layer], self.weights[layer], table, lens, new_table,
+                                budget, recent)
+            except BaseException:
+                # the old pages are as they were
+                self._free.extend(p for pages in reversed(new) for p in reversed(pages))
+                raise
             for s, o, p in zip(now, old, new):
                 self._free.extend(reversed(o))
                 self._pages[s], self._len[s] = p, budget
