@@ -105,7 +105,6 @@ class _HostWords:
         self.view = (ctypes.c_int32 * 4).from_address(base)
         self.low, self.high = (ctypes.c_int64.from_address(base + 8 * i) for i in range(2))   # all four, in two reads
         self.address = [base + 4 * op for op in range(len(self.OPS))]
-        self.used = False
 
 
 _words = {}
@@ -141,7 +140,6 @@ def host_word(key: int, op: int):
             w = _words.setdefault(key, _HostWords())
     elif w.low.value or w.high.value:
         _poll_words(key)
-    w.used = True
     return w.address[op], m == "sync"
 
 
@@ -216,15 +214,15 @@ def release(slot: Optional[Slot], op: str, decode: Callable[[str, int], Optional
 
 
 def check_errors(device=None) -> None:
-    """Wait for every op launched so far on ``device`` (default: all devices
-    with pending words) and raise for the first error a kernel reported."""
+    """Wait for every op launched so far on ``device``, in replayed graphs too
+    (default: all devices with pending words), and raise for the first error a kernel reported."""
     only = None if device is None else torch.device(device).index
     if device is not None and only is None:
         only = torch.cuda.current_device()
     for key, w in list(_words.items()):
-        if w.used and (only is None or key == only):
+        # whatever was called since the last check: a replayed graph writes its words too
+        if only is None or key == only:
             torch.cuda.synchronize(key)
-            w.used = False
             _poll_words(key)
     with _lock:
         rings = list(_rings.values()) if device is None else [_ring(torch.device(device))]
