@@ -1,6 +1,8 @@
 """The paged ops' error words: what the host reads, and when (words in plain memory here;
 on the GPU a replayed graph's errors)."""
 
+import types
+
 import pytest
 import torch
 
@@ -17,6 +19,7 @@ def words(monkeypatch):
     monkeypatch.setattr(torch.cuda, "synchronize", waits.append)
     monkeypatch.setattr(S, "_words", {})
     monkeypatch.setattr(S, "_rings", {})
+    monkeypatch.setattr(S, "_ring", lambda dev: types.SimpleNamespace(pending=[]))
     monkeypatch.setattr(S, "workspaces", {})
     monkeypatch.delenv("SSA_CHECKED", raising=False)
     return waits
