@@ -31,12 +31,11 @@ __global__ void __launch_bounds__(256) append_kernel(PagedAppendParams p, int el
     const PagedSeq q = paged_seq(c, p.q_starts, p.rows, lo);
     int64_t k_at = -1, v_at = 0, w_at = 0;
     if (t >= q.q0 && t < q.q0 + q.n) {              // else a skipped sequence, or a row of none
-      const int64_t slot = static_cast<int64_t>(q.len) - q.n + (t - q.q0);
-      if (slot < 0) {
+      if (q.n > q.len) {                            // more rows than the sequence holds: none of them is written
         paged_error(c, SSA_DEVICE_BAD_LENGTH);
       } else {
         int page, row;
-        page_of(c, static_cast<int>(slot), page, row);
+        page_of(c, q.len - q.n + static_cast<int>(t - q.q0), page, row);
         const int64_t pg = physical_page(c, c.table, c.table_stride, lo, page);
         if (pg >= 0) {
           k_at = pg * c.k_sp + row * c.k_sn;

@@ -609,3 +609,21 @@ def test_rows_without_sequences(dtype):
     out, lse = ssa.paged_attention(c["q"], c["k"], c["v"], none, start, none[:, 0], weights=c["w"], return_lse=True)
     assert out.shape == (5, 4, 64) and lse.shape == (5, 4) and torch.equal(c["w"], before)
     ssa.check_errors()
+
+
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+@pytest.mark.parametrize("lens,q_lens,bad", [([9, 40, 30], [2, 41, 5], 1), ([1, 20], [300, 20], 0), ([0, 7], [3, 1], 0)])
+def test_append_of_more_rows_than_a_sequence_holds_writes_none_of_them(lens, q_lens, bad, layout):
+    c = make(lens, q_lens, 4, 2, 64, 16, torch.bfloat16, layout, seed=5, weights=True)
+    k_new, v_new = torch.randn((2, c["starts"][-1], 2, 64), device=DEV).to(torch.bfloat16).unbind()
+    ref = {n: c[n].clone() for n in ("k", "v", "w")}
+    for s, (n, L_) in enumerate(zip(q_lens, lens)):
+        if s != bad:
+            pg, sl = slots(c, s, L_)
+            pg, sl, r = pg[L_ - n:], sl[L_ - n:], slice(c["starts"][s], c["starts"][s + 1])
+            ref["k"][pg, sl], ref["v"][pg, sl], ref["w"][pg, sl] = k_new[r], v_new[r], 0.0
+    ssa.paged_append(k_new, v_new, c["k"], c["v"], c["page_table"], c["q_starts"], c["kv_lens"], c["w"])
+    with pytest.raises(ValueError, match="paged_append"):
+        ssa.check_errors()
+    for n in ("k", "v", "w"):
+        assert torch.equal(c[n], ref[n]), n
