@@ -69,12 +69,12 @@ typedef enum {
 #define SSA_DEVICE_BAD_PAGE 0x10   /* paged cache: a page table entry of a used slot is
                                       outside [0, num_pages); the slot is not written,
                                       and what is computed from it is undefined       */
-#define SSA_DEVICE_BAD_LENGTH 0x20 /* paged cache: q_starts does not ascend within
+#define SSA_DEVICE_TIMEOUT 0x100   /* route: a pipeline wait gave up (~1 s); the
+                                      affected codes are undefined                  */
+#define SSA_DEVICE_BAD_LENGTH 0x10000 /* paged cache: q_starts does not ascend within
                                       [0, rows], a length is outside its table, or more
                                       rows are appended than the sequence holds; the
                                       sequence is skipped                             */
-#define SSA_DEVICE_TIMEOUT 0x100   /* route: a pipeline wait gave up (~1 s); the
-                                      affected codes are undefined                  */
 
 typedef enum { SSA_F32 = 0, SSA_BF16 = 1, SSA_F16 = 2 } ssa_dtype;
 typedef enum { SSA_I32 = 0, SSA_I64 = 1 } ssa_index_dtype;
@@ -343,7 +343,9 @@ typedef struct {
   const int32_t* page_table; int64_t table_stride;            /* [batch, max_pages]   */
   const int32_t* kv_lens;                                     /* [batch]              */
   int32_t* status;            /* optional word that device code can write (device
-                                 memory or mapped host memory), SSA_DEVICE_* bits     */
+                                 memory or mapped host memory), SSA_DEVICE_* bits.  Each
+                                 of these ops' errors has a byte of its own in it, which
+                                 plain stores write: the bits of one call add up          */
 } SsaPagedCache;
 
 /* A chunk of new rows of the sequences: rows q_starts[s] .. q_starts[s+1]-1

@@ -21,8 +21,8 @@ SSA_DEVICE_BAD_CODE = 0x2
 SSA_DEVICE_BAD_INDEX = 0x4
 SSA_DEVICE_INDEX_FULL = 0x8
 SSA_DEVICE_BAD_PAGE = 0x10
-SSA_DEVICE_BAD_LENGTH = 0x20
 SSA_DEVICE_TIMEOUT = 0x100
+SSA_DEVICE_BAD_LENGTH = 0x10000
 SSA_PAGED_ZEROED = 16384
 STATUS_NAMES = {0: "SSA_OK", 1: "SSA_ERR_INVALID_ARG", 2: "SSA_ERR_UNSUPPORTED", 3: "SSA_ERR_WORKSPACE",
                 4: "SSA_ERR_ALIGNMENT", 5: "SSA_ERR_CUDA", 6: "SSA_ERR_DEVICE"}

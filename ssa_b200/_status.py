@@ -24,6 +24,8 @@ The paged-cache ops, called once per layer and token, are too short for a
 copy, a reset and an event each.  Their kernels write an error straight into a
 word of mapped pinned host memory, one per op and device, which later op calls
 read as plain memory (:func:`poll`); it is valid inside a graph capture too.
+With ``SSA_CHECKED=0`` they write a word of which only timeouts are read: a
+kernel that gave up leaves its workspace unfit for the next call.
 """
 
 from __future__ import annotations
@@ -95,16 +97,27 @@ def poll(dev: torch.device) -> None:
 
 
 class _HostWords:
-    """A word of mapped pinned memory per paged-cache op of one device."""
+    """A word of mapped pinned memory per paged-cache op of one device, and one for all
+    calls with ``SSA_CHECKED=0``, of which only timeouts are looked at.  A kernel stores
+    the byte of the error's kind, so that none hides another."""
 
     OPS = ("paged_append", "paged_attention", "paged_evict")
 
     def __init__(self):
         self.host = torch.zeros(4, dtype=torch.int32).pin_memory()
         base = self.host.data_ptr()
-        self.view = (ctypes.c_int32 * 4).from_address(base)
+        self.bytes = (ctypes.c_uint8 * 16).from_address(base)
         self.low, self.high = (ctypes.c_int64.from_address(base + 8 * i) for i in range(2))   # all four, in two reads
-        self.address = [base + 4 * op for op in range(len(self.OPS))]
+        self.unchecked = ctypes.c_int32.from_address(base + 12)
+        self.address = [base + 4 * word for word in range(4)]
+
+    def take(self, word: int, bits: int) -> bool:
+        """Whether an error of the kind ``bits`` stands in a word; clears that kind alone."""
+        at = 4 * word + (bits.bit_length() - 1) // 8
+        if not self.bytes[at]:
+            return False
+        self.bytes[at] = 0
+        return True
 
 
 _words = {}
@@ -128,17 +141,19 @@ workspaces = {}
 
 def host_word(key: int, op: int):
     """Address of the error word of op number ``op`` (in ``_HostWords.OPS``) on
-    device number ``key``, or None with ``SSA_CHECKED=0``, and whether
-    :func:`host_word_done` is to follow the launch; raises for an error already
-    found."""
+    device number ``key``, and whether :func:`host_word_done` is to follow the launch;
+    raises for an error already found (with ``SSA_CHECKED=0``, where the word is
+    another one, never)."""
     m = mode()
-    if m == "off":
-        return None, False
     w = _words.get(key)
     if w is None:
         with _lock:
             w = _words.setdefault(key, _HostWords())
-    elif w.low.value or w.high.value:
+    if m == "off":
+        if w.unchecked.value:
+            _clear_unchecked(w)
+        return w.address[3], False
+    if w.low.value or w.high.value:
         _poll_words(key)
     return w.address[op], m == "sync"
 
@@ -150,15 +165,23 @@ def host_word_done(dev: torch.device) -> None:
         _poll_words(dev.index)
 
 
+def _clear_unchecked(w: _HostWords) -> None:
+    if w.take(3, L.SSA_DEVICE_TIMEOUT):
+        workspaces.clear()
+    w.unchecked.value = 0
+
+
 def _poll_words(key: int) -> None:
+    """Raises for one kind of error of one op, and leaves the others for the next time:
+    timeouts first, since they leave the workspaces' heads undefined."""
     w = _words.get(key)
     if w is None:
         return
-    for i, op in enumerate(w.OPS):
-        bits = w.view[i]
-        if bits:
-            w.view[i] = 0
-            raise paged_error(op, bits)
+    _clear_unchecked(w)
+    for bits, error in _PAGED_ERRORS:
+        for word, op in enumerate(w.OPS):
+            if w.take(word, bits):
+                raise error(op)
 
 
 class Slot:
@@ -259,12 +282,14 @@ def attn_error(op: str, bits: int) -> Optional[Exception]:
     return RuntimeError(f"{op}: device status 0x{bits:x}")
 
 
-def paged_error(op: str, bits: int) -> Exception:
-    if bits & L.SSA_DEVICE_BAD_PAGE:
-        return IndexError(f"{op}: a page table entry is outside [0, num_pages)")
-    if bits & L.SSA_DEVICE_BAD_LENGTH:
-        return ValueError(f"{op}: q_starts or a length does not fit the rows and the page table")
-    if bits & L.SSA_DEVICE_TIMEOUT:
-        workspaces.clear()
-        return RuntimeError(f"{op}: a device pipeline wait timed out; results are undefined")
-    return RuntimeError(f"{op}: device status 0x{bits:x}")
+def _paged_timeout(op: str) -> Exception:
+    workspaces.clear()
+    return RuntimeError(f"{op}: a device pipeline wait timed out; results are undefined")
+
+
+_PAGED_ERRORS = (
+    (L.SSA_DEVICE_TIMEOUT, _paged_timeout),
+    (L.SSA_DEVICE_BAD_PAGE, lambda op: IndexError(f"{op}: a page table entry is outside [0, num_pages)")),
+    (L.SSA_DEVICE_BAD_LENGTH,
+     lambda op: ValueError(f"{op}: q_starts or a length does not fit the rows and the page table")),
+)

@@ -77,9 +77,12 @@ struct PagedEvictParams {
   int new_max_pages, budget, recent;
 };
 
-// A run-time error word: plain stores, so that it may be mapped host memory.
-__device__ __forceinline__ void paged_error(const PagedCacheParams& c, int32_t bits) {
-  if (c.status) *reinterpret_cast<volatile int32_t*>(c.status) = bits;
+// A run-time error word: plain stores, so that it may be mapped host memory, of
+// the byte that the kind of error has to itself, so that none hides another.
+__device__ __forceinline__ void paged_error(const PagedCacheParams& c, uint32_t bits) {
+  static_assert(SSA_DEVICE_BAD_PAGE < 0x100 && SSA_DEVICE_TIMEOUT == 0x100 && SSA_DEVICE_BAD_LENGTH == 0x10000, "a byte each");
+  const int at = bits >= 0x10000u ? 2 : bits >= 0x100u ? 1 : 0;
+  if (c.status) reinterpret_cast<volatile uint8_t*>(c.status)[at] = static_cast<uint8_t>(bits >> (8 * at));
 }
 
 __device__ __forceinline__ void page_of(const PagedCacheParams& c, int slot, int& page, int& row) {

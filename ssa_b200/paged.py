@@ -216,9 +216,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     """
     if k_pages.is_cuda:
         key = k_pages.get_device()
+        word, sync = S.host_word(key, _ATTEND)            # before the look-up: it drops workspaces left unfit
         ws = S.workspaces.get((key, _raw_stream(key)))
         if ws is not None and not torch.cuda.is_current_stream_capturing():
-            word, sync = S.host_word(key, _ATTEND)
             with ws.launching:
                 done = L.paged_call().attend(q, k_pages, v_pages, page_table, q_starts, kv_lens, scale, is_causal,
                                              weights, return_lse, word, ws.buffer)

@@ -102,6 +102,20 @@ def test_a_workspace_is_handed_out_zeroed(launches, monkeypatch):
     assert seen == [False, False]
 
 
+def test_a_workspace_dropped_by_an_errors_look_up_is_not_used(launches, monkeypatch):
+    """A timeout leaves the head of a workspace undefined: the call that learns of it takes
+    another one."""
+    plain = torch.zeros((5, 4, 64))
+    _attend(plain)
+    old = S.workspaces[0, 7].buffer
+    launches.calls.clear()
+    monkeypatch.setattr(S, "host_word", lambda key, op: (S.workspaces.clear(), (None, False))[1])
+    used = []
+    monkeypatch.setattr(launches, "attend", lambda *args: used.append(args[-1]) and None)
+    _attend(plain)
+    assert not any(u is old for u in used) and S.workspaces[0, 7].buffer is not old
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 64)])
 @pytest.mark.parametrize("q_lens", [[1, 1, 1], [70, 300, 5]])
