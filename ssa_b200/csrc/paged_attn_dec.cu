@@ -15,10 +15,10 @@
 // 12 us, all of it latency.
 //
 // P enters the product with V as two 16-bit terms (p = hi + lo, off by 2^-17),
-// sums and outputs are fp32.  Slots hidden from a row have p = 0; where the
-// sixteen slots of a warp hold a non-finite value in V and some are hidden,
-// the product is made on the CUDA cores over the visible ones alone (0 times
-// infinity is NaN).
+// sums and outputs are fp32.  Slots hidden from a row have p = 0, and so has lo at
+// many others: 0 times infinity is NaN.  So two more warps look through V as it comes,
+// and a tile that holds a non-finite value has its product made on the CUDA cores, over
+// the visible slots and with p in fp32.
 //
 // Every wait is bounded (about one second); on expiry the CTA records
 // SSA_DEVICE_TIMEOUT and runs to its end without further waits.
@@ -41,7 +41,8 @@ constexpr int kKT = 64;
 constexpr int kExtra = 4;          // units an item costs besides its tiles
 constexpr int kLeast = 4;          // units a CTA takes at least (1: 9.8 us, 4: 8.4 us, 8: 11.3 us at 128 slots)
 constexpr int kWarps = 8;          // consumers: two groups of four, 16 slots of a tile each
-constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kLookers = 2;        // warps that look through V, the tiles of one group each
+constexpr int kThreads = 32 * (kWarps + 1 + kLookers);
 
 template <int D>
 struct Geo {
@@ -52,7 +53,7 @@ struct Geo {
   static_assert(kStages % 2 == 0, "stages alternate between the two groups");
   static constexpr int kJoinRow = D + 4;                            // floats
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * 2 * kTileBytes +
-                                  kWarps * kRows * kJoinRow * 4 + 16 * kStages + 16 + sizeof(PagedStart);
+                                  kWarps * kRows * kJoinRow * 4 + 28 * kStages + 16 + sizeof(PagedStart);
 };
 
 template <typename T, int D>
@@ -67,22 +68,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   float* join = reinterpret_cast<float*>(base + G::kStages * 2 * G::kTileBytes);   // [warp][row][D + 4]
   uint64_t* bars = reinterpret_cast<uint64_t*>(join + kWarps * kRows * G::kJoinRow);
-  const uint32_t ring = smem_u32(base), full = smem_u32(bars), empty = full + 8 * G::kStages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * G::kStages);
+  const uint32_t ring = smem_u32(base), full = smem_u32(bars), empty = full + 8 * G::kStages, seen = empty + 8 * G::kStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 3 * G::kStages);
   volatile int* last = abort_flag + 1;
+  volatile int* odd_tile = abort_flag + 2;               // [kStages] V of the stage holds a non-finite value
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int tt = tile_tokens(kRows, p.group);
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) {
       mbar_init(full + 8 * s, 1);
       mbar_init(empty + 8 * s, kWarps / 2);
+      mbar_init(seen + 8 * s, 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
-  PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 2 * G::kStages + 1);
+  PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 3 * G::kStages + 1 + G::kStages / 2);
   paged_start(p, tt, kKT, kExtra, kLeast, &start);
   __syncthreads();
   PagedWalk w = start.w;
@@ -131,6 +134,37 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
     if (lane == 0)
       for (int64_t r = g - 1; r >= 0 && r >= g - G::kStages; --r)
         mbar_wait(full + 8 * static_cast<int>(r % G::kStages), static_cast<uint32_t>((r / G::kStages) & 1));
+    return;
+  }
+
+  if (warp > kWarps) {
+    // ---------------- lookers: does V of a tile hold a non-finite value? ----------------
+    const int mine = warp - kWarps - 1;
+    int64_t g = 0;
+    for (bool going = true; going; going = paged_advance(p, tt, kKT, kExtra, w)) {
+      const PagedSegment seg = paged_segment(w, kExtra);
+      for (int t = seg.first; t < seg.last; ++t, ++g) {
+        if ((g & 1) != mine) continue;
+        const int st = static_cast<int>(g % G::kStages);
+        wait(full + 8 * st, static_cast<uint32_t>((g / G::kStages) & 1));
+        const uint4* v = reinterpret_cast<const uint4*>(base + (2 * st + 1) * G::kTileBytes) + lane;
+        uint4 odd = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 8
+        for (int x = 0; x < G::kTileBytes / 512; ++x) {
+          const uint4 a = v[32 * x];
+          odd.x = times_zero<T>(a.x, odd.x);
+          odd.y = times_zero<T>(a.y, odd.y);
+          odd.z = times_zero<T>(a.z, odd.z);
+          odd.w = times_zero<T>(a.w, odd.w);
+        }
+        const bool any = __any_sync(0xffffffffu, odd_bits<T>(odd.x | odd.y | odd.z | odd.w) != 0);
+        if (lane == 0) {
+          odd_tile[st] = any;
+          mbar_arrive(seen + 8 * st);
+        }
+        __syncwarp();
+      }
+    }
     return;
   }
 
@@ -245,16 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_dec_kernel(const __grid_cons
       const int key = (warp & 3) * 16 + vk;
       const uint32_t row = vb + key * 128;
       auto v_at = [&](int t) { return row + (t / 4) * (kKT * 128) + ((((t % 4) * 2 + vp) ^ (key & 7)) << 4); };
-      uint32_t odd = 0;
-      if (masked) {
-#pragma unroll
-        for (int t = 0; t < NT / 2; ++t) {
-          uint32_t v[4];
-          ldsm_x4_t(v_at(t), v[0], v[1], v[2], v[3]);
-          odd |= odd_bits<T>(v[0]) | odd_bits<T>(v[1]) | odd_bits<T>(v[2]) | odd_bits<T>(v[3]);
-        }
-      }
-      if (__any_sync(0xffffffffu, odd != 0)) {
+      wait(seen + 8 * st, static_cast<uint32_t>((g / G::kStages) & 1));
+      if (__any_sync(0xffffffffu, odd_tile[st])) {
         for (int j = 0; j < 16; ++j) {
           // p of rows gr, gr + 8 at slot j: fragment t = j / 8, lane column (j % 8) / 2
           const int src = (lane & 28) + ((j & 7) >> 1);

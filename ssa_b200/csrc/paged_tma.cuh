@@ -6,6 +6,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "paged.cuh"
@@ -51,6 +52,18 @@ template <> struct Half16<__half> { static constexpr uint32_t kExp = 0x7c007c00u
 template <typename T>
 __device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
   return ((w & Half16<T>::kExp) + Half16<T>::kOne) & 0x80008000u;
+}
+
+// x * 0 + acc of both halves: from acc = 0, NaN in a half that met a non-finite
+// value and 0 elsewhere.
+template <typename T>
+__device__ __forceinline__ uint32_t times_zero(uint32_t x, uint32_t acc) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0u), "r"(acc));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0u), "r"(acc));
+  return d;
 }
 
 template <typename T>

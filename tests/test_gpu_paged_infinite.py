@@ -1,0 +1,52 @@
+"""Infinite and NaN values that rows see: the paged attention gives what the formula
+gives -- the same infinities, NaN where it has NaN, and its tolerance elsewhere."""
+
+import math
+
+import pytest
+import torch
+
+import ssa_b200 as ssa
+from test_gpu_paged import U, make, oracle, slots
+
+pytestmark = pytest.mark.gpu
+
+KINDS = [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float16, 128), (torch.float16, 64), (torch.float32, 64),
+         (torch.bfloat16, 96)]
+
+
+def _check(c, causal=True):
+    out = ssa.paged_attention(c["q"], c["k"], c["v"], c["page_table"], c["q_starts"], c["kv_lens"], is_causal=causal)
+    ref, amp, _, _ = oracle(c, causal=causal)
+    for same in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(same(out), same(ref)), same.__name__
+    fine = torch.isfinite(ref)
+    u = U[out.dtype]
+    assert ((out.double() - ref).abs() <= u * ref.abs() + (u + 2e-5) * amp + 1e-7)[fine].all()
+    return out
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+@pytest.mark.parametrize("q_len", [1, 3])
+@pytest.mark.parametrize("sharp", [1.0, 5.0])
+def test_infinite_values(dtype, d, q_len, sharp):
+    """Weights down to some 2^-60 of a row's largest: of every infinite value a part, and no
+    NaN but where infinities of both signs or a NaN are seen."""
+    c = make([700, 320], [q_len, 1], 8, 2, d, 32, dtype, seed=d, weights=True)
+    c["q"].mul_(sharp)
+    pg, sl = slots(c, 0, 700)
+    v = c["v"]
+    v[pg[5], sl[5], 0, 3] = math.inf               # a tile that every row sees
+    v[pg[70], sl[70], 0, 4] = -math.inf
+    v[pg[200], sl[200], 0, 5] = math.nan
+    v[pg[6], sl[6], 0, 6] = math.inf
+    v[pg[300], sl[300], 0, 6] = -math.inf
+    v[pg[699], sl[699], 1, 7] = math.inf           # the last row alone sees it
+    v[pg[3], sl[3], 1, 7] = math.inf
+    pg, sl = slots(c, 1, 320)
+    v[pg[:], sl[:], 1, 0] = -math.inf
+    out = _check(c)
+    assert torch.isposinf(out[:q_len, :4, 3]).all() and torch.isneginf(out[:q_len, :4, 4]).all()
+    assert torch.isnan(out[:q_len, :4, 5:7]).all() and torch.isneginf(out[-1, 4:, 0]).all()
+    _check(c, causal=False)
+    ssa.check_errors()
