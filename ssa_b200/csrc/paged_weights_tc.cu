@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float c = p.inv_scale * kLog2e;
     const uint64_t c2 = pair(c, c);
+    const int rows = tt * g;                             // of a Q tile that boxes fill
     bool going = true;
     for (int second = 0; going && !__any_sync(0xffffffffu, *abort_flag); second = 1, going = advance()) {
       const PagedSegment seg = row_tiles();
@@ -277,6 +278,12 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         for (int q4 = 0; q4 < 4; ++q4) {
           tmem_wait();
           if (q4 < 3) tmem_ld32_async(ta + 32 * (q4 + 1), v[(q4 + 1) & 1]);
+          if (q4 == 3 && rows < kRows) {
+            // rows that no box fills, fewer than g: zero queries, whose score with an
+            // infinite key is NaN
+#pragma unroll
+            for (int j = 16; j < 32; ++j) v[q4 & 1][j] = 96 + j < rows ? v[q4 & 1][j] : 0u;
+          }
           if (!masked) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {

@@ -50,3 +50,24 @@ def test_infinite_values(dtype, d, q_len, sharp):
     assert torch.isnan(out[:q_len, :4, 5:7]).all() and torch.isneginf(out[-1, 4:, 0]).all()
     _check(c, causal=False)
     ssa.check_errors()
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+@pytest.mark.parametrize("h_q,h_kv", [(28, 4), (3, 1), (13, 1), (8, 2)])
+@pytest.mark.parametrize("q_lens", [[200, 1], [1, 1], [300, 129]])
+def test_slot_weights_beside_an_infinite_key(dtype, d, h_q, h_kv, q_lens):
+    """A key with an infinite entry that every query meets with the other sign: its weight is
+    0 in every row, and all else stays finite."""
+    c = make([700, 320], q_lens, h_q, h_kv, d, 32, dtype, seed=d + h_q, weights=True)
+    c["q"][..., 3] = -c["q"][..., 3].abs() - 0.25
+    pg, sl = slots(c, 0, 700)
+    for at in (5, 130, 380):                       # tiles that every row sees
+        c["k"][pg[at], sl[at], 0, 3] = math.inf
+    w0 = c["w"].double()
+    ssa.paged_attention(c["q"], c["k"], c["v"], c["page_table"], c["q_starts"], c["kv_lens"], weights=c["w"])
+    _, _, _, add = oracle(c)
+    assert bool(torch.isfinite(add).all()) and not add[pg[5], sl[5], 0].any()
+    err = (c["w"].double() - w0 - add).abs()
+    assert (err <= 3e-5 * add + 2.0 ** -23 * (w0 + add)).all()
+    _check(c)
+    ssa.check_errors()
