@@ -19,6 +19,7 @@
 //   warps 4-7   stream B
 //   warp 8      TMEM allocation, single-thread MMA issue
 //   warp 9      TMA producer: a lane per page box, K and V tiles in a ring
+//   warps 10-11 look through V for non-finite values
 //
 // TMEM (512 columns): S_A, S_B (128 each; P in the first 64), O_A, O_B (d each).
 //
@@ -31,10 +32,11 @@
 // normal numbers.
 //
 // Hidden slots (past a row's position, or past the sequence in the last page)
-// have P = 0, but 0 times an infinite or NaN value is NaN.  So on a tile that
-// some row does not see whole, the streams look through V: if it holds a
-// non-finite value, that tile's product is made on the CUDA cores over the
-// visible slots alone.
+// have P = 0, and so have small weights rounded to fp16 (below 2^-31 of the largest), but
+// 0 times an infinite or NaN value is NaN.  So two warps look through V as it comes, for
+// bf16 on the tiles that some row does not see whole, for fp16 on all: the product of a
+// tile with a non-finite value is made on the CUDA cores over the visible slots alone,
+// in fp16 with P in fp32.
 //
 // Every wait is bounded (about one second); on expiry the CTA records
 // SSA_DEVICE_TIMEOUT, waits (bounded) for its copies and MMAs in flight, frees
@@ -57,14 +59,15 @@ constexpr int kRows = 256;         // rows of an item
 constexpr int kKT = 128;           // slots per key tile
 constexpr int kExtra = 4;          // units an item costs besides its tiles
 constexpr int kLeast = 1;          // units a CTA takes at least
-constexpr int kThreads = 320;
+constexpr int kLookers = 2;        // warps that look through V, half a tile each
+constexpr int kThreads = 32 * (10 + kLookers);
 constexpr float kSlack = 8.f;      // how far (log2) a tile may exceed the running maximum
 
 template <int D>
 struct Geo {
   static constexpr int kTileBytes = kKT * D * 2;
   static constexpr int kStages = D == 128 ? 5 : 10;
-  static constexpr size_t kSmem = 1024 + 2 * kTileBytes + static_cast<size_t>(kStages) * kTileBytes + 512;
+  static constexpr size_t kSmem = 1024 + 2 * kTileBytes + static_cast<size_t>(kStages) * kTileBytes + 640;
 };
 
 // A from TMEM, B from shared memory.
@@ -85,9 +88,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // The tile's O += P V for this thread's row over its first `see` slots, on the
-// CUDA cores (P in TMEM columns of S, V swizzled in shared memory).  `fresh`: O
-// holds nothing yet.  The whole stream calls it.
-template <typename T, int D>
+// CUDA cores (P in TMEM over S, packed in T or in fp32; V swizzled in shared memory).
+// `fresh`: O holds nothing yet.  The whole stream calls it.
+template <typename T, int D, bool kPacked>
 __device__ __forceinline__ void visible_product(uint32_t s_addr, uint32_t o_addr, const unsigned char* v, int see,
                                              bool fresh) {
 #pragma unroll 1
@@ -100,15 +103,16 @@ __device__ __forceinline__ void visible_product(uint32_t s_addr, uint32_t o_addr
     float acc[16];
 #pragma unroll
     for (int x = 0; x < 16; ++x) acc[x] = fresh ? 0.f : __uint_as_float(o[x]);
+    constexpr int kSlots = kPacked ? 32 : 16;            // of 16 columns
 #pragma unroll 1
-    for (int j0 = 0; j0 < kKT; j0 += 32) {
+    for (int j0 = 0; j0 < kKT; j0 += kSlots) {
       uint32_t pk[16];
-      tmem_ld16_async(s_addr + j0 / 2, pk);
+      tmem_ld16_async(s_addr + j0 * 16 / kSlots, pk);
       tmem_wait();
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float2 two = unpack2<T>(pk[j / 2]);
-        const float pj = (j & 1) ? two.y : two.x;
+      for (int j = 0; j < kSlots; ++j) {
+        const float2 two = unpack2<T>(pk[j * 16 / kSlots]);
+        const float pj = !kPacked ? __uint_as_float(pk[j * 16 / kSlots]) : (j & 1) ? two.y : two.x;
         if (j0 + j < see) {
           const unsigned char* row = v + (c0 / 64) * (kKT * 128) + (j0 + j) * 128;
 #pragma unroll
@@ -132,6 +136,25 @@ __device__ __forceinline__ void visible_product(uint32_t s_addr, uint32_t o_addr
     tmem_wait_st();
   }
 }
+// The row's exponentials of the first `see` slots in fp32, over the scores; their sum.
+__device__ __forceinline__ float wide_exps(uint32_t s_addr, int see, float c, float off) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int j0 = 0; j0 < kKT; j0 += 16) {
+    uint32_t u[16];
+    tmem_ld16_async(s_addr + j0, u);
+    tmem_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float e = j0 + j < see ? ex2_approx(fmaf(__uint_as_float(u[j]), c, -off)) : 0.f;
+      sum += e;
+      u[j] = __float_as_uint(e);
+    }
+    tmem_st16(s_addr + j0, u);
+    tmem_wait_st();
+  }
+  return sum;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -140,6 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   using G = Geo<D>;
   constexpr bool kBf = std::is_same<T, __nv_bfloat16>::value;
   constexpr float kShift = kBf ? 0.f : 7.f;              // factor 2^kShift on every exponential
+  // weights that fp32 holds but fp16 rounds to 0: V matters where every row sees it too
+  constexpr bool kLookAll = !kBf;
   constexpr uint32_t kIdS = idesc_f16(128, kKT, kBf);
   constexpr uint32_t kIdO = idesc_f16(128, D, kBf) | (1u << 16);   // B (= V) is MN-major
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -148,19 +173,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
   unsigned char* q_tile = base;                          // [2][D / 64][128][128 B], SWIZZLE_128B
   unsigned char* ring = base + 2 * G::kTileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + G::kStages * G::kTileBytes);
-  const uint32_t full = smem_u32(bars), empty = full + 8 * G::kStages;
-  const uint32_t q_full = empty + 8 * G::kStages, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 32;
-  const uint32_t v_seen = o_full + 16, drain = v_seen + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * G::kStages + 13);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * G::kStages, seen = empty + 8 * G::kStages;
+  const uint32_t q_full = seen + 8 * G::kStages, s_full = q_full + 16, p_full = s_full + 16, o_full = p_full + 32;
+  const uint32_t drain = o_full + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * G::kStages + 11);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* odd_tile = abort_flag + 1;               // [2] the last tile whose product the stream made itself
+  volatile int* odd_half = abort_flag + 1;               // [stage][looker] the half of V holds a non-finite value
+  volatile int* made = odd_half + 2 * G::kStages;        // [stream] it makes the tile's product itself
   const int warp = threadIdx.x / kWarp, lane = threadIdx.x % kWarp;
   const int tt = tile_tokens(kRows, p.group);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < G::kStages; ++s) {
       mbar_init(full + 8 * s, 1);
-      mbar_init(empty + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1 + kLookers);
+      mbar_init(seen + 8 * s, kLookers);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(q_full + 8 * x, 4);
@@ -168,8 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       mbar_init(p_full + 16 * x, 4);                     // P of slots 0-63, and of 64-127
       mbar_init(p_full + 16 * x + 8, 4);
       mbar_init(o_full + 8 * x, 1);
-      mbar_init(v_seen + 8 * x, 4);
-      odd_tile[x] = 0;
+      made[x] = 0;
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -181,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 2 * G::kStages + 16);
+  PagedStart& start = *reinterpret_cast<PagedStart*>(bars + 4 * G::kStages + 14);
   paged_start(p, tt, kKT, kExtra, kLeast, &start);
   fence_before();
   __syncthreads();
@@ -195,11 +221,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     paged_error(p.c, SSA_DEVICE_TIMEOUT);
   };
 
-  // a tile is named by its number in the CTA's walk, from 1
-  // (and begins again after a multiple of the ring's period: its entry and
-  // phase follow from it)
-  constexpr int kNames = G::kStages << 20;
-  auto name_next = [](int n) { return n == kNames ? 1 : n + 1; };
+  // V of the next tile: its ring entry and phase (every tile takes two entries, K's and V's)
+  auto next_entries = [](int& st, uint32_t& par) {
+    st += 2;
+    if (st >= G::kStages) {
+      st -= G::kStages;
+      par ^= 1u;
+    }
+  };
 
   if (any && warp == 9) {
     // ---------------- TMA producer ----------------
@@ -256,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       return (static_cast<uint64_t>(kDescHi) << 32) | ((kKT * 128u >> 4) << 16) | (lo & 0x3fffu);
     };
     uint32_t p_ph = 0, q_ph = 0;                         // bit x: stream x
-    int ks = 0, name = 1;                     // ring entry of the current unit's K
+    int ks = 0;                               // ring entry of the current unit's K
     uint32_t kpar = 0;
     bool stop = false;
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -313,18 +342,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
           const uint32_t pp = (p_ph >> x) & 1u;
           if (!wait(p_full + 16 * x, pp)) break;
           p_ph ^= 1u << x;
-          const bool made = __shfl_sync(0xffffffffu, odd_tile[x] == name, 0);
+          const bool done = __shfl_sync(0xffffffffu, made[x], 0) != 0;    // by the stream
           const uint32_t vb = ring_lo + vs * kTileDesc, acc = ((fresh >> x) & 1u) ^ 1u;
           auto product = [&](int k0) {                   // four steps of 16 slots
 #pragma unroll
             for (int k = k0; k < k0 + 4; ++k)
               mma_f16_ta(tmem + 256 + x * D, tmem + x * 128 + k * 8, desc_v(vb + (k * 2048 >> 4)), kIdO, k > 0 ? 1u : acc);
           };
-          if (!made && elect_one()) product(0);
+          if (!done && elect_one()) product(0);
           __syncwarp();
           if (!wait(p_full + 16 * x + 8, pp)) break;
           if (elect_one()) {
-            if (!made) product(4);
+            if (!done) product(4);
             if (x == streams - 1) mma_commit(empty + 8 * vs);
             if (!more) mma_commit(o_full + 8 * x);
           }
@@ -338,7 +367,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         ks = ns;
         kpar = npar;
-        name = name_next(name);
       }
     }
     // after a failed wait: the commit arrives once every MMA issued before it is done
@@ -357,8 +385,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     unsigned char* stage = q_tile + x * G::kTileBytes + (warp & 3) * 32 * 128;
     auto stage_at = [](int rr, int pc) { return (pc / 8) * (kKT * 128) + rr * 128 + (((pc % 8) ^ (rr & 7)) << 4); };
     const float c = p.inv_scale * kLog2e;
-    uint32_t s_ph = 0, o_ph = 0, v_ph = 0;
-    int name = 1;
+    uint32_t s_ph = 0, o_ph = 0, vpar = 0;
+    int vs = 1;
     bool stop = false;
     // the same answer in every lane: what follows is done by whole warps
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -381,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       const int tok0 = w.tile * tt, rows = min(tt, w.n - tok0) * p.group;
       const bool whole = seg.whole;
       if (x == 1 && rows <= 128) {                        // nothing for this stream here
-        for (int i = 0; i < units; ++i) name = name_next(name);
+        for (int i = 0; i < units; ++i) next_entries(vs, vpar);
         continue;
       }
       const int row = x * 128 + r;
@@ -405,9 +433,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
       fence_proxy_async();
       fence_before();
       arrive(q_full + 8 * x);
+      if (r == 0) made[x] = 0;                            // tiles that are not looked at come first
       float m = -INFINITY, l = 0.f;
       int k0 = seg.first * kKT;
-      for (int i = 0; i < units; ++i, k0 += kKT, name = name_next(name)) {
+      for (int i = 0; i < units; ++i, k0 += kKT, next_entries(vs, vpar)) {
         if (!wait(s_full + 8 * x, s_ph)) break;
         s_ph ^= 1u;
         const bool masked = k0 + kKT > lim0;              // the same for the whole stream
@@ -449,6 +478,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             tmem_wait_st();
           }
         }
+        // V holds a non-finite value: the product is made here, over the slots a row sees
+        auto odd = [&]() {
+          const bool is = wait(seen + 8 * vs, vpar) && (odd_half[2 * vs] | odd_half[2 * vs + 1]) != 0;
+          if (r == 0) made[x] = is;                       // before the MMA warp is told of P
+          return is;
+        };
         const float off = (m == -INFINITY ? 0.f : m) - kShift;
         const uint64_t c2 = pair(c, c), off2 = pair(-off, -off);
         uint64_t sum[2] = {0, 0};
@@ -481,32 +516,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
           }
         };
-        if (masked) exps(std::true_type{});
-        else exps(std::false_type{});
-        {
+        const unsigned char* v_tile = ring + vs * G::kTileBytes;
+        if (kLookAll && odd()) {
+          l += wide_exps(s_addr, see, c, off);
+          visible_product<T, D, false>(s_addr, o_addr, v_tile, see, i == 0);
+          fence_before();
+          arrive(p_full + 16 * x);
+        } else {
+          if (masked) exps(std::true_type{});
+          else exps(std::false_type{});
           float a, b;
           unpair(add_pair(sum[0], sum[1]), a, b);
           l += a + b;
+          tmem_wait_st();
+          if (!kLookAll && masked && odd()) visible_product<T, D, true>(s_addr, o_addr, v_tile, see, i == 0);
+          fence_before();
+          if (masked) arrive(p_full + 16 * x);
         }
-        tmem_wait_st();
-        if (masked) {
-          // a non-finite value in V, perhaps hidden from this row or another?
-          const int e = 2 * (name - 1) + 1, st = e % G::kStages;
-          if (!wait(full + 8 * st, static_cast<uint32_t>(e / G::kStages) & 1u)) break;
-          const unsigned char* v = ring + st * G::kTileBytes;
-          uint32_t odd = 0;
-          for (int y = r; y < G::kTileBytes / 16; y += 128) {
-            const uint4 a = *reinterpret_cast<const uint4*>(v + y * 16);
-            odd |= odd_bits<T>(a.x) | odd_bits<T>(a.y) | odd_bits<T>(a.z) | odd_bits<T>(a.w);
-          }
-          if (odd) odd_tile[x] = name;
-          arrive(v_seen + 8 * x);
-          if (!wait(v_seen + 8 * x, v_ph)) break;
-          v_ph ^= 1u;
-          if (odd_tile[x] == name) visible_product<T, D>(s_addr, o_addr, v, lim - k0, i == 0);
-        }
-        fence_before();
-        if (masked) arrive(p_full + 16 * x);
+        if (stop) break;
         arrive(p_full + 16 * x + 8);
       }
       if (stop) break;
@@ -573,6 +600,53 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         } else {
           part[D] = m - kShift;
           part[D + 1] = l;
+        }
+      }
+    }
+  } else if (any) {
+    // ---------------- lookers: does V hold a non-finite value? ----------------
+    // They pass every entry, K's too, before it is filled again: so each sees every
+    // phase of its barrier.
+    const int half = warp - 10;
+    int st = 0;
+    uint32_t par = 0;
+    bool stop = false;
+    for (bool going = true; going && !stop; going = !stop && paged_advance(p, tt, kKT, kExtra, w)) {
+      const PagedSegment seg = paged_segment(w, kExtra);
+      // as the streams: the first row's slots
+      const int lim0 = p.causal ? max(w.len - w.n + w.tile * tt + 1, 0) : w.len;
+      for (int t = seg.first; t < seg.last && !stop; ++t) {
+        const bool look = kLookAll || t * kKT + kKT > lim0;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!__all_sync(0xffffffffu, mbar_wait_or(full + 8 * st, par, abort_flag))) {
+            stop = true;
+            fail();
+            break;
+          }
+          if (kv == 1 && look) {
+            const uint4* v = reinterpret_cast<const uint4*>(ring + st * G::kTileBytes + half * (G::kTileBytes / 2)) + lane;
+            uint4 z = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 8
+            for (int y = 0; y < G::kTileBytes / 1024; ++y) {
+              const uint4 a = v[32 * y];
+              z.x = times_zero<T>(a.x, z.x);
+              z.y = times_zero<T>(a.y, z.y);
+              z.z = times_zero<T>(a.z, z.z);
+              z.w = times_zero<T>(a.w, z.w);
+            }
+            const bool found = __any_sync(0xffffffffu, odd_bits<T>(z.x | z.y | z.z | z.w) != 0);
+            if (lane == 0) odd_half[2 * st + half] = found;
+          }
+          if (lane == 0) {
+            mbar_arrive(seen + 8 * st);
+            mbar_arrive(empty + 8 * st);
+          }
+          __syncwarp();
+          if (++st == G::kStages) {
+            st = 0;
+            par ^= 1u;
+          }
         }
       }
     }

@@ -27,7 +27,7 @@ def _check(c, causal=True):
 
 
 @pytest.mark.parametrize("dtype,d", KINDS)
-@pytest.mark.parametrize("q_len", [1, 3])
+@pytest.mark.parametrize("q_len", [1, 3, 200])
 @pytest.mark.parametrize("sharp", [1.0, 5.0])
 def test_infinite_values(dtype, d, q_len, sharp):
     """Weights down to some 2^-60 of a row's largest: of every infinite value a part, and no
@@ -70,4 +70,16 @@ def test_slot_weights_beside_an_infinite_key(dtype, d, h_q, h_kv, q_lens):
     err = (c["w"].double() - w0 - add).abs()
     assert (err <= 3e-5 * add + 2.0 ** -23 * (w0 + add)).all()
     _check(c)
+    ssa.check_errors()
+
+
+@pytest.mark.parametrize("dtype,d", KINDS)
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+def test_many_items_with_infinite_values_past_their_lengths(dtype, d, fill):
+    """Several items on every CTA: tiles that hold such values, hidden, and tiles without them
+    take turns."""
+    lens = [130 + 37 * s % 500 for s in range(48)]
+    c = make(lens, [1 + 11 * s % 40 for s in range(48)], 8, 8, d, 64, dtype, seed=d, fill=fill)
+    _check(c)
+    _check(c, causal=False)
     ssa.check_errors()
