@@ -15,7 +15,8 @@ other lengths.
 The reference keeps no cache.  These ops are exact attention for what runs
 next to its sparse attention: dense layers, prompts too short to route, and
 caches that must not grow (:func:`paged_evict`).  They serve; they have no
-gradient.
+gradient: a backward pass that reaches :func:`paged_attention` raises, and what was
+appended is cut off from its history.
 
 Errors in the data (a page number outside the cache, lengths that do not fit)
 are found on the device and raised by a later op call or by
@@ -189,6 +190,28 @@ def paged_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pages: torch.Tensor
     _call(key, sync, L.lib().ssa_paged_append, c, a)
 
 
+class _NoGradient(torch.autograd.Function):
+    """Hands a result on as one of its inputs' that fails where a gradient is asked of it."""
+
+    @staticmethod
+    def forward(ctx, result, *inputs):
+        ctx.mark_dirty(result)
+        return result
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("paged_attention has no gradient (it serves): train with sparse_exact_attention or "
+                           "dense_attention, or run it under torch.no_grad()")
+
+
+def _results(q, k_pages, v_pages, out, lse):
+    """What paged_attention returns (``lse`` None: not asked for)."""
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        out = _NoGradient.apply(out, q, k_pages, v_pages)
+        lse = None if lse is None else _NoGradient.apply(lse, q, k_pages, v_pages)
+    return out if lse is None else (out, lse)
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                     q_starts: torch.Tensor, kv_lens: torch.Tensor, scale: Optional[float] = None,
                     is_causal: bool = True, weights: Optional[torch.Tensor] = None, return_lse: bool = False
@@ -212,7 +235,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Returns ``[T, h_q, d]`` in ``q``'s dtype (and ``[T, h_q]`` float32).  A row that
     sees no slot gets zeros (and ``-inf``).  Rows outside ``q_starts`` are not
-    written.
+    written.  There is no gradient: a backward pass through the results raises
+    ``RuntimeError``.
     """
     if k_pages.is_cuda:
         key = k_pages.get_device()
@@ -225,7 +249,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             if done is not None:
                 code, out, lse = done
                 _finish(key, sync, "ssa_paged_attn", code)
-                return (out, lse) if return_lse else out
+                return _results(q, k_pages, v_pages, out, lse)
     key, c, sync, keep = _cache_args(k_pages, v_pages, page_table, kv_lens, weights, _ATTEND)
     shape = q.shape
     q = _check_rows(q, "q", key, k_pages.dtype, shape)
@@ -247,7 +271,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     with ws.launching:
         code = _launch(key, lib.ssa_paged_attn, c, a, ws.buffer.data_ptr(), nbytes)
     _finish(key, sync, "ssa_paged_attn", code)
-    return (out, lse) if return_lse else out
+    return _results(q, k_pages, v_pages, out, lse)
 
 
 def _check_budget(budget: int, recent: int) -> None:
