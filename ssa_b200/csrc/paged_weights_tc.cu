@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) weights_tc_kernel(const __grid_co
         const int tokens = min(tt, w.n - tile * tt);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          z[e] = row_tok[e] < tokens ? __ldg(p.lse2 + (tok + row_tok[e]) * h_q + head * g + row_head[e]) : INFINITY;
+          z[e] = row_tok[e] < tokens ? __ldcg(p.lse2 + (tok + row_tok[e]) * h_q + head * g + row_head[e]) : INFINITY;
       };
       fetch(seg.first);
       for (int r = seg.first; r < seg.last; ++r, ++t) {

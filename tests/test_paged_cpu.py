@@ -4,6 +4,7 @@ ABI before any launch, and the refusals of the Python ops."""
 import ctypes
 import math
 import os
+import re
 import subprocess
 import sys
 
@@ -142,3 +143,14 @@ for dtype in (L.SSA_F32, L.SSA_BF16, L.SSA_F16):
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
     assert r.returncode == 0, (r.returncode, r.stderr)
+
+
+def test_dependent_kernels_do_not_read_results_through_the_read_only_cache():
+    """They start while the kernel before them writes, and __ldg is for what nothing writes
+    while the reader runs."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ssa_b200", "csrc")
+    for name in sorted(os.listdir(csrc)):
+        if name.startswith("paged"):
+            with open(os.path.join(csrc, name)) as f:
+                found = re.findall(r"__ldg\(\s*(?:\w+\.)*(?:lse2|lse|part|split|scores|kept)\b", f.read())
+            assert not found, (name, found)
