@@ -482,6 +482,12 @@ int simt_resident(int rows, int d) {
   return 2 * (one + 2048) <= 228 * 1024 ? 2 : 1;       // with what a CTA takes besides
 }
 
+// Kept scores take as much as the table could hold, whatever is filled: with wide
+// tables (131072 slots, 32 heads: 17 MB a row) more than a serving cache leaves free.
+// Beyond this they are made again for the weights, which takes twice the time of
+// the call (32 tokens x 32 heads over 8192 slots: 195 us kept, 418 made again).
+constexpr size_t kMostScores = static_cast<size_t>(4) << 30;
+
 // The kernel that serves a call, its tile rows and grid, and the workspace.
 enum class AttnKernel { kSimt, kTokens, kChunks };
 struct AttnPlan {
@@ -515,7 +521,10 @@ AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {
   a.lse2 = a.split + up(a.grid * sizeof(PagedSplit));
   a.scores = a.lse2 + (p.c.w ? up(lines * 4) : 0);
   a.total = a.scores;
-  if (p.c.w && a.rows == 16) a.total += up(lines * score_stride(p.c) * 4);
+  if (p.c.w && a.rows == 16) {
+    const size_t bytes = lines * score_stride(p.c) * 4;
+    if (bytes <= kMostScores) a.total += up(bytes);
+  }
   return a;
 }
 
@@ -552,7 +561,7 @@ cudaError_t launch_paged_attn(PagedAttnParams p, ssa_dtype dt, void* ws, cudaStr
   }
   if (e != cudaSuccess || !p.c.w) return e;
   if (p.scores) return launch_paged_weights_dec(p, st);
-  if (a.kernel == AttnKernel::kChunks && paged_weights_tc_supported(p, dt)) return launch_paged_weights_tc(p, dt, st);
+  if (a.kernel != AttnKernel::kSimt && paged_weights_tc_supported(p, dt)) return launch_paged_weights_tc(p, dt, st);
   return launch_weights_simt(p, dt, st);
 }
 

@@ -145,6 +145,16 @@ for dtype in (L.SSA_F32, L.SSA_BF16, L.SSA_F16):
     assert r.returncode == 0, (r.returncode, r.stderr)
 
 
+@pytest.mark.parametrize("dtype,d", [(L.SSA_BF16, 128), (L.SSA_F16, 64), (L.SSA_F32, 64), (L.SSA_BF16, 96)])
+def test_workspace_of_weights_with_wide_tables(lib, dtype, d):
+    """The kept scores of single tokens follow the table's width: they are bounded."""
+    c = _cache(batch=4096, max_pages=2048, page_size=64, h_kv=8, d=d, dtype=dtype, weights=0x8000,
+               num_pages=8, k_stride_p=64 * 8 * d, k_stride_n=8 * d, k_stride_h=d, v_stride_p=64 * 8 * d,
+               v_stride_n=8 * d, v_stride_h=d, table_stride=2048)
+    a = _attn(rows=4096, h_q=32, q_stride_n=32 * d, q_stride_h=d, out_stride_n=32 * d, out_stride_h=d)
+    assert 0 < lib.ssa_paged_attn_workspace_size(ctypes.byref(c), ctypes.byref(a)) < 4.1 * 2 ** 30, lib.ssa_last_error()
+
+
 def test_dependent_kernels_do_not_read_results_through_the_read_only_cache():
     """They start while the kernel before them writes, and __ldg is for what nothing writes
     while the reader runs."""
