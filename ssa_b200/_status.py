@@ -175,7 +175,7 @@ def _poll_words(key: int) -> None:
     """Raises for one kind of error of one op, and leaves the others for the next time:
     timeouts first, since they leave the workspaces' heads undefined."""
     w = _words.get(key)
-    if w is None:
+    if w is None or not (w.low.value or w.high.value):
         return
     _clear_unchecked(w)
     for bits, error in _PAGED_ERRORS:
