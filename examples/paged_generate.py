@@ -104,9 +104,14 @@ def main():
     p.add_argument("--budget", type=int, default=0, help="cached slots per KV head a sequence may keep (0: all)")
     p.add_argument("--recent", type=int, default=32)
     args = p.parse_args()
+    lengths = [int(n) for n in args.prompts.split(",")]
+    if min(lengths) < 1 or args.new < 1 or args.chunk < 1:
+        p.error("prompts, --new and --chunk: at least one token each")
+    if args.budget and not 0 <= args.recent <= args.budget:
+        p.error("--recent must be within --budget")
     torch.manual_seed(0)
     model = Decoder(args.layers).cuda()
-    prompts = [torch.randint(0, 512, (int(n),)) for n in args.prompts.split(",")]
+    prompts = [torch.randint(0, 512, (n,)) for n in lengths]
     seqs, last, cache = serve(model, prompts, args.new, args.chunk, args.budget, args.recent)
     ssa.check_errors()
     for i, (prompt, seq) in enumerate(zip(prompts, seqs)):
