@@ -69,8 +69,9 @@ typedef enum {
 #define SSA_DEVICE_BAD_PAGE 0x10   /* paged cache: a page table entry of a used slot is
                                       outside [0, num_pages); the slot is not written,
                                       and what is computed from it is undefined       */
-#define SSA_DEVICE_TIMEOUT 0x100   /* route: a pipeline wait gave up (~1 s); the
-                                      affected codes are undefined                  */
+#define SSA_DEVICE_TIMEOUT 0x100   /* route, paged cache: a pipeline wait gave up
+                                      (~1 s); the affected codes or results are
+                                      undefined                                     */
 #define SSA_DEVICE_BAD_LENGTH 0x10000 /* paged cache: q_starts does not ascend within
                                       [0, rows], a length is outside its table, or more
                                       rows are appended than the sequence holds; the

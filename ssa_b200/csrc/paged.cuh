@@ -153,9 +153,10 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedCacheParams& c, const i
   return r;
 }
 
-// sum_{i < n} floor((a i + b) / m) for m > 0 and a n + b < 2^32, by the Euclidean
-// reduction of lattice points under a line (32-bit divisions: every CTA starts
-// with a few of these).
+// sum_{i < n} floor((a i + b) / m) for m > 0 and a n + b < 2^32: the lattice points
+// under a line, whole parts taken out and the axes exchanged in turn as in Euclid's
+// algorithm (the reciprocity of floor sums: Graham, Knuth, Patashnik, Concrete
+// Mathematics, section 3.5; 32-bit divisions: every CTA starts with a few of these).
 __host__ __device__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   int64_t ans = 0;
   while (n > 0) {

@@ -499,7 +499,8 @@ struct AttnPlan {
 // More than 16 rows (new tokens x heads of a group) per sequence on average
 // take tiles of many rows; 16-bit caches that page tiles fit, the tensor cores
 // (24 x 5 tokens over 8000 slots, four heads a group: 167 us, and 249 with tiles of
-// 16 rows; one such sequence over 2000: 18.0 and 15.8).
+// 16 rows; one such sequence over 2000: 18.0 and 15.8).  Both are measured for equal
+// sequences: many single tokens beside one chunk may take either.
 // On the CUDA cores a tile costs its rows whether they are used or not, and a
 // row of a 32-row tile about 5/4 of one of a 64-row tile.
 AttnPlan attn_plan(const PagedAttnParams& p, ssa_dtype dt) {

@@ -11,7 +11,7 @@
 // a tile are a few hundred clocks against about 1400 to fetch its 32 KB at
 // d = 128.  (One group of four warps was 8% slower, bound by its own steps; a
 // ring of 96 KB is as fast as one of 192 KB.)  32 tokens x 32 heads over 8192
-// slots each, bf16: 1.07 GB in 172 us, 6.2 TB/s.  One token over 1024 slots:
+// slots each, bf16: 1.07 GB in 174 us, 6.2 TB/s.  One token over 1024 slots:
 // 12 us, all of it latency.
 //
 // P enters the product with V as two 16-bit terms (p = hi + lo, off by 2^-17),

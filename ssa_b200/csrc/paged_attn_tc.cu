@@ -10,10 +10,11 @@
 // tile costs them 4 * 128 * 128 * d flops and the MUFU 128 * 128 exponentials,
 // about 1000 clocks each at d = 128.  Neither bounds it (each is busy 48% of the
 // time): a stream's softmax, 2100 clocks, and the two products of its next tile
-// follow one another.  2048 tokens x 32 heads over 32768 slots, bf16: 978 us,
-// 1.09 PFLOP/s.  Slower on that call: tiles of 64 slots with two S buffers each
-// (1349 us), two threads a row (1148), a quarter of the exponentials as
-// polynomials (2%).
+// follow one another.  2048 tokens x 32 heads over 32768 slots, bf16: 1154 us a
+// call, 0.92 PFLOP/s (1022 in a replayed graph; it runs at the power limit, and a tenth
+// more or less from box to box).  Slower on that call, beside 978 us in the same run:
+// tiles of 64 slots with two S buffers each (1349), two threads a row (1148), a quarter
+// of the exponentials as polynomials (2%).
 //
 //   warps 0-3   stream A: loads its Q rows, softmax, epilogue (a row per thread)
 //   warps 4-7   stream B
@@ -27,7 +28,9 @@
 // tile exceeds it by more than 2^8 (O, in TMEM, is then multiplied by the
 // quotient): exponentials stay below 2^8, sums in fp32.  P is rounded to the
 // input type, as the tensor cores take it (relative error at most 2^-8 / 2^-11 of
-// each weight); the row sum adds the unrounded values.  For fp16 every exponential
+// each weight); the row sum adds the unrounded values.  (P in two terms, as for single
+// tokens, lengthens the chain by the split and by a second product: 1040 -> 1490 us on
+// the call above, 311 -> 402 for 24 mixed sequences.)  For fp16 every exponential
 // carries a factor 2^7, so that weights down to 2^-21 of the largest stay
 // normal numbers.
 //

@@ -14,7 +14,7 @@
 // Per row tile and stream the tensor cores do 128 x 128 x d products, the MUFU
 // 128 x 128 exponentials, which bound it (1024 clocks against 512 at d = 128);
 // a quarter of them is made on the FMA pipe instead (4% faster; a half, no more).
-// 2 x 1024 tokens x 32 heads over 8192 slots, bf16: 218 us, 590 TFLOP/s (whole
+// 2 x 1024 tokens x 32 heads over 8192 slots, bf16: 225 us, 570 TFLOP/s (whole
 // items in turn: 235; 4 x 1618 tokens x 8 heads of 64 over 3529: 12% of the call
 // gained; items of two row tiles lose 5% by the join).  Two threads a slot (16
 // warps) took the same time.

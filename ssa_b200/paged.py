@@ -237,6 +237,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     sees no slot gets zeros (and ``-inf``).  Rows outside ``q_starts`` are not
     written.  There is no gradient: a backward pass through the results raises
     ``RuntimeError``.
+
+    Sums and statistics are float32.  A 16-bit call of more than 16 rows (new rows x
+    heads of a group) per sequence on average holds the softmax weights in ``q``'s
+    dtype for their product with the values, smaller calls in two such terms: so a
+    row's last bits can differ with what else is in its batch.  Threads that share a
+    stream take turns to launch.
     """
     if k_pages.is_cuda:
         key = k_pages.get_device()
